@@ -73,6 +73,8 @@ MODULES: Dict[str, str] = {
     "gemm_tcgen05": "gemm_tcgen05.cu",
     "gemm_f32_parts": "gemm_f32_parts.cu",
     "attention_fast": "attention_fast.cu",
+    "attention_shared": "attention_shared.cu",
+    "logit_shaping": "logit_shaping.cu",
     "gemm_tcgen05_static": "gemm_tcgen05_static.cu",
     "diagnostics": "diagnostics.cu",
 }
@@ -80,7 +82,8 @@ MODULES: Dict[str, str] = {
 _HEADERS = ["common.cuh"]
 # further files a module's source includes (they take part in its hash)
 _INCLUDES: Dict[str, List[str]] = {
-    "attention_fast.cu": ["tma_util.cuh"],
+    "attention_fast.cu": ["attention_common.cuh", "tma_util.cuh"],
+    "attention_shared.cu": ["attention_common.cuh", "tma_util.cuh"],
     "mixed_head_prompt.cu": ["tma_util.cuh"],
     "gemm_tcgen05.cu": ["tma_util.cuh"],
     "gemm_f32_parts.cu": ["tma_util.cuh"],

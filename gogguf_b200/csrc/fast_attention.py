@@ -2,12 +2,13 @@
 decode kernel (every sequence brings one token) and the prefill kernel, scratch for the splits."""
 from __future__ import annotations
 
-from typing import Callable, Optional
+from typing import Callable, List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from . import kernels as K
-from .build import kernel, module, stream_ptr
+from .build import KernelError, kernel, module, stream_ptr
 
 
 def decode_splits(n_tokens: int, nkv: int, max_ctx: int) -> int:
@@ -49,6 +50,155 @@ def attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page
         positions.data_ptr(), seq_of_token.data_ptr(), table.data_ptr(), table.shape[-1], page_size,
         k_pool.shape[0], n_tokens, nq, nkv, d, d if dv is None else int(dv), float(scale), int(window), int(chunk), int(splits),
         int(bool(cluster)), sink.data_ptr() if sink is not None else 0, float(out_scale), *_gate(gate),
+        status_word(q.device).data_ptr(), stream_ptr())
+
+
+PREFIX_CTAS = 296       # of the kernel over the prefixes (csrc/attention_shared.cu)
+
+
+def shared_scratch(n_tokens: int, nq: int, nkv: int, dv: int) -> int:
+    """Floats of scratch that `attn_decode_shared` needs: the parts' rows, and two numbers beside each."""
+    if n_tokens <= 0 or nkv <= 0 or nq <= 0 or nq % nkv or dv <= 0:
+        raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {dv}, {n_tokens} tokens")
+    return (nq * n_tokens + 128 * PREFIX_CTAS) * (dv + 2)
+
+
+def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[int], int]]:
+    """The rows of a page table that read the same leading pages: [(rows, pages)], each with two rows and one page at least.
+    `limits[r]`: how many leading pages of row r may be shared (those that lie wholly before its newest position).  A row is
+    in one group at most: where some rows of a group share more pages than all of it, the cut that saves more reads is taken."""
+    table = np.asarray(table)
+
+    def best(rows: List[int], depth: int) -> Tuple[int, List[Tuple[List[int], int]]]:
+        if len(rows) < 2:
+            return 0, []
+        most = min(limits[r] for r in rows)
+        part = table[rows, depth:most]
+        differs = np.nonzero((part != part[0]).any(axis=0))[0]
+        common = depth + int(differs[0]) if differs.size else most
+        whole = (len(rows) - 1) * common, ([(rows, common)] if common else [])
+        below = {}
+        for r in rows:
+            if limits[r] > common:
+                below.setdefault(int(table[r, common]), []).append(r)
+        saved, groups = 0, []
+        for members in below.values():
+            s, g = best(members, common + 1)
+            saved, groups = saved + s, groups + g
+        return (saved, groups) if saved > whole[0] else whole
+
+    roots = {}
+    for r, n in enumerate(limits):
+        if n > 0:
+            roots.setdefault(int(table[r, 0]), []).append(r)
+    return [g for rows in roots.values() for g in best(rows, 1)[1]]
+
+
+class PrefixPlan:
+    """Which token rows of a decode step read which prefix together, as `attn_decode_shared` takes it: `groups` is a list of
+    (token rows, leading pages that are the same in all their sequences).  Every shared page must lie wholly before its rows'
+    own positions.  A plan serves all layers of a step that read through the same page table."""
+
+    def __init__(self, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, device):
+        host = torch.empty(5 + 5 * n_tokens, dtype=torch.int32)
+        self.pack(groups, n_tokens, host.numpy())
+        self.n_tokens = n_tokens
+        self.words = host.to(device)
+
+    @staticmethod
+    def words_for(n_tokens: int) -> int:
+        return 5 + 5 * n_tokens
+
+    @classmethod
+    def over(cls, words: torch.Tensor, n_tokens: int) -> "PrefixPlan":
+        """A plan whose words are (or will be) on the device already, packed by `pack`."""
+        plan = cls.__new__(cls)
+        if words.dtype != torch.int32 or words.numel() != cls.words_for(n_tokens) or not words.is_contiguous():
+            raise KernelError(f"shared attention: a plan of {n_tokens} tokens has {cls.words_for(n_tokens)} int32 words")
+        plan.n_tokens, plan.words = n_tokens, words
+        return plan
+
+    @classmethod
+    def pack(cls, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, out: np.ndarray) -> None:
+        """Write the plan's words (csrc/attention_common.cuh: AttnShared) to `out`; refuses rows that are not the step's, that
+        appear twice, and groups without a row or page."""
+        if n_tokens <= 0:
+            raise KernelError("shared attention: a plan needs at least one token row")
+        first, pages = out[4:5 + n_tokens], out[5 + n_tokens:5 + 2 * n_tokens]
+        rows, group_of, member_of = (out[5 + k * n_tokens:5 + (k + 1) * n_tokens] for k in (2, 3, 4))
+        group_of[:] = -1
+        first[0] = at = 0
+        for g, (members, shared) in enumerate(groups):
+            members = list(members)
+            if not members or shared <= 0:
+                raise KernelError("shared attention: a group has at least one row and one page")
+            if min(members) < 0 or max(members) >= n_tokens or len(set(members)) != len(members) or (group_of[members] >= 0).any():
+                raise KernelError(f"shared attention: rows {members} are not rows of {n_tokens} tokens, or appear twice")
+            first[g], pages[g] = at, shared
+            rows[at:at + len(members)] = members
+            group_of[members] = g
+            member_of[members] = np.arange(len(members))
+            at += len(members)
+            first[g + 1] = at
+        out[:4] = (len(groups), 0, 0, 0)
+
+    @classmethod
+    def of_pages(cls, pages: Sequence[Sequence[int]], lengths: Sequence[int], page_size: int, device) -> "PrefixPlan":
+        """The plan of a step with one token per sequence: `pages[r]` lists the pages of row r's sequence, `lengths[r]` is its
+        length with the new token."""
+        if len(pages) != len(lengths):
+            raise KernelError(f"shared attention: {len(pages)} page lists and {len(lengths)} lengths")
+        if not pages:
+            raise KernelError("shared attention: a plan needs at least one token row")
+        for r, (p, n) in enumerate(zip(pages, lengths)):
+            if n < 0 or len(p) * page_size < n:
+                raise KernelError(f"shared attention: row {r} has {n} positions in {len(p)} pages of {page_size}")
+        table = np.full((len(pages), max(1, max(len(p) for p in pages))), -1, dtype=np.int64)
+        for r, p in enumerate(pages):
+            table[r, :len(p)] = p
+        return cls(shared_groups(table, [max(0, (n - 1) // page_size) for n in lengths]), len(pages), device)
+
+
+def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, page_size, plan: PrefixPlan, scratch, nq, nkv, d, scale,
+                       sink=None, out_scale: float = 1.0, dv: Optional[int] = None, gate=None, splits: Optional[int] = None) -> None:
+    """Decode attention (`attn_decode_tma`, without windows and chunks) of the plan's token rows: the keys and values of a
+    prefix that several rows share are read once for all of them, in two kernels.  scratch: float32, `shared_scratch` of it;
+    two launches that may run at the same time need scratch of their own.  splits (1, 2, 4, 8): CTAs that share a row's own pages."""
+    from .tcgen05_gemm import status_word
+    dv = d if dv is None else int(dv)
+    T = plan.n_tokens
+    if not takes(nq, nkv, d, dv):
+        raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {d} and {dv} are outside what the kernels take")
+    here = torch.cuda.current_device() if q.is_cuda else -1
+    for t, what in ((q, "q"), (k_pool, "k_pool"), (v_pool, "v_pool"), (out, "out"), (positions, "positions"), (seq_of_token, "seq_of_token"),
+                    (table, "table"), (plan.words, "plan"), (scratch, "scratch")) + (((sink, "sink"),) if sink is not None else ()) + \
+            (((gate, "gate"),) if gate is not None else ()):
+        if not t.is_cuda or t.device.index != here:
+            raise KernelError(f"shared attention: {what} is on {t.device}, not on the current CUDA device")
+        if what != "gate" and not t.is_contiguous():
+            raise KernelError(f"shared attention: {what} must be contiguous")
+    for t, what in ((q, "q"), (k_pool, "k_pool"), (v_pool, "v_pool"), (out, "out")):
+        if t.dtype != torch.bfloat16:
+            raise KernelError(f"shared attention: {what} must be torch.bfloat16, got {t.dtype}")
+    for t, what in ((positions, "positions"), (seq_of_token, "seq_of_token"), (table, "table")):
+        if t.dtype != torch.int32:
+            raise KernelError(f"shared attention: {what} must be torch.int32, got {t.dtype}")
+    if scratch.dtype != torch.float32 or scratch.numel() < shared_scratch(T, nq, nkv, dv):
+        raise KernelError(f"shared attention: scratch must be float32 with {shared_scratch(T, nq, nkv, dv)} elements")
+    if (q.numel() < T * nq * d or out.numel() < T * nq * dv or positions.numel() < T or seq_of_token.numel() < T or table.dim() != 2
+            or k_pool.dim() != 4 or tuple(k_pool.shape[1:]) != (nkv, page_size, d)
+            or tuple(v_pool.shape) != (k_pool.shape[0], nkv, page_size, dv)):
+        raise KernelError("shared attention: shapes disagree")
+    if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nq):
+        raise KernelError(f"shared attention: a sink is float32 with {nq} elements")
+    if gate is not None and (gate.dtype != torch.bfloat16 or gate.dim() != 2 or gate.shape[0] < T or gate.shape[1] < nq * dv or gate.stride(1) != 1):
+        raise KernelError(f"shared attention: a gate is bfloat16 with {T} rows of {nq * dv}")
+    if splits is None:
+        splits = min(8, decode_tma_splits(T, nkv, table.shape[1] * page_size, cluster=True))
+    kernel("attention_shared", "gg_attn_decode_shared")(
+        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(),
+        table.data_ptr(), table.shape[1], page_size, k_pool.shape[0], plan.words.data_ptr(), T, nq, nkv, d, dv, float(scale), int(splits),
+        sink.data_ptr() if sink is not None else 0, float(out_scale), *_gate(gate), scratch.data_ptr(), scratch.numel(),
         status_word(q.device).data_ptr(), stream_ptr())
 
 

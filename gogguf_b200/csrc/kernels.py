@@ -7,6 +7,7 @@ tensor that is not on a CUDA device, or a missing compiler, raises.
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 from operator import index
 from typing import List, Optional, Sequence, Tuple
@@ -1420,6 +1421,82 @@ def history_append(tokens: torch.Tensor, ring_rows: torch.Tensor, hist: torch.Te
         _need(t, torch.int32, n)
     kernel("sampling", "gg_history_append")(_p(tokens), _p(ring_rows), _p(hist), _p(hist_len), _p(hist_pos),
                                              hist.shape[1], rows, _stream())
+
+
+def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, hist: Optional[torch.Tensor] = None,
+                 hist_len: Optional[torch.Tensor] = None, ring_rows: Optional[torch.Tensor] = None, repeat: float = 1.0,
+                 frequency: float = 0.0, presence: float = 0.0, bias=None, masks: Optional[torch.Tensor] = None,
+                 mask_rows: Optional[torch.Tensor] = None, rows: Optional[int] = None) -> torch.Tensor:
+    """Penalties, biases and a mask of allowed ids on `rows` (default: all) rows of float32 logits, into `out` (default: in
+    place).  With c the number of times id v stands among the hist_len[q] ids of hist[q]:
+    z = x / repeat (x > 0) or x * repeat, then z -= frequency * c + presence, where c > 0; z += bias of v; -inf where masks
+    does not allow v.  q = ring_rows[r] (default: r) names row r's request: `hist` [requests, n] and `hist_len` (int32) its last
+    ids (ids outside the vocabulary count for nothing); `bias` = (start [requests + 1], ids, values): its biases are
+    the entries start[q]..start[q + 1] - 1 (of an id that is listed twice the last one counts); `masks` [states, words >= V / 32]
+    int32, bit v % 32 of word v / 32 set where id v is allowed, of which it takes row mask_rows[q] (negative: everything is
+    allowed; beyond the table: nothing is)."""
+    if out is None:
+        out = logits
+    for t, what in ((logits, "logits"), (out, "out")):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise KernelError(f"shape_logits: {what} must be float32 rows")
+    R, V = logits.shape[0] if rows is None else int(rows), logits.shape[1]
+    if R < 0 or R > logits.shape[0] or out.shape[0] < R or out.shape[1] != V:
+        raise KernelError(f"shape_logits: {R} rows of logits {tuple(logits.shape)} into {tuple(out.shape)}")
+    if R == 0 or V == 0:
+        return out
+    ld, ldo = (logits.stride(0), out.stride(0)) if R > 1 else (V, V)
+    if logits.data_ptr() != out.data_ptr() or ld != ldo:
+        a, b = logits.data_ptr(), out.data_ptr()
+        if a < b + 4 * ((R - 1) * ldo + V) and b < a + 4 * ((R - 1) * ld + V):
+            raise KernelError("shape_logits: out is neither the logits nor apart from them")
+    if not (repeat > 0 and math.isfinite(repeat) and math.isfinite(frequency) and math.isfinite(presence)):
+        raise KernelError("shape_logits: repeat must be positive, and it, frequency and presence finite")
+    if (hist is None) != (hist_len is None) or (masks is None) != (mask_rows is None):
+        raise KernelError("shape_logits: hist goes with hist_len, masks with mask_rows")
+    if ring_rows is not None:
+        _need(ring_rows, torch.int32, "ring_rows")
+        if ring_rows.numel() < R:
+            raise KernelError(f"shape_logits: {ring_rows.numel()} ring_rows for {R} rows")
+    requests = []
+    if hist is not None:
+        _need(hist, torch.int32, "hist")
+        _need(hist_len, torch.int32, "hist_len")
+        if hist.dim() != 2 or hist_len.numel() != hist.shape[0]:
+            raise KernelError("shape_logits: hist and hist_len disagree")
+        requests.append(hist.shape[0])
+        if hist.shape[1] == 0:
+            hist = hist_len = None
+    start = ids = values = None
+    if bias is not None:
+        start, ids, values = bias
+        _need(start, torch.int32, "bias start")
+        _need(ids, torch.int32, "bias ids")
+        _need(values, torch.float32, "bias values")
+        if start.numel() < 2 or ids.numel() != values.numel():
+            raise KernelError("shape_logits: bias ids and values disagree")
+        requests.append(start.numel() - 1)
+        if ids.numel() == 0:
+            start = ids = values = None
+    if masks is not None:
+        _need(masks, torch.int32, "masks")
+        _need(mask_rows, torch.int32, "mask_rows")
+        if masks.dim() != 2 or masks.shape[0] == 0 or masks.shape[1] * 32 < V:
+            raise KernelError(f"shape_logits: masks {tuple(masks.shape)} do not cover {V} ids")
+        requests.append(mask_rows.numel())
+    if len(set(requests)) > 1 or (ring_rows is None and requests and requests[0] < R):
+        raise KernelError(f"shape_logits: {R} rows, and requests by their parts: {requests}")
+    if not logits.is_cuda:
+        raise KernelError("kernel argument is not on a CUDA device (there is no CPU path)")
+    for t in (logits, out, hist, hist_len, ring_rows, start, ids, values, masks, mask_rows):
+        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
+            raise KernelError(f"shape_logits: a tensor is on {t.device}, not on the current CUDA device")
+    kernel("logit_shaping", "gg_shape_logits")(
+        _p(logits), ld, _p(out), ldo, R, V, _p(ring_rows), requests[0] if requests else R, _p(hist), _p(hist_len),
+        hist.shape[1] if hist is not None else 0, float(repeat), float(frequency), float(presence), _p(start), _p(ids), _p(values),
+        ids.numel() if ids is not None else 0, _p(masks), _p(mask_rows), masks.shape[0] if masks is not None else 0,
+        masks.shape[1] if masks is not None else 0, _stream())
+    return out
 
 
 TOPK_MAX = 1024      # largest top-k the on-device chain takes (csrc/sampling.cu)

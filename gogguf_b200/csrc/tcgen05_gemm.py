@@ -32,16 +32,17 @@ def check_status(device: torch.device) -> None:
     v = int(t.item())
     if v != 0:
         t.zero_()
-        if 41 <= v <= 53:
+        if 41 <= v <= 54:
             who = {41: "attention_plain", 42: "attn_decode", 43: "attn_prefill", 44: "attn_decode_tma",
                    45: "attn_prefill_tc", 46: "qk_norm_rope_cache", 47: "qk_norm_rope_cache (16-byte form)",
                    48: "the q/k/v product's cache write", 49: "latent_prep", 50: "diff_qk_prep",
-                   51: "diff_attention", 52: "head_kv_prep", 53: "mixed_head_attention"}[v]
+                   51: "diff_attention", 52: "head_kv_prep", 53: "mixed_head_attention",
+                   54: "attn_decode_shared"}[v]
             raise KernelError(f"debug build: kernel {who} met a page-table index or page id out of range (code {v}); "
                               "it read page 0 (a reader) or wrote nothing (a writer), results of that step are invalid")
         raise KernelError(f"a bounded wait inside a kernel ran out (code {v}: 1 TMA producer, 2 MMA issuer, "
                           "3 epilogue of a product, 11-12 decode attention, 21-28 prefill attention, 61-68 prefill attention "
-                          "with mixed heads); "
+                          "with mixed heads, 71-79 a shared prefix); "
                           "results of that step are invalid")
 
 
