@@ -169,37 +169,40 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
     T = plan.n_tokens
     if not takes(nq, nkv, d, dv):
         raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {d} and {dv} are outside what the kernels take")
-    here = torch.cuda.current_device() if q.is_cuda else -1
-    for t, what in ((q, "q"), (k_pool, "k_pool"), (v_pool, "v_pool"), (out, "out"), (positions, "positions"), (seq_of_token, "seq_of_token"),
-                    (table, "table"), (plan.words, "plan"), (scratch, "scratch")) + (((sink, "sink"),) if sink is not None else ()) + \
-            (((gate, "gate"),) if gate is not None else ()):
-        if not t.is_cuda or t.device.index != here:
+    here = torch._C._cuda_getDevice() if q.is_cuda else -1
+
+    def need(t, dt, what):
+        if t.dtype != dt or not t.is_contiguous():
+            raise KernelError(f"shared attention: {what} must be contiguous {dt}, got {t.dtype}")
+        if here < 0 or t.get_device() != here:
             raise KernelError(f"shared attention: {what} is on {t.device}, not on the current CUDA device")
-        if what != "gate" and not t.is_contiguous():
-            raise KernelError(f"shared attention: {what} must be contiguous")
-    for t, what in ((q, "q"), (k_pool, "k_pool"), (v_pool, "v_pool"), (out, "out")):
-        if t.dtype != torch.bfloat16:
-            raise KernelError(f"shared attention: {what} must be torch.bfloat16, got {t.dtype}")
-    for t, what in ((positions, "positions"), (seq_of_token, "seq_of_token"), (table, "table")):
-        if t.dtype != torch.int32:
-            raise KernelError(f"shared attention: {what} must be torch.int32, got {t.dtype}")
-    if scratch.dtype != torch.float32 or scratch.numel() < shared_scratch(T, nq, nkv, dv):
-        raise KernelError(f"shared attention: scratch must be float32 with {shared_scratch(T, nq, nkv, dv)} elements")
+        return t.data_ptr()
+
+    bf16, i32 = torch.bfloat16, torch.int32
+    p_q, p_k, p_v, p_out = need(q, bf16, "q"), need(k_pool, bf16, "k_pool"), need(v_pool, bf16, "v_pool"), need(out, bf16, "out")
+    p_pos, p_seq, p_table = need(positions, i32, "positions"), need(seq_of_token, i32, "seq_of_token"), need(table, i32, "table")
+    p_plan, p_scratch = need(plan.words, i32, "plan"), need(scratch, torch.float32, "scratch")
+    room = shared_scratch(T, nq, nkv, dv)
+    if scratch.numel() < room:
+        raise KernelError(f"shared attention: scratch must have {room} elements")
     if (q.numel() < T * nq * d or out.numel() < T * nq * dv or positions.numel() < T or seq_of_token.numel() < T or table.dim() != 2
-            or k_pool.dim() != 4 or tuple(k_pool.shape[1:]) != (nkv, page_size, d)
-            or tuple(v_pool.shape) != (k_pool.shape[0], nkv, page_size, dv)):
+            or k_pool.shape != (k_pool.shape[0], nkv, page_size, d) or v_pool.shape != (k_pool.shape[0], nkv, page_size, dv)):
         raise KernelError("shared attention: shapes disagree")
-    if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nq):
-        raise KernelError(f"shared attention: a sink is float32 with {nq} elements")
-    if gate is not None and (gate.dtype != torch.bfloat16 or gate.dim() != 2 or gate.shape[0] < T or gate.shape[1] < nq * dv or gate.stride(1) != 1):
-        raise KernelError(f"shared attention: a gate is bfloat16 with {T} rows of {nq * dv}")
+    p_sink = p_gate = ldg = 0
+    if sink is not None:
+        p_sink = need(sink, torch.float32, "sink")
+        if sink.numel() != nq:
+            raise KernelError(f"shared attention: a sink has {nq} elements")
+    if gate is not None:
+        if (gate.dtype != bf16 or gate.dim() != 2 or gate.shape[0] < T or gate.shape[1] < nq * dv or gate.stride(1) != 1
+                or gate.get_device() != here):
+            raise KernelError(f"shared attention: a gate is bfloat16 with {T} rows of {nq * dv}, on the current CUDA device")
+        p_gate, ldg = gate.data_ptr(), gate.stride(0)
     if splits is None:
         splits = min(8, decode_tma_splits(T, nkv, table.shape[1] * page_size, cluster=True))
     kernel("attention_shared", "gg_attn_decode_shared")(
-        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(),
-        table.data_ptr(), table.shape[1], page_size, k_pool.shape[0], plan.words.data_ptr(), T, nq, nkv, d, dv, float(scale), int(splits),
-        sink.data_ptr() if sink is not None else 0, float(out_scale), *_gate(gate), scratch.data_ptr(), scratch.numel(),
-        status_word(q.device).data_ptr(), stream_ptr())
+        p_q, p_k, p_v, p_out, p_pos, p_seq, p_table, table.shape[1], page_size, k_pool.shape[0], p_plan, T, nq, nkv, d, dv, float(scale),
+        int(splits), p_sink, float(out_scale), p_gate, ldg, p_scratch, scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
 
 
 def attn_prefill(q, k_pool, v_pool, out, cu_seqlens, ctx_lens, seq_of_token, table, page_size, n_seqs,

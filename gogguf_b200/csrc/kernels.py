@@ -1437,65 +1437,72 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, hi
     allowed; beyond the table: nothing is)."""
     if out is None:
         out = logits
-    for t, what in ((logits, "logits"), (out, "out")):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-            raise KernelError(f"shape_logits: {what} must be float32 rows")
-    R, V = logits.shape[0] if rows is None else int(rows), logits.shape[1]
-    if R < 0 or R > logits.shape[0] or out.shape[0] < R or out.shape[1] != V:
+    here = torch._C._cuda_getDevice() if logits.is_cuda else -1
+
+    def need(t, dt, what):
+        if t.dtype != dt or not t.is_contiguous() or t.get_device() != here:
+            raise KernelError(f"shape_logits: {what} must be contiguous {dt} on the logits' device, got {t.dtype} on {t.device}")
+        return t.data_ptr()
+
+    (have, V), (ld, one) = logits.shape, logits.stride()
+    R = have if rows is None else index(rows)
+    ldo = out.stride(0)
+    if logits.dtype != torch.float32 or out.dtype != torch.float32 or one != 1 or out.stride(1) != 1:
+        raise KernelError("shape_logits: logits and out must be float32 rows")
+    if R < 0 or R > have or out.shape[0] < R or out.shape[1] != V or (R > 1 and (ld < V or ldo < V)):
         raise KernelError(f"shape_logits: {R} rows of logits {tuple(logits.shape)} into {tuple(out.shape)}")
-    if R == 0 or V == 0:
-        return out
-    ld, ldo = (logits.stride(0), out.stride(0)) if R > 1 else (V, V)
-    if logits.data_ptr() != out.data_ptr() or ld != ldo:
-        a, b = logits.data_ptr(), out.data_ptr()
-        if a < b + 4 * ((R - 1) * ldo + V) and b < a + 4 * ((R - 1) * ld + V):
-            raise KernelError("shape_logits: out is neither the logits nor apart from them")
-    if not (repeat > 0 and math.isfinite(repeat) and math.isfinite(frequency) and math.isfinite(presence)):
+    if not (0 < repeat < math.inf and -math.inf < frequency < math.inf and -math.inf < presence < math.inf):
         raise KernelError("shape_logits: repeat must be positive, and it, frequency and presence finite")
     if (hist is None) != (hist_len is None) or (masks is None) != (mask_rows is None):
         raise KernelError("shape_logits: hist goes with hist_len, masks with mask_rows")
+    if R == 0 or V == 0:
+        return out
+    if R == 1:
+        ld = ldo = V
+    a, b = logits.data_ptr(), out.data_ptr()
+    if (a != b or ld != ldo) and a < b + 4 * ((R - 1) * ldo + V) and b < a + 4 * ((R - 1) * ld + V):
+        raise KernelError("shape_logits: out is neither the logits nor apart from them")
+    p_ring = p_hist = p_len = p_start = p_ids = p_values = p_masks = p_mask_rows = 0
+    last_n = n_biases = states = words = 0
+    requests = -1                                # the parts' number of requests
+
+    def agree(n, what):
+        if n != requests and requests >= 0 or (ring_rows is None and n < R):
+            raise KernelError(f"shape_logits: {what} is for {n} requests, other parts for {requests}, and there are {R} rows")
+        return n
+
     if ring_rows is not None:
-        _need(ring_rows, torch.int32, "ring_rows")
+        p_ring = need(ring_rows, torch.int32, "ring_rows")
         if ring_rows.numel() < R:
             raise KernelError(f"shape_logits: {ring_rows.numel()} ring_rows for {R} rows")
-    requests = []
     if hist is not None:
-        _need(hist, torch.int32, "hist")
-        _need(hist_len, torch.int32, "hist_len")
+        p_hist, p_len = need(hist, torch.int32, "hist"), need(hist_len, torch.int32, "hist_len")
         if hist.dim() != 2 or hist_len.numel() != hist.shape[0]:
             raise KernelError("shape_logits: hist and hist_len disagree")
-        requests.append(hist.shape[0])
-        if hist.shape[1] == 0:
-            hist = hist_len = None
-    start = ids = values = None
+        requests, last_n = agree(hist.shape[0], "hist"), hist.shape[1]
+        if last_n == 0:
+            p_hist = p_len = 0
     if bias is not None:
         start, ids, values = bias
-        _need(start, torch.int32, "bias start")
-        _need(ids, torch.int32, "bias ids")
-        _need(values, torch.float32, "bias values")
-        if start.numel() < 2 or ids.numel() != values.numel():
+        p_start, p_ids, p_values = need(start, torch.int32, "bias start"), need(ids, torch.int32, "bias ids"), need(values, torch.float32,
+                                                                                                               "bias values")
+        n_biases = ids.numel()
+        if start.numel() < 2 or n_biases != values.numel():
             raise KernelError("shape_logits: bias ids and values disagree")
-        requests.append(start.numel() - 1)
-        if ids.numel() == 0:
-            start = ids = values = None
+        requests = agree(start.numel() - 1, "bias")
+        if n_biases == 0:
+            p_start = p_ids = p_values = 0
     if masks is not None:
-        _need(masks, torch.int32, "masks")
-        _need(mask_rows, torch.int32, "mask_rows")
+        p_masks, p_mask_rows = need(masks, torch.int32, "masks"), need(mask_rows, torch.int32, "mask_rows")
         if masks.dim() != 2 or masks.shape[0] == 0 or masks.shape[1] * 32 < V:
             raise KernelError(f"shape_logits: masks {tuple(masks.shape)} do not cover {V} ids")
-        requests.append(mask_rows.numel())
-    if len(set(requests)) > 1 or (ring_rows is None and requests and requests[0] < R):
-        raise KernelError(f"shape_logits: {R} rows, and requests by their parts: {requests}")
-    if not logits.is_cuda:
-        raise KernelError("kernel argument is not on a CUDA device (there is no CPU path)")
-    for t in (logits, out, hist, hist_len, ring_rows, start, ids, values, masks, mask_rows):
-        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
-            raise KernelError(f"shape_logits: a tensor is on {t.device}, not on the current CUDA device")
+        requests = agree(mask_rows.numel(), "mask_rows")
+        states, words = masks.shape
+    if here < 0 or logits.get_device() != here or out.get_device() != here:
+        raise KernelError("shape_logits: logits and out must be on the current CUDA device (there is no CPU path)")
     kernel("logit_shaping", "gg_shape_logits")(
-        _p(logits), ld, _p(out), ldo, R, V, _p(ring_rows), requests[0] if requests else R, _p(hist), _p(hist_len),
-        hist.shape[1] if hist is not None else 0, float(repeat), float(frequency), float(presence), _p(start), _p(ids), _p(values),
-        ids.numel() if ids is not None else 0, _p(masks), _p(mask_rows), masks.shape[0] if masks is not None else 0,
-        masks.shape[1] if masks is not None else 0, _stream())
+        a, ld, b, ldo, R, V, p_ring, requests if requests >= 0 else R, p_hist, p_len, last_n, float(repeat), float(frequency),
+        float(presence), p_start, p_ids, p_values, n_biases, p_masks, p_mask_rows, states, words, _stream())
     return out
 
 

@@ -39,51 +39,104 @@ __device__ __forceinline__ float shaped(float x, int c, int b, const Shaping& s)
     return x;
 }
 
-template <bool IN_PLACE>
+// VEC: logits of a load (4: rows on 16-byte boundaries).  A thread's logits lie THREADS * VEC apart, so that a warp's lie side by
+// side; they are asked for before the row's request is known, and its state's bits before its ids are counted.
+template <bool IN_PLACE, int VEC>
 __global__ void __launch_bounds__(THREADS) shape_logits_kernel(const float* logits, long long ld, float* out, long long ldo, int V,
                                                                const int* __restrict__ ring_rows, int rings, const Shaping s) {
-    __shared__ int count[SLICE];
-    __shared__ int bias_at[SLICE];
+    constexpr int GROUPS = PER / VEC;
+    __shared__ __align__(16) int count[SLICE];
+    __shared__ __align__(16) int bias_at[SLICE];
     const int r = blockIdx.y, lo = blockIdx.x * SLICE, n = min(SLICE, V - lo);
     pdl_launch();
     const bool sparse = s.hist != nullptr || s.bias_start != nullptr;
     if (sparse) {
-        for (int i = threadIdx.x; i < SLICE; i += THREADS) { count[i] = 0; bias_at[i] = 0; }
+        for (int i = threadIdx.x * 4; i < SLICE; i += THREADS * 4) {
+            *reinterpret_cast<int4*>(count + i) = make_int4(0, 0, 0, 0);
+            *reinterpret_cast<int4*>(bias_at + i) = make_int4(0, 0, 0, 0);
+        }
         __syncthreads();
     }
     pdl_wait();
-    const int ring = ring_rows != nullptr ? ring_rows[r] : r;
-    const bool known = ring >= 0 && ring < rings;
     const float* x = logits + (size_t)r * ld + lo;
     float* y = out + (size_t)r * ldo + lo;
+    float v[GROUPS][VEC];
+    if (!IN_PLACE) {
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) {
+            const int i = (k * THREADS + threadIdx.x) * VEC;
+            if (VEC == 4 && i + 4 <= n) {
+                const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
+                v[k][0] = f.x; v[k][1 % VEC] = f.y; v[k][2 % VEC] = f.z; v[k][3 % VEC] = f.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[k][e] = i + e < n ? __ldcs(x + i + e) : 0.f;
+            }
+        }
+    }
+    const int ring = ring_rows != nullptr ? ring_rows[r] : r;
+    const bool known = ring >= 0 && ring < rings;
+    const int state = known && s.masks != nullptr ? s.mask_rows[ring] : -1;
+    // bits of allowed ids, a thread's groups'  (a state beyond the table allows nothing)
+    unsigned allowed[GROUPS];
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+        const int at = lo + (k * THREADS + threadIdx.x) * VEC;
+        allowed[k] = state < 0 ? 0xffffffffu : state < s.states && at < V ? (unsigned)s.masks[(size_t)state * s.words + (at >> 5)] >> (at & 31) : 0u;
+    }
+    bool any = false;                               // an id of this slice is penalised or has a bias
     if (sparse) {
         if (known && s.hist != nullptr) {
             const int* h = s.hist + (size_t)ring * s.last_n;
             const int m = min(s.hist_len[ring], s.last_n);
             for (int t = threadIdx.x; t < m; t += THREADS) {
                 const int id = h[t];
-                if (id >= lo && id - lo < n) atomicAdd(&count[id - lo], 1);
+                if (id >= lo && id - lo < n) { atomicAdd(&count[id - lo], 1); any = true; }
             }
         }
         if (known && s.bias_start != nullptr) {
             const int e = min(s.bias_start[ring + 1], s.biases);
             for (int t = max(s.bias_start[ring], 0) + threadIdx.x; t < e; t += THREADS) {
                 const int id = s.bias_ids[t];
-                if (id >= lo && id - lo < n) atomicMax(&bias_at[id - lo], t + 1);     // of an id that is listed twice, the last entry
+                // (of an id that is listed twice, the last entry)
+                if (id >= lo && id - lo < n) { atomicMax(&bias_at[id - lo], t + 1); any = true; }
             }
         }
-        __syncthreads();
+        any = __syncthreads_or(any);
     }
-    const int state = known && s.masks != nullptr ? s.mask_rows[ring] : -1;
-    // (a state beyond the table allows nothing)
-    const int* bits = state >= 0 && state < s.states ? s.masks + (size_t)state * s.words : nullptr;
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-        const int v = lo + i;
-        const bool allowed = state < 0 || (bits != nullptr && (bits[v >> 5] >> (v & 31) & 1));
-        if (!allowed) { y[i] = -INFINITY; continue; }
-        const int c = sparse ? count[i] : 0, b = sparse ? bias_at[i] : 0;
-        if (IN_PLACE && c == 0 && b == 0) continue;
-        y[i] = shaped(x[i], c, b, s);
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+        const int i = (k * THREADS + threadIdx.x) * VEC;
+        if (i >= n) break;
+        int c[VEC] = {}, b[VEC] = {};
+        if (any) {
+            if (VEC == 4) {
+                const int4 c4 = *reinterpret_cast<const int4*>(count + i), b4 = *reinterpret_cast<const int4*>(bias_at + i);
+                c[0] = c4.x; c[1 % VEC] = c4.y; c[2 % VEC] = c4.z; c[3 % VEC] = c4.w;
+                b[0] = b4.x; b[1 % VEC] = b4.y; b[2 % VEC] = b4.z; b[3 % VEC] = b4.w;
+            } else { c[0] = count[i]; b[0] = bias_at[i]; }
+        }
+        if (IN_PLACE) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (i + e >= n) break;
+                if (!(allowed[k] >> e & 1)) y[i + e] = -INFINITY;
+                else if (c[e] > 0 || b[e] > 0) y[i + e] = shaped(x[i + e], c[e], b[e], s);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (any && (c[e] > 0 || b[e] > 0)) v[k][e] = shaped(v[k][e], c[e], b[e], s);
+                if (!(allowed[k] >> e & 1)) v[k][e] = -INFINITY;
+            }
+            if (VEC == 4 && i + 4 <= n) {
+                __stcs(reinterpret_cast<float4*>(y + i), make_float4(v[k][0], v[k][1 % VEC], v[k][2 % VEC], v[k][3 % VEC]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (i + e < n) __stcs(y + i + e, v[k][e]);
+            }
+        }
     }
 }
 
@@ -103,10 +156,11 @@ GG_API gg_shape_logits(const float* logits, long long ld, float* out, long long 
     const Shaping s = {hist, hist_len, last_n, repeat, frequency, presence, bias_start, bias_ids, bias_values, biases,
                        masks, mask_rows, states, words};
     const dim3 grid((V + SLICE - 1) / SLICE, R);
-    if (out == logits) {
-        if (ld != ldo) return GG_ERR_ARG;
-        if (hist == nullptr && bias_start == nullptr && masks == nullptr) return 0;
-        return gg_launch(shape_logits_kernel<true>, grid, dim3(THREADS), 0, stream, 1, logits, ld, out, ldo, V, ring_rows, rings, s);
-    }
-    return gg_launch(shape_logits_kernel<false>, grid, dim3(THREADS), 0, stream, 1, logits, ld, out, ldo, V, ring_rows, rings, s);
+    const bool vec = ((uintptr_t)logits & 15) == 0 && ((uintptr_t)out & 15) == 0 && (R == 1 || ((ld | ldo) & 3) == 0);
+    const bool in_place = out == logits;
+    if (in_place && R > 1 && ld != ldo) return GG_ERR_ARG;
+    if (in_place && hist == nullptr && bias_start == nullptr && masks == nullptr) return 0;
+    auto kern = in_place ? (vec ? shape_logits_kernel<true, 4> : shape_logits_kernel<true, 1>)
+                         : (vec ? shape_logits_kernel<false, 4> : shape_logits_kernel<false, 1>);
+    return gg_launch(kern, grid, dim3(THREADS), 0, stream, 1, logits, ld, out, ldo, V, ring_rows, rings, s);
 }
