@@ -60,6 +60,20 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t local_addr, uint32_t rank
     return v;
 }
 
+// from the shared memory of CTA `rank` of the cluster, at the address that `local` is in this CTA
+__device__ __forceinline__ void attn_remote(uint32_t local, int rank, float& a, float& b) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(a), "=f"(b) : "r"(remote) : "memory");
+}
+__device__ __forceinline__ float4 attn_remote4(uint32_t local, int rank) {
+    uint32_t remote;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ uint4 ldg16(const bf16* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
 __device__ __forceinline__ void cp_async16(void* smem, const void* gmem) {
@@ -134,18 +148,19 @@ constexpr int ATT_RECV_BYTES = ATT_RECV_O + ATT_RECV_ML;
 // are; per group the place of its first member in `rows` (and one place beyond the last group's) and its pages; `rows`, the
 // members' token rows group by group; per token row its group (-1: none) and its place among the group's members.  A group's
 // members are cut into tiles of equal size whose rows, members times the query heads of a kv head, fit 128; the units of work
-// are the pages of (group, tile, kv head) in that order, and CTA c of the prefix kernel takes `per` of them from c per on.
-// A run of pages that a CTA takes of one (tile, kv head) is a part: per row the values' sum, the maximum it was taken against
-// and the sum of the weights.  The part's rows begin at row0 + 128 c, with row0 the rows of all (tile, kv head)s before:
-// later parts are later in c or in row0, and 128 is the most a part has, so no two overlap.
+// are the pages of (group, tile, kv head) in that order, and cluster c of the prefix kernel takes `per` of them from c per on.
+// A run of pages that a cluster takes of one (tile, kv head) is a part: per row the values' sum, the maximum it was taken
+// against and the sum of the weights.  The part's rows begin at row0 + 128 c, with row0 the rows of all (tile, kv head)s
+// before: later parts are later in c or in row0, and 128 is the most a part has, so no two overlap.
 struct AttnShared {
     const int* plan;
     int cap;                          // token rows that the plan has room for
-    int ctas;                         // of the prefix kernel
+    int clusters;                     // of the prefix kernel
     float* part_o;                    // [rows][dv]
     float2* part_ml;                  // [rows] (maximum in log2 units, sum)
 };
 constexpr int SHARED_ROWS = 128;      // of a tile
+constexpr int SHARED_CLUSTER = 8;     // CTAs that share a run's pages
 
 struct SharedPlan {
     const int *first, *pages, *rows, *group_of, *member_of;
@@ -169,9 +184,8 @@ struct SharedPlan {
         for (int i = 0; i < g; ++i) u += pages[i] * tiles(i, G) * nkv;
         return u;
     }
-    // units of a CTA: all of them have the same number, and at least two pages (one page's part costs as much to write and
-    // to add up as reading two pages takes)
-    __device__ __forceinline__ int per(int total, int ctas) const { return max(2, (total + ctas - 1) / ctas); }
+    // units of a cluster: as many for each, and a page for each of its CTAs at least
+    __device__ __forceinline__ int per(int total, int clusters) const { return max(SHARED_CLUSTER, (total + clusters - 1) / clusters); }
 };
 
 // The parts of one token row and kv head: `count` of them, 128 rows apart.
@@ -184,7 +198,7 @@ struct SharedParts {
         const int g = p.group_of[tok];
         count = 0;
         if (g < 0) return;
-        const int pg = p.pages[g], per = p.per(p.units_before(p.groups, nkv, G), a.ctas), tm = p.tile_members(g, G);
+        const int pg = p.pages[g], per = p.per(p.units_before(p.groups, nkv, G), a.clusters), tm = p.tile_members(g, G);
         const int mine = p.member_of[tok], tile = mine / tm, inside = mine - tile * tm;
         const int u0 = p.units_before(g, nkv, G) + (tile * nkv + kvh) * pg;
         const int c0 = u0 / per, c1 = (u0 + pg - 1) / per;
@@ -194,29 +208,52 @@ struct SharedParts {
         ml = a.part_ml + row;
         count = c1 - c0 + 1;
     }
-    // row r's column c: the parts' shares beside what was seen elsewhere (maximum M, sum L, values acc), in their order
-    __device__ __forceinline__ void join(float& M, float& L, float& acc, int r, int c, int dv) const {
-        for (int k0 = 0; k0 < count; k0 += 8) {
+    // One warp's share of the parts (every `step`-th from k0 on) of the kv head's G rows, added up into sm_o [G][DV] and sm_ml
+    // [G][2], four columns a lane; eight rows of parts are asked for at a time, whichever row or part they are of.
+    template <int DV>
+    __device__ __forceinline__ void add_up(int k0, int step, int G, int dv, int lane, float* sm_o, float* sm_ml) const {
+        const int mine = k0 < count ? (count - 1 - k0) / step + 1 : 0;
+        const bool in = lane * 4 < dv;
+        if (mine == 0) {
+            if (lane < G) { sm_ml[lane * 2] = -INFINITY; sm_ml[lane * 2 + 1] = 0.f; }
+            for (int r = 0; in && r < G; ++r) *reinterpret_cast<float4*>(sm_o + r * DV + lane * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+            return;
+        }
+        float M = -INFINITY, L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        int r_ask = 0, i_ask = 0, r = 0, i = 0;          // row and part that are asked for, and that are added, next
+        while (r < G) {
             float2 v[8];
-            float x[8];
-            float top = M;
+            float4 x[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const bool in = k0 + k < count;
-                v[k] = in ? ml[(size_t)(k0 + k) * SHARED_ROWS + r] : make_float2(-INFINITY, 0.f);
-                x[k] = in ? o[((size_t)(k0 + k) * SHARED_ROWS + r) * dv + c] : 0.f;
-                top = fmaxf(top, v[k].x);
+            for (int e = 0; e < 8; ++e) {
+                v[e] = make_float2(-INFINITY, 0.f);
+                x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r_ask < G) {
+                    const size_t at = (size_t)(k0 + i_ask * step) * SHARED_ROWS + r_ask;
+                    v[e] = ml[at];
+                    if (in) x[e] = *reinterpret_cast<const float4*>(o + at * dv + lane * 4);
+                    if (++i_ask == mine) { i_ask = 0; ++r_ask; }
+                }
             }
-            if (top == -INFINITY) continue;
-            const float f = fast_exp2(M - top);
-            L *= f;
-            acc *= f;
-            M = top;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float w = fast_exp2(v[k].x - top);
-                L = fmaf(v[k].y, w, L);
-                acc = fmaf(x[k], w, acc);
+            for (int e = 0; e < 8; ++e) {
+                if (r >= G) break;
+                const float top = fmaxf(M, v[e].x);
+                if (top != -INFINITY) {
+                    const float f = fast_exp2(M - top), w = fast_exp2(v[e].x - top);
+                    M = top;
+                    L = fmaf(v[e].y, w, L * f);
+                    acc.x = fmaf(x[e].x, w, acc.x * f); acc.y = fmaf(x[e].y, w, acc.y * f);
+                    acc.z = fmaf(x[e].z, w, acc.z * f); acc.w = fmaf(x[e].w, w, acc.w * f);
+                }
+                if (++i == mine) {
+                    if (in) *reinterpret_cast<float4*>(sm_o + r * DV + lane * 4) = acc;
+                    if (lane == 0) { sm_ml[r * 2] = M; sm_ml[r * 2 + 1] = L; }
+                    i = 0; ++r;
+                    M = -INFINITY; L = 0.f;
+                    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
             }
         }
     }
@@ -285,6 +322,9 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
         p_end = min(last + 1, p_begin + pps);
     }
     const int npg = max(0, p_end - p_begin);
+
+    SharedParts parts;
+    if constexpr (SHARED) parts.find(shared, tok, kvh, nkv, G, dv);
 
     float o[NT][4];
 #pragma unroll
@@ -393,9 +433,12 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
         while (clock64() - t0 < 2000000LL) { }       // let copies in flight land before the CTA goes away
         __syncthreads();
     }
-    float* sm_o = reinterpret_cast<float*>(smem);                 // [4][16][DV]
-    float* sm_ml = sm_o + 4 * 16 * DV;                            // [4][16][2]
-    float* res_o = sm_ml + 4 * 16 * 2;                            // [16][DV]  this CTA's merged output (cluster form)
+    // what this CTA adds up: the four warps' shares of its pages, and (SHARED) the five warps' shares of the prefix's parts,
+    // which go round the CTAs of a row
+    constexpr int ADDENDS = SHARED ? 9 : 4;
+    float* sm_o = reinterpret_cast<float*>(smem);                 // [ADDENDS][16][DV]
+    float* sm_ml = sm_o + ADDENDS * 16 * DV;                      // [ADDENDS][16][2]
+    float* res_o = sm_ml + ADDENDS * 16 * 2;                      // [16][DV]  this CTA's merged output (cluster form)
     float* res_ml = res_o + 16 * DV;                              // [16][2]
     if (warp < 4) {
 #pragma unroll
@@ -417,18 +460,18 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
             if (t == 0) { sm_ml[(warp * 16 + g + 8) * 2] = m[1]; sm_ml[(warp * 16 + g + 8) * 2 + 1] = l[1]; }
         }
     }
+    if constexpr (SHARED)
+        parts.add_up<DV>(split * 5 + warp, 5 * nsplit, G, dv, lane, sm_o + (4 + warp) * 16 * DV, sm_ml + (4 + warp) * 16 * 2);
     __syncthreads();
-    SharedParts parts;
-    if constexpr (SHARED) parts.find(shared, tok, kvh, nkv, G, dv);
     for (int idx = threadIdx.x; idx < G * dv; idx += blockDim.x) {
         const int r = idx / dv, c = idx - r * dv;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_ml[(w * 16 + r) * 2]);
+        for (int w = 0; w < ADDENDS; ++w) M = fmaxf(M, sm_ml[(w * 16 + r) * 2]);
         float L = 0.f, acc = 0.f;
         if (M != -INFINITY) {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < ADDENDS; ++w) {
                 const float f = fast_exp2(sm_ml[(w * 16 + r) * 2] - M);
                 L += sm_ml[(w * 16 + r) * 2 + 1] * f;
                 acc += sm_o[(w * 16 + r) * DV + c] * f;
@@ -436,7 +479,6 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
         }
         const int head = kvh * G + r;
         if (nsplit == 1) {
-            if constexpr (SHARED) parts.join(M, L, acc, r, c, dv);
             const float Ls = attn_sink_sum(L, M, sink, head);
             out[((size_t)tok * nq + head) * dv + c] =
                 __float2bfloat16_rn(attn_gate(Ls > 0.f ? acc * out_scale / Ls : 0.f, sh, tok, head * dv + c));
@@ -481,7 +523,6 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
                     acc += recv_o[(k * rounds + round) * 32 + lane] * f;
                 }
             }
-            if constexpr (SHARED) parts.join(M, L, acc, r, idx - r * dv, dv);
             const float Ls = attn_sink_sum(L, M, sink, kvh * G + r);
             out[((size_t)tok * nq + kvh * G) * dv + idx] =
                 __float2bfloat16_rn(attn_gate(Ls > 0.f ? acc * out_scale / Ls : 0.f, sh, tok, kvh * G * dv + idx));
@@ -513,7 +554,6 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
                     acc += as[k] * f;
                 }
             }
-            if constexpr (SHARED) parts.join(M, L, acc, r, c, dv);
             const float Ls = attn_sink_sum(L, M, sink, kvh * G + r);
             out[((size_t)tok * nq + kvh * G + r) * dv + c] =
                 __float2bfloat16_rn(attn_gate(Ls > 0.f ? acc * out_scale / Ls : 0.f, sh, tok, (kvh * G + r) * dv + c));
@@ -524,9 +564,9 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
 }
 
 template <int DK, int DV, int STAGES>
-constexpr int decode_tma_smem() {
+constexpr int decode_tma_smem(int addends = 4) {
     constexpr int ring = STAGES * ((DK + DV) / 64) * 8192;    // bytes: a box of 8 KB per 64 columns of K and of V
-    constexpr int merge = (5 * 16 * DV + 5 * 16 * 2) * 4;
+    const int merge = ((addends + 1) * 16 * DV + (addends + 1) * 16 * 2) * 4;
     return (ring > merge ? ring : merge) + 1024 + 256 + ATT_RECV_BYTES;
 }
 

@@ -472,20 +472,6 @@ int launch_decode_tma(const CUtensorMap& tk, const CUtensorMap& tv, const void* 
 // share of the rows per CTA, read through distributed shared memory and always in rank order.
 // All exponentials go to the special-function unit: computing a share of them as polynomials on the FMA pipe,
 // and a pass over the scores for their maximum, cost more issue slots than the unit's time they saved.
-// from the shared memory of CTA `rank` of the cluster, at the address that `local` is in this CTA
-__device__ __forceinline__ void attn_remote(uint32_t local, int rank, float& a, float& b) {
-    uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(a), "=f"(b) : "r"(remote) : "memory");
-}
-__device__ __forceinline__ float4 attn_remote4(uint32_t local, int rank) {
-    uint32_t remote;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
-    return v;
-}
-
 template <int DK, int DV, bool EXACT>
 __global__ void __launch_bounds__(192) attn_prefill_tc_kernel(
     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,

@@ -7,15 +7,19 @@
 // shared_prefix_kernel: a tile is up to 128 rows, members of a group times the query heads of a kv head.  Per page of 64 keys
 // S = Q K^T (tcgen05.mma 128 x 64 x 16) lands in tensor memory, four warps take a row per thread, leave P as bfloat16 where S
 // was and O += P V accumulates in tensor memory, as in the prefill kernel (attention_fast.cu), without its masks: every reader
-// sees every key of the prefix.  All (group, tile, kv head)s' pages are one line of work cut into equal runs, one per CTA, so
-// that the grid is the same for every plan (a captured step replays with other groups) and no CTA has more pages than another.
+// sees every key of the prefix.  All (group, tile, kv head)s' pages are one line of work cut into equal runs, one per cluster
+// of eight CTAs, which share a run's pages and add up their parts through distributed shared memory: the grid is the same for
+// every plan (a captured step replays with other groups), no cluster has more pages than another, and a row is left with the
+// few parts that the kernel after this one adds up (a part per CTA instead was 37 of them for 16 (tile, kv head)s: 20 MB
+// written and read again).
 //
 // Replaces, for rows that share pages, the reading of those pages once per row.
 #include "attention_common.cuh"
 
 namespace {
 
-constexpr int SHARED_CTAS = 296;      // two per SM
+// Clusters of eight that run side by side, two CTAs an SM (an SM group takes four).
+constexpr int SHARED_CLUSTERS = 32;
 
 template <int DK, int DV, bool EXACT>
 __global__ void __launch_bounds__(192) shared_prefix_kernel(
@@ -47,9 +51,10 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = nq / nkv;
     const SharedPlan plan(shared);
-    const int total = plan.units_before(plan.groups, nkv, G), per = plan.per(total, shared.ctas);
-    const int u_begin = min((int)blockIdx.x * per, total), u_end = min(u_begin + per, total);
-    if (u_begin >= u_end) {                         // (every kernel of a step waits for the one before it: common.cuh)
+    const int total = plan.units_before(plan.groups, nkv, G), per = plan.per(total, shared.clusters);
+    const int rank = (int)blockIdx.z, u_begin = min((int)blockIdx.x * per, total), u_end = min(u_begin + per, total);
+    pdl_launch();                                   // (the whole grid is resident at once: the rule in common.cuh)
+    if (u_begin >= u_end) {                         // (every kernel of a step waits for the one before it, too)
         pdl_wait();
         return;
     }
@@ -76,8 +81,8 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
     const bool aligned = (tma::smem_u32(smem) & 1023u) == 0;
     if (!aligned && threadIdx.x == 0) atomicCAS(status, 0, 29);
 
-    // A CTA's run of units is cut where the (tile, kv head) changes.  Every role walks the same cuts.
-    struct Run { int first, members, head, page0, pages; size_t row0; };
+    // A cluster's units are cut where the (tile, kv head) changes; of a run's pages, this CTA takes its share.
+    struct Run { int first, members, head, page0, pages, all; size_t row0; };
     auto run_at = [&](int u) -> Run {
         int g = 0, before = 0;
         for (; g + 1 < plan.groups; ++g) {
@@ -86,25 +91,33 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
             before += n;
         }
         const int pg = plan.pages[g], tm = plan.tile_members(g, G), rel = u - before;
-        const int th = rel / pg, tile = th / nkv;
+        const int th = rel / pg, tile = th / nkv, page = rel - th * pg;
         Run r;
         r.head = th - tile * nkv;
-        r.page0 = rel - th * pg;
-        r.pages = min(pg - r.page0, u_end - u);
+        r.all = min(pg - page, u_end - u);
+        const int a = r.all * rank / SHARED_CLUSTER, e = r.all * (rank + 1) / SHARED_CLUSTER;
+        r.page0 = page + a;
+        r.pages = e - a;
         r.first = plan.first[g] + tile * tm;
         r.members = min(tm, plan.first[g + 1] - r.first);
         r.row0 = (size_t)nkv * G * r.first + (size_t)r.head * G * r.members + (size_t)blockIdx.x * SHARED_ROWS;
         return r;
     };
+    // (a warp goes on or leaves as a whole: what follows a wait is for whole warps)
+    auto wait = [&](uint64_t* bar, uint32_t phase, int code) -> bool {
+        return __all_sync(0xffffffffu, tma::mbar_wait(bar, phase, abort_flag, status, code));
+    };
 
-    if (warp == 4) {
-        // The prefix's pages were written by earlier steps (this step's tokens go to pages of the rows' own), so they are
-        // streamed before the kernel before this one has finished.
-        if (lane == 0 && aligned) {
-            int j = 0;
-            bool ok = true;
-            for (int u = u_begin; u < u_end && ok;) {
-                const Run r = run_at(u);
+    int j = 0, run = 0, used = 0;                   // pages of this CTA so far (each role counts its own); runs, and those with pages
+    bool ok = aligned;
+    for (int u = u_begin; u < u_end; ++run) {
+        const Run r = run_at(u);
+        const int rows = r.members * G;
+        u += r.all;
+        if (warp == 4) {
+            // The prefix's pages were written by earlier steps (this step's tokens go to pages of the rows' own), so they are
+            // streamed before the kernel before this one has finished.
+            if (lane == 0 && ok) {
                 const int* pt = page_table + (size_t)seq_of_token[plan.rows[r.first]] * max_pages;
                 for (int i = 0; i < r.pages; ++i, ++j) {
                     const int s = j & 1;
@@ -119,34 +132,27 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
 #pragma unroll
                     for (int hf = 0; hf < HV; ++hf) tma::load_2d(Vs + s * V_STAGE + hf * KBOX, &tmV, &v_full[s], hf * 64, row);
                 }
-                u += r.pages;
             }
-        }
-    } else if (warp == 5) {
-        if (lane == 0 && aligned) {
-            const uint32_t idesc_qk = tc5::idesc_bf16(128, 64, 0), idesc_pv = tc5::idesc_bf16(128, EXACT ? DV : (dv + 15) & ~15, 1);
-            const uint32_t q_a = tma::smem_u32(Qs), k_a = tma::smem_u32(Ks), v_a = tma::smem_u32(Vs);
-            auto issue_scores = [&](int j) -> bool {
-                const int s = j & 1;
-                if (!tma::mbar_wait(&k_full[s], (uint32_t)((j >> 1) & 1), abort_flag, status, 73)) return false;
-                tc5::fence_after();
+        } else if (warp == 5) {
+            if (lane == 0 && ok && r.pages > 0) {
+                const uint32_t idesc_qk = tc5::idesc_bf16(128, 64, 0), idesc_pv = tc5::idesc_bf16(128, EXACT ? DV : (dv + 15) & ~15, 1);
+                const uint32_t q_a = tma::smem_u32(Qs), k_a = tma::smem_u32(Ks), v_a = tma::smem_u32(Vs);
+                auto issue_scores = [&](int j) -> bool {
+                    const int s = j & 1;
+                    if (!tma::mbar_wait(&k_full[s], (uint32_t)((j >> 1) & 1), abort_flag, status, 73)) return false;
+                    tc5::fence_after();
 #pragma unroll
-                for (int ks = 0; ks < DK / 16; ++ks) {
-                    if (!EXACT && ks * 16 >= d) break;
-                    const uint64_t a = tc5::smem_desc(q_a + (ks >> 2) * QBOX + (ks & 3) * 32, 16, 1024);
-                    const uint64_t b = tc5::smem_desc(k_a + s * K_STAGE + (ks >> 2) * KBOX + (ks & 3) * 32, 16, 1024);
-                    tc5::mma(S_t + (uint32_t)(s * 64), a, b, idesc_qk, ks > 0 ? 1u : 0u);
-                }
-                tc5::commit(&s_full[s]);
-                tc5::commit(&k_empty[s]);
-                return true;
-            };
-            int j = 0, run = 0;
-            bool ok = true;
-            for (int u = u_begin; u < u_end && ok; ++run) {
-                const Run r = run_at(u);
-                // (the run's first scores come after the last P V of the run before: its Q is written when that is read)
-                ok = tma::mbar_wait(q_full, (uint32_t)(run & 1), abort_flag, status, 74);
+                    for (int ks = 0; ks < DK / 16; ++ks) {
+                        if (!EXACT && ks * 16 >= d) break;
+                        const uint64_t a = tc5::smem_desc(q_a + (ks >> 2) * QBOX + (ks & 3) * 32, 16, 1024);
+                        const uint64_t b = tc5::smem_desc(k_a + s * K_STAGE + (ks >> 2) * KBOX + (ks & 3) * 32, 16, 1024);
+                        tc5::mma(S_t + (uint32_t)(s * 64), a, b, idesc_qk, ks > 0 ? 1u : 0u);
+                    }
+                    tc5::commit(&s_full[s]);
+                    tc5::commit(&k_empty[s]);
+                    return true;
+                };
+                ok = tma::mbar_wait(q_full, (uint32_t)(used & 1), abort_flag, status, 74);
                 if (ok) ok = issue_scores(j);
                 for (int i = 0; i < r.pages && ok; ++i, ++j) {
                     // The next page's scores do not wait for this page's softmax: their buffer was last read by the
@@ -167,24 +173,14 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
                     tc5::commit(&v_empty[s]);
                 }
                 if (ok) tc5::commit(o_done);
-                u += r.pages;
             }
-        }
-    } else if (aligned) {
-        const int row = threadIdx.x;                       // row of the tile = tensor-memory lane
-        const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-        pdl_wait();                                        // q
-        // (a warp goes on or leaves as a whole: what follows a wait is for whole warps)
-        auto wait = [&](uint64_t* bar, uint32_t phase, int code) -> bool {
-            return __all_sync(0xffffffffu, tma::mbar_wait(bar, phase, abort_flag, status, code));
-        };
-        int j = 0, run = 0;
-        bool ok = true;
-        for (int u = u_begin; u < u_end && ok; ++run) {
-            const Run r = run_at(u);
-            const int rows = r.members * G;
+        } else {
+            const int row = threadIdx.x;                       // row of the tile = tensor-memory lane
+            const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
             const bool live = row < rows, idle = warp * 32 >= rows;     // (a warp without rows only keeps the pace)
-            {
+            float m_used = -INFINITY, l = 0.f;
+            if (run == 0) pdl_wait();                          // q
+            if (ok && r.pages > 0) {
                 // Q into its swizzled tile: row r of a box is 128 bytes, 16-byte chunk c at place c ^ (r & 7)
                 const int member = live ? row / G : 0;
                 const bf16* src = q + ((size_t)plan.rows[r.first + member] * nq + (size_t)r.head * G + (row - member * G)) * d;
@@ -200,8 +196,7 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
                 __syncwarp();
                 if (lane == 0) tma::mbar_arrive(q_full);
             }
-            float m_used = -INFINITY, l = 0.f;
-            for (int i = 0; i < r.pages; ++i, ++j) {
+            for (int i = 0; i < r.pages && ok; ++i, ++j) {
                 const int s = j & 1;
                 if (!(ok = wait(&s_full[s], (uint32_t)((j >> 1) & 1), 77))) break;
                 tc5::fence_after();
@@ -281,32 +276,63 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
                 __syncwarp();
                 if (lane == 0) tma::mbar_arrive(&p_ready[s]);
             }
-            if (!ok) break;
-            // the run's last P V, then the part: O as it is, the maximum it was taken against and its sum
-            // (a barrier of its own: by pv_done's parity, two phases not yet complete would look like the last one being so)
-            if (!(ok = wait(o_done, (uint32_t)(run & 1), 79))) break;
-            tc5::fence_after();
-            if (!idle) {
-                float* dst = shared.part_o + (r.row0 + row) * dv;
+            // The run's last P V (on a barrier of its own: by pv_done's parity, two phases not yet complete would look like the
+            // last one being so), then O as it is for the cluster, over Q, K and V, which every product is done with; 16-byte
+            // chunk c of row r lies at place c ^ (r & 7)
+            if (ok && r.pages > 0) ok = wait(o_done, (uint32_t)(used & 1), 79);
+            if (ok && !idle) {
+                tc5::fence_after();
+                uint4* os = reinterpret_cast<uint4*>(smem) + row * (DV / 4);
 #pragma unroll 1
-                for (int c0 = 0; c0 < (EXACT ? DV : dv); c0 += 32) {
+                for (int c0 = 0; c0 < (r.pages > 0 ? DV : 0); c0 += 32) {
                     uint32_t o[32];
                     tc5::ld32(O_t + lane_off + c0, o);
                     tc5::wait_ld();
-                    if (live) {
 #pragma unroll
-                        for (int c = 0; c < 32; c += 4)
-                            if (EXACT || c0 + c < dv) *reinterpret_cast<uint4*>(dst + c0 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-                    }
+                    for (int c = 0; c < 8; ++c) os[(c0 / 4 + c) ^ (row & 7)] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
                 }
-                if (live) shared.part_ml[r.row0 + row] = make_float2(m_used, l);
+                tc5::fence_before();
             }
-            u += r.pages;
+            reinterpret_cast<float2*>(bars + 32)[row] = make_float2(m_used, l);
         }
+        if (r.pages > 0) ++used;
+        // (every CTA of the cluster passes both barriers, whatever happened before: they share the run)
+        __syncthreads();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        {
+            // the rows go round the cluster's CTAs and their warps; the shares are added in rank order
+            const uint32_t os = tma::smem_u32(smem), ml = tma::smem_u32(bars + 32);
+            for (int x = rank + warp * SHARED_CLUSTER; x < rows; x += 6 * SHARED_CLUSTER) {
+                float m[SHARED_CLUSTER], l[SHARED_CLUSTER], M = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < SHARED_CLUSTER; ++k) attn_remote(ml + 8u * (uint32_t)x, k, m[k], l[k]);
+                float4 v[SHARED_CLUSTER], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < SHARED_CLUSTER; ++k) {
+                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    // (a share without pages has left nothing)
+                    if (m[k] != -INFINITY && lane < DV / 4) v[k] = attn_remote4(os + 16u * (uint32_t)(x * (DV / 4) + (lane ^ (x & 7))), k);
+                    M = fmaxf(M, m[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < SHARED_CLUSTER; ++k) {
+                    const float f = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - M);
+                    sum = fmaf(l[k], f, sum);
+                    acc.x = fmaf(v[k].x, f, acc.x); acc.y = fmaf(v[k].y, f, acc.y); acc.z = fmaf(v[k].z, f, acc.z); acc.w = fmaf(v[k].w, f, acc.w);
+                }
+                if (lane * 4 < dv) *reinterpret_cast<float4*>(shared.part_o + (r.row0 + x) * dv + lane * 4) = acc;
+                if (lane == 0) shared.part_ml[r.row0 + x] = make_float2(M, sum);
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        // (what the next run's copies and products write was read and written as ordinary memory in between)
+        tc5::fence_proxy_async_smem();
+        __syncthreads();
     }
     pdl_wait();
-    tc5::fence_before();
-    __syncthreads();
     if (*abort_flag) {
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000LL) { }       // let copies in flight land before the CTA goes away
@@ -321,13 +347,15 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
 template <int DK, int DV, bool EXACT>
 int launch_prefix(const CUtensorMap& tk, const CUtensorMap& tv, const void* q, const int* page_table, const int* seq_of_token, int max_pages,
                   int nq, int nkv, float scale_log2, int n_pages, int* status, int d, int dv, const AttnShared& shared, cudaStream_t stream) {
-    constexpr int smem = (DK / 64) * (16384 + 2 * 8192) + (DV / 64) * 2 * 8192 + 256;
+    // Q, K x 2, V x 2 (boxes of 64 columns: 16 KB of Q, 8 KB of K or V), barriers, the rows' maxima and sums
+    constexpr int tiles = (DK / 64) * (16384 + 2 * 8192) + (DV / 64) * 2 * 8192, smem = tiles + 256 + 1024;
+    static_assert(tiles >= 128 * DV * 4, "the float32 rows that a cluster adds lie where Q, K and V were");
     static int known[GG_MAX_DEVICES];
     auto kern = shared_prefix_kernel<DK, DV, EXACT>;
     int resident = 0;
     const int rc = gg_resident(kern, 192, smem, known, resident);
     if (rc != 0) return rc;
-    return gg_launch(kern, dim3(shared.ctas), dim3(192), smem, stream, 1, tk, tv, (const bf16*)q, page_table, seq_of_token, max_pages, nq,
+    return gg_launch(kern, dim3(shared.clusters, 1, SHARED_CLUSTER), dim3(192), smem, stream, SHARED_CLUSTER, tk, tv, (const bf16*)q, page_table, seq_of_token, max_pages, nq,
                      nkv, scale_log2, n_pages, status, d, dv, shared);
 }
 
@@ -335,7 +363,7 @@ template <int DK, int DV, int STAGES, bool EXACT>
 int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const void* q, void* out, const int* positions, const int* seq_of_token,
                 const int* page_table, int max_pages, int ntok, int nq, int nkv, float scale_log2, int splits, const float* sink,
                 float out_scale, int n_pages, int* status, const AttnShape& sh, const AttnShared& shared, cudaStream_t stream) {
-    constexpr int smem = decode_tma_smem<DK, DV, STAGES>();
+    constexpr int smem = decode_tma_smem<DK, DV, STAGES>(9);
     static int known[GG_MAX_DEVICES];
     auto kern = attn_decode_tma_kernel<DK, DV, STAGES, EXACT, true>;
     int resident = 0;
@@ -347,12 +375,12 @@ int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const void* q, voi
                      ctas <= resident ? 1 : 0, sink, out_scale, n_pages, status, sh, shared);
 }
 
-long long part_rows(int ntok, int nq) { return (long long)nq * ntok + (long long)SHARED_ROWS * SHARED_CTAS; }
+long long part_rows(int ntok, int nq) { return (long long)nq * ntok + (long long)SHARED_ROWS * SHARED_CLUSTERS; }
 
 }  // namespace
 
 // Decode attention (see gg_attn_decode_tma) of a step with shared prefixes: plan as at AttnShared, part: gg_attn_shared
-// scratch of (nq ntok + 128 * 296) (dv + 2) floats, 16-byte aligned.  splits: 1, 2, 4 or 8 CTAs share a row's own pages.
+// scratch of (nq ntok + 128 * 32) (dv + 2) floats, 16-byte aligned.  splits: 1, 2, 4 or 8 CTAs share a row's own pages.
 // status: codes 71-79 name the prefix kernel's wait that ran out, 11 and 12 the other's.
 GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_pool, void* out, const int* positions,
                              const int* seq_of_token, const int* page_table, int max_pages, int page_size, int n_pages, const int* plan,
@@ -373,7 +401,7 @@ GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_po
     if ((rc = tma::make_map_bf16(&tv, v_pool, pool_rows, dv, dv, PAGE)) != 0) return rc;
     const float scale_log2 = scale * 1.4426950408889634f;
     const AttnShape sh = {d, dv, 0, (const bf16*)gate, ldg};
-    const AttnShared shared = {plan, ntok, SHARED_CTAS, part, reinterpret_cast<float2*>(part + rows * dv)};
+    const AttnShared shared = {plan, ntok, SHARED_CLUSTERS, part, reinterpret_cast<float2*>(part + rows * dv)};
 #define GG_PREFIX(DK_, DV_, EX_) \
     launch_prefix<DK_, DV_, EX_>(tk, tv, q, page_table, seq_of_token, max_pages, nq, nkv, scale_log2, n_pages, status, d, dv, shared, stream)
 #define GG_ROWS(DK_, DV_, ST_, EX_)                                                                                                      \

@@ -53,14 +53,14 @@ def attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page
         status_word(q.device).data_ptr(), stream_ptr())
 
 
-PREFIX_CTAS = 296       # of the kernel over the prefixes (csrc/attention_shared.cu)
+PREFIX_CLUSTERS = 32    # of the kernel over the prefixes (csrc/attention_shared.cu)
 
 
 def shared_scratch(n_tokens: int, nq: int, nkv: int, dv: int) -> int:
     """Floats of scratch that `attn_decode_shared` needs: the parts' rows, and two numbers beside each."""
     if n_tokens <= 0 or nkv <= 0 or nq <= 0 or nq % nkv or dv <= 0:
         raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {dv}, {n_tokens} tokens")
-    return (nq * n_tokens + 128 * PREFIX_CTAS) * (dv + 2)
+    return (nq * n_tokens + 128 * PREFIX_CLUSTERS) * (dv + 2)
 
 
 def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[int], int]]:
