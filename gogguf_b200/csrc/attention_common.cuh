@@ -145,13 +145,14 @@ constexpr int ATT_RECV_BYTES = ATT_RECV_O + ATT_RECV_ML;
 
 
 // A prefix that several rows of a decode step read (attention_shared.cu).  The plan, integers of a step: how many groups there
-// are; per group the place of its first member in `rows` (and one place beyond the last group's) and its pages; `rows`, the
-// members' token rows group by group; per token row its group (-1: none) and its place among the group's members.  A group's
-// members are cut into tiles of equal size whose rows, members times the query heads of a kv head, fit 128; the units of work
-// are the pages of (group, tile, kv head) in that order, and cluster c of the prefix kernel takes `per` of them from c per on.
-// A run of pages that a cluster takes of one (tile, kv head) is a part: per row the values' sum, the maximum it was taken
-// against and the sum of the weights.  The part's rows begin at row0 + 128 c, with row0 the rows of all (tile, kv head)s
-// before: later parts are later in c or in row0, and 128 is the most a part has, so no two overlap.
+// are; per group the place of its first member in `rows` (and one place beyond the last group's), its pages and its first
+// member; `rows`, the members' token rows group by group; per token row the pages that are its prefix (0: none), its group (-1:
+// none) and its place among the group's members.  A group's members are cut into tiles of equal size whose rows, members times
+// the query heads of a kv head, fit 128; the units of work are the pages of (group, tile, kv head) in that order, and cluster c
+// of the prefix kernel takes `per` of them from c per on.  A run of pages that a cluster takes of one (tile, kv head) is a part:
+// per row the values' sum, the maximum it was taken against and the sum of the weights.  The part's rows begin at row0 + 128 c,
+// with row0 the rows of all (tile, kv head)s before: later parts are later in c or in row0, and 128 is the most a part has, so
+// no two overlap.
 struct AttnShared {
     const int* plan;
     int cap;                          // token rows that the plan has room for
@@ -163,29 +164,67 @@ constexpr int SHARED_ROWS = 128;      // of a tile
 constexpr int SHARED_CLUSTER = 8;     // CTAs that share a run's pages
 
 struct SharedPlan {
-    const int *first, *pages, *rows, *group_of, *member_of;
-    int groups;
+    const int *count, *first, *pages, *lead, *rows, *pages_of, *group_of, *member_of;
+    int cap;
     __device__ __forceinline__ SharedPlan(const AttnShared& a)
-        : first(a.plan + 4), pages(first + a.cap + 1), rows(pages + a.cap), group_of(rows + a.cap), member_of(group_of + a.cap),
-          groups(a.plan[0]) {}
-    // tiles of group g, and the members of each but the last
-    __device__ __forceinline__ int members(int g) const { return first[g + 1] - first[g]; }
-    __device__ __forceinline__ int tiles(int g, int G) const {
+        : count(a.plan), first(a.plan + 4), pages(first + a.cap + 1), lead(pages + a.cap), rows(lead + a.cap), pages_of(rows + a.cap),
+          group_of(pages_of + a.cap), member_of(group_of + a.cap), cap(a.cap) {}
+    static __device__ __forceinline__ int tiles(int members, int G) {
         const int most = SHARED_ROWS / G;
-        return (members(g) + most - 1) / most;
+        return (members + most - 1) / most;
     }
-    __device__ __forceinline__ int tile_members(int g, int G) const {
-        const int n = tiles(g, G);
-        return (members(g) + n - 1) / n;
-    }
-    // units of all groups before g
-    __device__ __forceinline__ int units_before(int g, int nkv, int G) const {
-        int u = 0;
-        for (int i = 0; i < g; ++i) u += pages[i] * tiles(i, G) * nkv;
-        return u;
+    // members of each tile but the last
+    static __device__ __forceinline__ int tile_members(int members, int G) {
+        const int n = tiles(members, G);
+        return (members + n - 1) / n;
     }
     // units of a cluster: as many for each, and a page for each of its CTAs at least
-    __device__ __forceinline__ int per(int total, int clusters) const { return max(SHARED_CLUSTER, (total + clusters - 1) / clusters); }
+    static __device__ __forceinline__ int per(int total, int clusters) { return max(SHARED_CLUSTER, (total + clusters - 1) / clusters); }
+
+    // All units, and the group that unit u is of (u < 0: group `which`), by a whole warp: a lane a group.
+    struct Group { int before, pages, first, members, lead; };
+    __device__ __forceinline__ Group find(int u, int which, int nkv, int G, int lane, int& total) const {
+        Group found = {};
+        int groups = 1;
+        total = 0;
+        for (int g0 = 0; g0 < groups; g0 += 32) {
+            const int g = min(g0 + lane, cap - 1);
+            // (asked for before the number of groups is known: beyond the last one stands something that is not used)
+            const int pg = pages[g], f = first[g], m = first[g + 1] - f, head = lead[g];
+            if (g0 == 0) groups = *count;
+            const int units = g0 + lane < groups ? pg * tiles(m, G) * nkv : 0;
+            int upto = units;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            upto += total;
+            const bool it = u < 0 ? g0 + lane == which : u >= upto - units && u < upto;
+            const unsigned mine = __ballot_sync(0xffffffffu, it && units > 0);
+            if (mine != 0) {
+                const int from = __ffs(mine) - 1;
+                found.before = __shfl_sync(0xffffffffu, upto - units, from);
+                found.pages = __shfl_sync(0xffffffffu, pg, from);
+                found.first = __shfl_sync(0xffffffffu, f, from);
+                found.members = __shfl_sync(0xffffffffu, m, from);
+                found.lead = __shfl_sync(0xffffffffu, head, from);
+            }
+            total = __shfl_sync(0xffffffffu, upto, 31);
+        }
+        return found;
+    }
+    // where the parts of a token row and kv head are (the first one's first row, and their number), by a whole warp
+    __device__ __forceinline__ int2 where(int tok, int kvh, int nkv, int G, int clusters, int lane) const {
+        const int which = group_of[tok], mine = member_of[tok];
+        if (which < 0) return make_int2(0, 0);
+        int total;
+        const Group g = find(-1, which, nkv, G, lane, total);
+        const int tm = tile_members(g.members, G), p = per(total, clusters), tile = mine / tm;
+        const int u0 = g.before + (tile * nkv + kvh) * g.pages, c0 = u0 / p, c1 = (u0 + g.pages - 1) / p;
+        return make_int2(nkv * G * (g.first + tile * tm) + kvh * G * min(tm, g.members - tile * tm) + c0 * SHARED_ROWS + (mine - tile * tm) * G,
+                         c1 - c0 + 1);
+    }
 };
 
 // The parts of one token row and kv head: `count` of them, 128 rows apart.
@@ -193,21 +232,7 @@ struct SharedParts {
     const float* o;
     const float2* ml;
     int count;
-    __device__ __forceinline__ void find(const AttnShared& a, int tok, int kvh, int nkv, int G, int dv) {
-        const SharedPlan p(a);
-        const int g = p.group_of[tok];
-        count = 0;
-        if (g < 0) return;
-        const int pg = p.pages[g], per = p.per(p.units_before(p.groups, nkv, G), a.clusters), tm = p.tile_members(g, G);
-        const int mine = p.member_of[tok], tile = mine / tm, inside = mine - tile * tm;
-        const int u0 = p.units_before(g, nkv, G) + (tile * nkv + kvh) * pg;
-        const int c0 = u0 / per, c1 = (u0 + pg - 1) / per;
-        const size_t row = (size_t)nkv * G * (p.first[g] + tile * tm) + (size_t)kvh * G * min(tm, p.members(g) - tile * tm) +
-                           (size_t)c0 * SHARED_ROWS + inside * G;
-        o = a.part_o + row * dv;
-        ml = a.part_ml + row;
-        count = c1 - c0 + 1;
-    }
+    __device__ __forceinline__ SharedParts(const AttnShared& a, int2 w, int dv) : o(a.part_o + (size_t)w.x * dv), ml(a.part_ml + w.x), count(w.y) {}
     // One warp's share of the parts (every `step`-th from k0 on) of the kv head's G rows, added up into sm_o [G][DV] and sm_ml
     // [G][2], four columns a lane; eight rows of parts are asked for at a time, whichever row or part they are of.
     template <int DV>
@@ -283,6 +308,7 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
     uint64_t* full = (uint64_t*)(smem + STAGES * STAGE_BYTES);
     uint64_t* empty = full + STAGES;
     volatile int* abort_flag = (volatile int*)(empty + STAGES);
+    int2* parts_at = (int2*)(empty + STAGES + 1);                                     // (SHARED) where the prefix's parts are
     float* recv_o = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES + 256);      // see ATT_RECV_BYTES
     float* recv_ml = recv_o + ATT_RECV_O / 4;
 
@@ -306,6 +332,7 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
     // and waits for it only before the page that holds the new token; the consumers wait before they read q.
     const int b = seq_of_token[tok];
     const int pos = b >= 0 ? positions[tok] : -1;
+    const int prefix = SHARED ? SharedPlan(shared).pages_of[tok] : 0;
 
     int lo = 0, p_begin = 0, p_end = 0;
     if (b >= 0) {
@@ -313,18 +340,13 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
         int first = lo / PAGE;
         const int last = pos / PAGE;
         if constexpr (SHARED) {
-            const SharedPlan plan(shared);
-            const int group = plan.group_of[tok];
-            if (group >= 0) first = max(first, plan.pages[group]);
+            first = max(first, prefix);
         }
         const int pps = (last - first + 1 + nsplit - 1) / nsplit;
         p_begin = first + split * pps;
         p_end = min(last + 1, p_begin + pps);
     }
     const int npg = max(0, p_end - p_begin);
-
-    SharedParts parts;
-    if constexpr (SHARED) parts.find(shared, tok, kvh, nkv, G, dv);
 
     float o[NT][4];
 #pragma unroll
@@ -349,6 +371,12 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
 #pragma unroll
                 for (int hf = 0; hf < HV; ++hf) tma::load_2d(dst + (HK + hf) * BOX_BYTES, &tmV, &full[s], hf * 64, row);
             }
+        }
+        if constexpr (SHARED) {
+            // (while the others work on the pages)
+            __syncwarp();
+            const int2 w = SharedPlan(shared).where(tok, kvh, nkv, G, shared.clusters, lane);
+            if (lane == 0) *parts_at = w;
         }
     } else if (npg > 0) {
         // Q fragments in the standard A layout: row = head of the group, k = head dimension
@@ -461,7 +489,7 @@ __global__ void __launch_bounds__(160) attn_decode_tma_kernel(
         }
     }
     if constexpr (SHARED)
-        parts.add_up<DV>(split * 5 + warp, 5 * nsplit, G, dv, lane, sm_o + (4 + warp) * 16 * DV, sm_ml + (4 + warp) * 16 * 2);
+        SharedParts(shared, *parts_at, dv).add_up<DV>(split * 5 + warp, 5 * nsplit, G, dv, lane, sm_o + (4 + warp) * 16 * DV, sm_ml + (4 + warp) * 16 * 2);
     __syncthreads();
     for (int idx = threadIdx.x; idx < G * dv; idx += blockDim.x) {
         const int r = idx / dv, c = idx - r * dv;

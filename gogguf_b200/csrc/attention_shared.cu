@@ -51,9 +51,11 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = nq / nkv;
     const SharedPlan plan(shared);
-    const int total = plan.units_before(plan.groups, nkv, G), per = plan.per(total, shared.clusters);
-    const int rank = (int)blockIdx.z, u_begin = min((int)blockIdx.x * per, total), u_end = min(u_begin + per, total);
     pdl_launch();                                   // (the whole grid is resident at once: the rule in common.cuh)
+    int total;
+    plan.find(-1, -1, nkv, G, lane, total);
+    const int per = plan.per(total, shared.clusters);
+    const int rank = (int)blockIdx.z, u_begin = min((int)blockIdx.x * per, total), u_end = min(u_begin + per, total);
     if (u_begin >= u_end) {                         // (every kernel of a step waits for the one before it, too)
         pdl_wait();
         return;
@@ -82,24 +84,21 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
     if (!aligned && threadIdx.x == 0) atomicCAS(status, 0, 29);
 
     // A cluster's units are cut where the (tile, kv head) changes; of a run's pages, this CTA takes its share.
-    struct Run { int first, members, head, page0, pages, all; size_t row0; };
+    struct Run { int first, members, head, page0, pages, all, lead; size_t row0; };
     auto run_at = [&](int u) -> Run {
-        int g = 0, before = 0;
-        for (; g + 1 < plan.groups; ++g) {
-            const int n = plan.pages[g] * plan.tiles(g, G) * nkv;
-            if (u < before + n) break;
-            before += n;
-        }
-        const int pg = plan.pages[g], tm = plan.tile_members(g, G), rel = u - before;
-        const int th = rel / pg, tile = th / nkv, page = rel - th * pg;
+        int all;
+        const SharedPlan::Group g = plan.find(u, -1, nkv, G, lane, all);
+        const int tm = plan.tile_members(g.members, G), rel = u - g.before;
+        const int th = rel / g.pages, tile = th / nkv, page = rel - th * g.pages;
         Run r;
         r.head = th - tile * nkv;
-        r.all = min(pg - page, u_end - u);
+        r.all = min(g.pages - page, u_end - u);
         const int a = r.all * rank / SHARED_CLUSTER, e = r.all * (rank + 1) / SHARED_CLUSTER;
         r.page0 = page + a;
         r.pages = e - a;
-        r.first = plan.first[g] + tile * tm;
-        r.members = min(tm, plan.first[g + 1] - r.first);
+        r.first = g.first + tile * tm;
+        r.members = min(tm, g.members - tile * tm);
+        r.lead = g.lead;
         r.row0 = (size_t)nkv * G * r.first + (size_t)r.head * G * r.members + (size_t)blockIdx.x * SHARED_ROWS;
         return r;
     };
@@ -118,7 +117,7 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
             // The prefix's pages were written by earlier steps (this step's tokens go to pages of the rows' own), so they are
             // streamed before the kernel before this one has finished.
             if (lane == 0 && ok) {
-                const int* pt = page_table + (size_t)seq_of_token[plan.rows[r.first]] * max_pages;
+                const int* pt = page_table + (size_t)seq_of_token[r.lead] * max_pages;
                 for (int i = 0; i < r.pages; ++i, ++j) {
                     const int s = j & 1;
                     const uint32_t ph = (uint32_t)((j >> 1) & 1) ^ 1u;
@@ -179,7 +178,7 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
             const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
             const bool live = row < rows, idle = warp * 32 >= rows;     // (a warp without rows only keeps the pace)
             float m_used = -INFINITY, l = 0.f;
-            if (run == 0) pdl_wait();                          // q
+            if (run == 0) pdl_wait();                          // q, and the scratch is free
             if (ok && r.pages > 0) {
                 // Q into its swizzled tile: row r of a box is 128 bytes, 16-byte chunk c at place c ^ (r & 7)
                 const int member = live ? row / G : 0;
@@ -304,21 +303,20 @@ __global__ void __launch_bounds__(192) shared_prefix_kernel(
             // the rows go round the cluster's CTAs and their warps; the shares are added in rank order
             const uint32_t os = tma::smem_u32(smem), ml = tma::smem_u32(bars + 32);
             for (int x = rank + warp * SHARED_CLUSTER; x < rows; x += 6 * SHARED_CLUSTER) {
-                float m[SHARED_CLUSTER], l[SHARED_CLUSTER], M = -INFINITY;
+                float m[SHARED_CLUSTER], l[SHARED_CLUSTER], M = -INFINITY, sum = 0.f;
+                float4 v[SHARED_CLUSTER], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                // (all at once, whether a share has left something or not: one way across the cluster instead of two)
 #pragma unroll
                 for (int k = 0; k < SHARED_CLUSTER; ++k) attn_remote(ml + 8u * (uint32_t)x, k, m[k], l[k]);
-                float4 v[SHARED_CLUSTER], acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < SHARED_CLUSTER; ++k)
+                    v[k] = attn_remote4(os + 16u * (uint32_t)(x * (DV / 4) + ((DV < 128 ? lane & (DV / 4 - 1) : lane) ^ (x & 7))), k);
+#pragma unroll
+                for (int k = 0; k < SHARED_CLUSTER; ++k) M = fmaxf(M, m[k]);
 #pragma unroll
                 for (int k = 0; k < SHARED_CLUSTER; ++k) {
-                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    // (a share without pages has left nothing)
-                    if (m[k] != -INFINITY && lane < DV / 4) v[k] = attn_remote4(os + 16u * (uint32_t)(x * (DV / 4) + (lane ^ (x & 7))), k);
-                    M = fmaxf(M, m[k]);
-                }
-#pragma unroll
-                for (int k = 0; k < SHARED_CLUSTER; ++k) {
-                    const float f = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - M);
+                    if (m[k] == -INFINITY) continue;
+                    const float f = fast_exp2(m[k] - M);
                     sum = fmaf(l[k], f, sum);
                     acc.x = fmaf(v[k].x, f, acc.x); acc.y = fmaf(v[k].y, f, acc.y); acc.z = fmaf(v[k].z, f, acc.z); acc.w = fmaf(v[k].w, f, acc.w);
                 }
@@ -379,8 +377,8 @@ long long part_rows(int ntok, int nq) { return (long long)nq * ntok + (long long
 
 }  // namespace
 
-// Decode attention (see gg_attn_decode_tma) of a step with shared prefixes: plan as at AttnShared, part: gg_attn_shared
-// scratch of (nq ntok + 128 * 32) (dv + 2) floats, 16-byte aligned.  splits: 1, 2, 4 or 8 CTAs share a row's own pages.
+// Decode attention (see gg_attn_decode_tma) of a step with shared prefixes: plan as at AttnShared, part: scratch of
+// (nq ntok + 128 * 32) (dv + 2) floats, 16-byte aligned.  splits: 1, 2, 4 or 8 CTAs share a row's own pages.
 // status: codes 71-79 name the prefix kernel's wait that ran out, 11 and 12 the other's.
 GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_pool, void* out, const int* positions,
                              const int* seq_of_token, const int* page_table, int max_pages, int page_size, int n_pages, const int* plan,
@@ -392,7 +390,7 @@ GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_po
         return GG_ERR_ARG;
     if ((((uintptr_t)q) & 15) || (((uintptr_t)k_pool) & 15) || (((uintptr_t)v_pool) & 15) || (((uintptr_t)part) & 15)) return GG_ERR_ARG;
     const long long rows = part_rows(ntok, nq);
-    if (part == nullptr || part_floats < rows * (dv + 2)) return GG_ERR_ARG;
+    if (part == nullptr || part_floats < rows * (dv + 2) || rows > 0x7fffffffll) return GG_ERR_ARG;
     CUtensorMap tk, tv;
     int rc;
     const unsigned long long pool_rows = (unsigned long long)n_pages * nkv * PAGE;

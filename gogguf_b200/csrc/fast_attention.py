@@ -100,14 +100,14 @@ class PrefixPlan:
     own positions.  A plan serves all layers of a step that read through the same page table."""
 
     def __init__(self, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, device):
-        host = torch.empty(5 + 5 * n_tokens, dtype=torch.int32)
+        host = torch.empty(5 + 7 * n_tokens, dtype=torch.int32)
         self.pack(groups, n_tokens, host.numpy())
         self.n_tokens = n_tokens
         self.words = host.to(device)
 
     @staticmethod
     def words_for(n_tokens: int) -> int:
-        return 5 + 5 * n_tokens
+        return 5 + 7 * n_tokens
 
     @classmethod
     def over(cls, words: torch.Tensor, n_tokens: int) -> "PrefixPlan":
@@ -124,23 +124,25 @@ class PrefixPlan:
         appear twice, and groups without a row or page."""
         if n_tokens <= 0:
             raise KernelError("shared attention: a plan needs at least one token row")
-        first, pages = out[4:5 + n_tokens], out[5 + n_tokens:5 + 2 * n_tokens]
-        rows, group_of, member_of = (out[5 + k * n_tokens:5 + (k + 1) * n_tokens] for k in (2, 3, 4))
+        first = out[4:5 + n_tokens]
+        pages, lead, rows, pages_of, group_of, member_of = (out[5 + k * n_tokens:5 + (k + 1) * n_tokens] for k in range(1, 7))
+        out[:5 + 7 * n_tokens] = 0
         group_of[:] = -1
-        first[0] = at = 0
+        at = 0
         for g, (members, shared) in enumerate(groups):
             members = list(members)
             if not members or shared <= 0:
                 raise KernelError("shared attention: a group has at least one row and one page")
             if min(members) < 0 or max(members) >= n_tokens or len(set(members)) != len(members) or (group_of[members] >= 0).any():
                 raise KernelError(f"shared attention: rows {members} are not rows of {n_tokens} tokens, or appear twice")
-            first[g], pages[g] = at, shared
+            first[g], pages[g], lead[g] = at, shared, members[0]
             rows[at:at + len(members)] = members
             group_of[members] = g
+            pages_of[members] = shared
             member_of[members] = np.arange(len(members))
             at += len(members)
             first[g + 1] = at
-        out[:4] = (len(groups), 0, 0, 0)
+        out[0] = len(groups)
 
     @classmethod
     def of_pages(cls, pages: Sequence[Sequence[int]], lengths: Sequence[int], page_size: int, device) -> "PrefixPlan":
