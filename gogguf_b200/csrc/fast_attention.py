@@ -53,14 +53,15 @@ def attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page
         status_word(q.device).data_ptr(), stream_ptr())
 
 
-PREFIX_CLUSTERS = 32    # of the kernel over the prefixes (csrc/attention_shared.cu)
+# Runs and rows of a tile of the shared-prefix kernel, and the most token rows it takes (csrc/attention_shared.cu).
+SHARED_RUNS, SHARED_ROWS, SHARED_TOKENS = 148, 256, 1024
 
 
 def shared_scratch(n_tokens: int, nq: int, nkv: int, dv: int) -> int:
-    """Floats of scratch that `attn_decode_shared` needs: the parts' rows, and two numbers beside each."""
+    """Floats of scratch that `attn_decode_shared` needs: the parts' rows, two numbers beside each, and where a row's parts are."""
     if n_tokens <= 0 or nkv <= 0 or nq <= 0 or nq % nkv or dv <= 0:
         raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {dv}, {n_tokens} tokens")
-    return (nq * n_tokens + 128 * PREFIX_CLUSTERS) * (dv + 2)
+    return (nq * n_tokens + SHARED_ROWS * SHARED_RUNS) * (dv + 2) + 4 * n_tokens * nkv
 
 
 def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[int], int]]:
@@ -100,14 +101,14 @@ class PrefixPlan:
     own positions.  A plan serves all layers of a step that read through the same page table."""
 
     def __init__(self, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, device):
-        host = torch.empty(5 + 7 * n_tokens, dtype=torch.int32)
+        host = torch.empty(self.words_for(n_tokens), dtype=torch.int32)
         self.pack(groups, n_tokens, host.numpy())
         self.n_tokens = n_tokens
         self.words = host.to(device)
 
     @staticmethod
     def words_for(n_tokens: int) -> int:
-        return 5 + 7 * n_tokens
+        return 5 + 4 * n_tokens
 
     @classmethod
     def over(cls, words: torch.Tensor, n_tokens: int) -> "PrefixPlan":
@@ -120,29 +121,33 @@ class PrefixPlan:
 
     @classmethod
     def pack(cls, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, out: np.ndarray) -> None:
-        """Write the plan's words (csrc/attention_common.cuh: AttnShared) to `out`; refuses rows that are not the step's, that
+        """Write the plan's words (csrc/attention_shared.cu: SharedArgs) to `out`; refuses rows that are not the step's, that
         appear twice, and groups without a row or page."""
         if n_tokens <= 0:
             raise KernelError("shared attention: a plan needs at least one token row")
         first = out[4:5 + n_tokens]
-        pages, lead, rows, pages_of, group_of, member_of = (out[5 + k * n_tokens:5 + (k + 1) * n_tokens] for k in range(1, 7))
-        out[:5 + 7 * n_tokens] = 0
-        group_of[:] = -1
+        pages, rows, prefix = (out[5 + k * n_tokens:5 + (k + 1) * n_tokens] for k in (1, 2, 3))
+        out[:cls.words_for(n_tokens)] = 0
+        alone = np.ones(n_tokens, dtype=bool)
         at = 0
         for g, (members, shared) in enumerate(groups):
             members = list(members)
             if not members or shared <= 0:
                 raise KernelError("shared attention: a group has at least one row and one page")
-            if min(members) < 0 or max(members) >= n_tokens or len(set(members)) != len(members) or (group_of[members] >= 0).any():
+            if min(members) < 0 or max(members) >= n_tokens or len(set(members)) != len(members) or not alone[members].all():
                 raise KernelError(f"shared attention: rows {members} are not rows of {n_tokens} tokens, or appear twice")
-            first[g], pages[g], lead[g] = at, shared, members[0]
+            pages[g] = shared
             rows[at:at + len(members)] = members
-            group_of[members] = g
-            pages_of[members] = shared
-            member_of[members] = np.arange(len(members))
+            prefix[at:at + len(members)] = shared
+            alone[members] = False
             at += len(members)
             first[g + 1] = at
-        out[0] = len(groups)
+        count = len(groups)
+        if at < n_tokens:                            # rows that share nothing: a group without shared pages
+            rows[at:] = np.nonzero(alone)[0]
+            count += 1
+            first[count] = n_tokens
+        out[0] = count
 
     @classmethod
     def of_pages(cls, pages: Sequence[Sequence[int]], lengths: Sequence[int], page_size: int, device) -> "PrefixPlan":
@@ -162,10 +167,10 @@ class PrefixPlan:
 
 
 def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, page_size, plan: PrefixPlan, scratch, nq, nkv, d, scale,
-                       sink=None, out_scale: float = 1.0, dv: Optional[int] = None, gate=None, splits: Optional[int] = None) -> None:
-    """Decode attention (`attn_decode_tma`, without windows and chunks) of the plan's token rows: the keys and values of a
-    prefix that several rows share are read once for all of them, in two kernels.  scratch: float32, `shared_scratch` of it;
-    two launches that may run at the same time need scratch of their own.  splits (1, 2, 4, 8): CTAs that share a row's own pages."""
+                       sink=None, out_scale: float = 1.0, dv: Optional[int] = None, gate=None) -> None:
+    """Decode attention (`attn_decode_tma`, without windows and chunks) of the plan's token rows: every page that they read is
+    read once per kv head, whoever reads it, in two kernels.  scratch: float32, `shared_scratch` of it; two launches that may run
+    at the same time need scratch of their own."""
     from .tcgen05_gemm import status_word
     dv = d if dv is None else int(dv)
     T = plan.n_tokens
@@ -187,6 +192,8 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
     room = shared_scratch(T, nq, nkv, dv)
     if scratch.numel() < room:
         raise KernelError(f"shared attention: scratch must have {room} elements")
+    if T > SHARED_TOKENS:
+        raise KernelError(f"shared attention: {T} token rows, and at most {SHARED_TOKENS} are taken")
     if (q.numel() < T * nq * d or out.numel() < T * nq * dv or positions.numel() < T or seq_of_token.numel() < T or table.dim() != 2
             or k_pool.shape != (k_pool.shape[0], nkv, page_size, d) or v_pool.shape != (k_pool.shape[0], nkv, page_size, dv)):
         raise KernelError("shared attention: shapes disagree")
@@ -200,11 +207,9 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
                 or gate.get_device() != here):
             raise KernelError(f"shared attention: a gate is bfloat16 with {T} rows of {nq * dv}, on the current CUDA device")
         p_gate, ldg = gate.data_ptr(), gate.stride(0)
-    if splits is None:
-        splits = min(8, decode_tma_splits(T, nkv, table.shape[1] * page_size, cluster=True))
     kernel("attention_shared", "gg_attn_decode_shared")(
         p_q, p_k, p_v, p_out, p_pos, p_seq, p_table, table.shape[1], page_size, k_pool.shape[0], p_plan, T, nq, nkv, d, dv, float(scale),
-        int(splits), p_sink, float(out_scale), p_gate, ldg, p_scratch, scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
+        p_sink, float(out_scale), p_gate, ldg, p_scratch, scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
 
 
 def attn_prefill(q, k_pool, v_pool, out, cu_seqlens, ctx_lens, seq_of_token, table, page_size, n_seqs,

@@ -123,20 +123,19 @@ def test_matches_the_formula(case):
     assert (s.out[s.T:] == 7.0).all()                   # rows behind the last one stay as they were
 
 
-@pytest.mark.parametrize("splits", [1, 2, 4, 8])
-def test_own_pages_in_shares(splits):
-    for kw in (dict(groups=[3, 2], prefix=[4, 9], own=(1, 700), nq=32, nkv=4, d=128), dict(groups=[4], prefix=[3], own=(1, 300), nq=32, nkv=2, d=128),
-               dict(groups=[4], prefix=[3], own=(1, 300), nq=8, nkv=2, d=64)):
-        s = Setup(**kw, seed=splits)
-        check(s.run(splits=splits, out_scale=0.5), *s.want(out_scale=0.5))
+@pytest.mark.parametrize("kw", [dict(groups=[3, 2], prefix=[4, 9], own=(1, 700), nq=32, nkv=4, d=128),
+                                dict(groups=[4], prefix=[3], own=(1, 300), nq=32, nkv=2, d=128),
+                                dict(groups=[70, 1, 1], prefix=[2, 30, 1], own=(1, 300), nq=24, nkv=8, d=128),
+                                dict(groups=[300], prefix=[1], own=(1, 4), nq=4, nkv=4, d=64)])
+def test_own_pages_and_a_factor(kw):
+    s = Setup(**kw)
+    check(s.run(out_scale=0.5), *s.want(out_scale=0.5))
 
 
-def test_a_plan_without_groups_is_the_unshared_step():
+def test_rows_that_share_nothing():
     from gogguf_b200.csrc import fast_attention as A
-    s = Setup(groups=[1, 1, 1], prefix=[3, 5, 1], own=(1, 90), nq=8, nkv=2, d=128)
-    got = s.run(plan=A.PrefixPlan([], 3, "cuda"), splits=2).clone()
-    A.attn_decode_tma(s.q, s.k, s.v, s.out, s.positions, s.rows, s.table, PAGE, 3, 8, 2, 128, s.scale, 0, 2, cluster=True)
-    assert torch.equal(got, s.out[:3])
+    s = Setup(groups=[1] * 37, prefix=[1 + i % 5 for i in range(37)], own=(1, 90), nq=8, nkv=2, d=128)
+    check(s.run(plan=A.PrefixPlan([], 37, "cuda")), *s.want())
 
 
 def test_padding_rows_and_two_tokens_of_a_sequence():
@@ -204,8 +203,10 @@ def test_refusals_on_the_device():
     plan = A.PrefixPlan.of_pages(s.lists, s.lengths, PAGE, "cuda")
     with pytest.raises(KernelError, match="scratch"):
         s.run(scratch=torch.empty(100, device="cuda"))
-    with pytest.raises(KernelError):
-        s.run(plan=plan, splits=3)
+    with pytest.raises(KernelError, match="plan of"):
+        A.PrefixPlan.over(plan.words, 3)
+    with pytest.raises(KernelError, match="1024"):
+        s.run(plan=A.PrefixPlan([], 1025, "cuda"), scratch=torch.empty(A.shared_scratch(1025, 4, 2, 64), device="cuda"))
     with pytest.raises(KernelError, match="plan"):
         s.run(plan=A.PrefixPlan.of_pages(s.lists, s.lengths, PAGE, "cpu"))
     with pytest.raises(KernelError, match="sink"):
