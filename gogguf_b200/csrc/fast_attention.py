@@ -53,15 +53,15 @@ def attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page
         status_word(q.device).data_ptr(), stream_ptr())
 
 
-# Runs and rows of a tile of the shared-prefix kernel, and the most token rows it takes (csrc/attention_shared.cu).
-SHARED_RUNS, SHARED_ROWS, SHARED_TOKENS = 148, 256, 1024
+# Runs over the prefixes and rows of a tile of the shared-prefix kernel (csrc/attention_shared.cu).
+SHARED_RUNS, SHARED_ROWS = 296, 128
 
 
 def shared_scratch(n_tokens: int, nq: int, nkv: int, dv: int) -> int:
-    """Floats of scratch that `attn_decode_shared` needs: the parts' rows, two numbers beside each, and where a row's parts are."""
+    """Floats of scratch that `attn_decode_shared` needs: the parts' rows, and two numbers beside each."""
     if n_tokens <= 0 or nkv <= 0 or nq <= 0 or nq % nkv or dv <= 0:
         raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {dv}, {n_tokens} tokens")
-    return (nq * n_tokens + SHARED_ROWS * SHARED_RUNS) * (dv + 2) + 4 * n_tokens * nkv
+    return (nq * n_tokens + SHARED_ROWS * SHARED_RUNS) * (dv + 2)
 
 
 def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[int], int]]:
@@ -98,25 +98,27 @@ def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[i
 class PrefixPlan:
     """Which token rows of a decode step read which prefix together, as `attn_decode_shared` takes it: `groups` is a list of
     (token rows, leading pages that are the same in all their sequences).  Every shared page must lie wholly before its rows'
-    own positions.  A plan serves all layers of a step that read through the same page table."""
+    own positions.  A plan serves all layers of a step that read through the same page table.  `own_pages`: the most pages that a
+    row reads beside the shared ones, where that is known."""
 
-    def __init__(self, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, device):
+    def __init__(self, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, device, own_pages: Optional[int] = None):
         host = torch.empty(self.words_for(n_tokens), dtype=torch.int32)
         self.pack(groups, n_tokens, host.numpy())
         self.n_tokens = n_tokens
         self.words = host.to(device)
+        self.own_pages = own_pages
 
     @staticmethod
     def words_for(n_tokens: int) -> int:
-        return 5 + 4 * n_tokens
+        return 5 + 7 * n_tokens
 
     @classmethod
-    def over(cls, words: torch.Tensor, n_tokens: int) -> "PrefixPlan":
+    def over(cls, words: torch.Tensor, n_tokens: int, own_pages: Optional[int] = None) -> "PrefixPlan":
         """A plan whose words are (or will be) on the device already, packed by `pack`."""
         plan = cls.__new__(cls)
         if words.dtype != torch.int32 or words.numel() != cls.words_for(n_tokens) or not words.is_contiguous():
             raise KernelError(f"shared attention: a plan of {n_tokens} tokens has {cls.words_for(n_tokens)} int32 words")
-        plan.n_tokens, plan.words = n_tokens, words
+        plan.n_tokens, plan.words, plan.own_pages = n_tokens, words, own_pages
         return plan
 
     @classmethod
@@ -126,28 +128,24 @@ class PrefixPlan:
         if n_tokens <= 0:
             raise KernelError("shared attention: a plan needs at least one token row")
         first = out[4:5 + n_tokens]
-        pages, rows, prefix = (out[5 + k * n_tokens:5 + (k + 1) * n_tokens] for k in (1, 2, 3))
+        pages, lead, rows, pages_of, group_of, member_of = (out[5 + k * n_tokens:5 + (k + 1) * n_tokens] for k in range(1, 7))
         out[:cls.words_for(n_tokens)] = 0
-        alone = np.ones(n_tokens, dtype=bool)
+        group_of[:] = -1
         at = 0
         for g, (members, shared) in enumerate(groups):
             members = list(members)
             if not members or shared <= 0:
                 raise KernelError("shared attention: a group has at least one row and one page")
-            if min(members) < 0 or max(members) >= n_tokens or len(set(members)) != len(members) or not alone[members].all():
+            if min(members) < 0 or max(members) >= n_tokens or len(set(members)) != len(members) or (group_of[members] >= 0).any():
                 raise KernelError(f"shared attention: rows {members} are not rows of {n_tokens} tokens, or appear twice")
-            pages[g] = shared
+            pages[g], lead[g] = shared, members[0]
             rows[at:at + len(members)] = members
-            prefix[at:at + len(members)] = shared
-            alone[members] = False
+            group_of[members] = g
+            pages_of[members] = shared
+            member_of[members] = np.arange(len(members))
             at += len(members)
             first[g + 1] = at
-        count = len(groups)
-        if at < n_tokens:                            # rows that share nothing: a group without shared pages
-            rows[at:] = np.nonzero(alone)[0]
-            count += 1
-            first[count] = n_tokens
-        out[0] = count
+        out[0] = len(groups)
 
     @classmethod
     def of_pages(cls, pages: Sequence[Sequence[int]], lengths: Sequence[int], page_size: int, device) -> "PrefixPlan":
@@ -163,14 +161,19 @@ class PrefixPlan:
         table = np.full((len(pages), max(1, max(len(p) for p in pages))), -1, dtype=np.int64)
         for r, p in enumerate(pages):
             table[r, :len(p)] = p
-        return cls(shared_groups(table, [max(0, (n - 1) // page_size) for n in lengths]), len(pages), device)
+        groups = shared_groups(table, [max(0, (n - 1) // page_size) for n in lengths])
+        own = [-(-n // page_size) for n in lengths]
+        for rows, shared in groups:
+            for r in rows:
+                own[r] -= shared
+        return cls(groups, len(pages), device, own_pages=max(own))
 
 
 def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, page_size, plan: PrefixPlan, scratch, nq, nkv, d, scale,
-                       sink=None, out_scale: float = 1.0, dv: Optional[int] = None, gate=None) -> None:
-    """Decode attention (`attn_decode_tma`, without windows and chunks) of the plan's token rows: every page that they read is
-    read once per kv head, whoever reads it, in two kernels.  scratch: float32, `shared_scratch` of it; two launches that may run
-    at the same time need scratch of their own."""
+                       sink=None, out_scale: float = 1.0, dv: Optional[int] = None, gate=None, splits: Optional[int] = None) -> None:
+    """Decode attention (`attn_decode_tma`, without windows and chunks) of the plan's token rows: the keys and values of a prefix
+    that several rows share are read once for all of them, in two kernels.  scratch: float32, `shared_scratch` of it; two launches
+    that may run at the same time need scratch of their own.  splits (1, 2, 4, 8): CTAs that share a row's own pages."""
     from .tcgen05_gemm import status_word
     dv = d if dv is None else int(dv)
     T = plan.n_tokens
@@ -192,8 +195,6 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
     room = shared_scratch(T, nq, nkv, dv)
     if scratch.numel() < room:
         raise KernelError(f"shared attention: scratch must have {room} elements")
-    if T > SHARED_TOKENS:
-        raise KernelError(f"shared attention: {T} token rows, and at most {SHARED_TOKENS} are taken")
     if (q.numel() < T * nq * d or out.numel() < T * nq * dv or positions.numel() < T or seq_of_token.numel() < T or table.dim() != 2
             or k_pool.shape != (k_pool.shape[0], nkv, page_size, d) or v_pool.shape != (k_pool.shape[0], nkv, page_size, dv)):
         raise KernelError("shared attention: shapes disagree")
@@ -207,9 +208,12 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
                 or gate.get_device() != here):
             raise KernelError(f"shared attention: a gate is bfloat16 with {T} rows of {nq * dv}, on the current CUDA device")
         p_gate, ldg = gate.data_ptr(), gate.stride(0)
+    if splits is None:
+        own = table.shape[1] if plan.own_pages is None else plan.own_pages
+        splits = min(8, decode_tma_splits(T, nkv, own * page_size, cluster=True))
     kernel("attention_shared", "gg_attn_decode_shared")(
         p_q, p_k, p_v, p_out, p_pos, p_seq, p_table, table.shape[1], page_size, k_pool.shape[0], p_plan, T, nq, nkv, d, dv, float(scale),
-        p_sink, float(out_scale), p_gate, ldg, p_scratch, scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
+        int(splits), p_sink, float(out_scale), p_gate, ldg, p_scratch, scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
 
 
 def attn_prefill(q, k_pool, v_pool, out, cu_seqlens, ctx_lens, seq_of_token, table, page_size, n_seqs,

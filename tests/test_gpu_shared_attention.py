@@ -129,7 +129,8 @@ def test_matches_the_formula(case):
                                 dict(groups=[300], prefix=[1], own=(1, 4), nq=4, nkv=4, d=64)])
 def test_own_pages_and_a_factor(kw):
     s = Setup(**kw)
-    check(s.run(out_scale=0.5), *s.want(out_scale=0.5))
+    for splits in (None, 1, 2, 4, 8):
+        check(s.run(out_scale=0.5, splits=splits), *s.want(out_scale=0.5))
 
 
 def test_rows_that_share_nothing():
@@ -205,8 +206,8 @@ def test_refusals_on_the_device():
         s.run(scratch=torch.empty(100, device="cuda"))
     with pytest.raises(KernelError, match="plan of"):
         A.PrefixPlan.over(plan.words, 3)
-    with pytest.raises(KernelError, match="1024"):
-        s.run(plan=A.PrefixPlan([], 1025, "cuda"), scratch=torch.empty(A.shared_scratch(1025, 4, 2, 64), device="cuda"))
+    with pytest.raises(KernelError):
+        s.run(plan=plan, splits=3)
     with pytest.raises(KernelError, match="plan"):
         s.run(plan=A.PrefixPlan.of_pages(s.lists, s.lengths, PAGE, "cpu"))
     with pytest.raises(KernelError, match="sink"):

@@ -70,14 +70,21 @@ def test_groups_of_random_trees_share_what_they_say(seed):
 def test_plan_words():
     plan = A.PrefixPlan([([3, 0], 7), ([2], 1)], 5, "cpu")
     w = plan.words.tolist()
-    assert len(w) == A.PrefixPlan.words_for(5) == 25 and w[0] == 3      # the third: rows that share nothing
-    assert w[4:8] == [0, 2, 3, 5]                   # first members
-    assert w[10:13] == [7, 1, 0]                    # pages
-    assert w[15:20] == [3, 0, 2, 1, 4]              # rows
-    assert w[20:25] == [7, 7, 1, 0, 0]              # their pages
-    assert A.PrefixPlan([], 3, "cpu").words.tolist() == [1, 0, 0, 0, 0, 3, 0, 0] + [0] * 3 + [0, 1, 2] + [0] * 3
-    full = A.PrefixPlan([([1, 0], 2)], 2, "cpu").words.tolist()
-    assert full[0] == 1 and full[4:7] == [0, 2, 0] and full[9:11] == [1, 0]
+    assert len(w) == A.PrefixPlan.words_for(5) == 40 and w[0] == 2
+    assert w[4:7] == [0, 2, 3]                      # first members
+    assert w[10:12] == [7, 1]                       # pages
+    assert w[15:17] == [3, 2]                       # first rows
+    assert w[20:23] == [3, 0, 2]                    # rows
+    assert w[25:30] == [7, 0, 1, 7, 0]              # pages of each row
+    assert w[30:35] == [0, -1, 1, 0, -1]            # group of each row
+    assert [w[35], w[37], w[38]] == [1, 0, 0]       # place among the members
+    empty = A.PrefixPlan([], 3, "cpu").words.tolist()
+    assert empty == [0] * 20 + [-1] * 3 + [0] * 3
+
+
+def test_own_pages():
+    assert A.PrefixPlan.of_pages([[0, 1, 2], [0, 1, 3], [5]], [140, 170, 3], 64, "cpu").own_pages == 1
+    assert A.PrefixPlan.of_pages([[0, 1, 2, 7], [0, 1, 3], [5]], [193, 170, 3], 64, "cpu").own_pages == 2
 
 
 @pytest.mark.parametrize("groups, n", [([([0, 5], 2)], 5), ([([-1, 2], 2)], 5), ([([1, 1], 2)], 5), ([([0, 1], 2), ([1, 2], 2)], 5),
@@ -95,7 +102,7 @@ def test_of_pages_refuses():
     with pytest.raises(KernelError):
         A.PrefixPlan.of_pages([], [], 64, "cpu")
     with pytest.raises(KernelError):
-        A.PrefixPlan.over(torch.zeros(24, dtype=torch.int32), 5)
+        A.PrefixPlan.over(torch.zeros(39, dtype=torch.int32), 5)
 
 
 def test_attention_refuses_what_is_not_on_the_device():
