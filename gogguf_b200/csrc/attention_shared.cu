@@ -1,24 +1,110 @@
-// Decode attention of a step some of whose rows share a prefix: the prefix's keys and values are read once for all its readers,
-// as the rows of one tensor-core product, and every row's own positions by the decode kernel that a step without prefixes uses
-// (attention_common.cuh), which adds the prefix's parts at its end.  With s_j = scale q . k_j, a part over a run of positions is
+// Decode attention of a step some of whose rows share a prefix: the prefix's keys and values are read once for all its readers.
+//
+// With s_j = scale q . k_j, a part over a run of positions is
 //     m >= some s_j of the run,   l = sum e^(s_j - m),   O = sum e^(s_j - m) v_j
-// and parts add up as O = sum e^(m_i - m) O_i, l alike, whatever the m_i are; the output is O / l.
+// and parts add up as O = sum e^(m_i - m) O_i, l alike, whatever the m_i are; the output is O / l.  Two kernels make the parts, side
+// by side, so that what computes and what waits for memory share the SMs; a third adds them, always in the same order.
 //
-// The prefix kernel: a tile is up to 128 rows, members of a group times the query heads of a kv head.  Per page of 64 keys
-// S = Q K^T (tcgen05.mma 128 x 64 x 16) lands in tensor memory, four warps take a row per thread, leave P as bfloat16 where S was
-// and O += P V accumulates in tensor memory, as in the prefill kernel (attention_fast.cu), without its masks: every reader sees
-// every key of the prefix.  All (group, tile, kv head)s' pages are one line of work cut into equal runs, one per CTA, so that
-// neither the number of readers nor that of kv heads leaves an SM without work, and the grid is the same for every plan: a
-// captured step replays with other groups.
+// Prefixes: a tile is up to 128 rows of a tensor-core product, members of a group times the query heads of a kv head.  Per page
+// of 64 keys S = Q K^T (tcgen05.mma 128 x 64 x 16) lands in tensor memory, four warps take a row per thread, leave P as bfloat16
+// where S was and O += P V accumulates in tensor memory, as in the prefill kernel (attention_fast.cu), without its masks: every
+// reader sees every key of the prefix.  All (group, tile, kv head)s' pages are one line of work cut into equal runs, one per CTA,
+// so that neither the number of readers nor that of kv heads leaves an SM without work, and the grid is the same for every plan:
+// a captured step replays with other groups.
 //
-// (Both as one kernel, whose CTAs are of the two kinds: a CTA of a kernel that allocates tensor memory keeps others off its SM
-// until it has done so, so that the rows' CTAs, which never do, ran one an SM instead of two.  A row's own pages as pages of the
-// prefix's product, seen by its rows only: they took the tensor core as long as any page.)
+// A row's own positions: a CTA a (token row, kv head, share), on mma.sync with the query heads as rows, as the decode kernel of a
+// step without prefixes does it (attention_fast.cu).  (As rows of the prefix's product, a page of a member's own took the tensor
+// core as long as one of the prefix: 64 rows with up to 500 positions of their own on 2,048 were 44 us.  As CTAs of the prefix's
+// kernel they ran one an SM: a CTA of a kernel that allocates tensor memory keeps others of it off its SM until it has done so.)
 #include "attention_common.cuh"
 
 namespace {
 
-constexpr int SHARED_RUNS = 296;      // two CTAs per SM
+constexpr int ROWS = 128;             // of a tile
+constexpr int THREADS = 192;
+constexpr int MAX_RUNS = 296;         // of the prefix kernel: two per SM
+constexpr int OWN_STAGES_BYTES = 96 * 1024;
+
+// The plan, integers of a step, with room for `cap` token rows: how many groups; from word 4 on, per group the place of its first
+// member in `rows` (and one place beyond the last group's), its pages and its first member; `rows`, the members' token rows group
+// by group; per token row the pages that are its prefix (0: none), its group (-1: none) and its place among the group's members.
+// A group's members are cut into tiles of equal size; the units of work are the pages of (group, tile, kv head) in that order, and
+// run c takes `per` of them from c per on.  The part that run c leaves of a (tile, kv head) begins at row row0 + 128 c, with row0
+// the rows of all (tile, kv head)s before: later parts are later in c or in row0, and 128 is the most a part has, so no two
+// overlap.
+struct SharedArgs {
+    const int* plan;
+    int cap, runs, shares;            // token rows that the plan has room for; runs; CTAs that share a row's own pages
+    float* part_o;                    // dv a row: the prefixes' parts, each [dv / 8][its rows][8], then [token row][query head][share][dv]
+    float2* part_ml;                  // [rows]: maximum in log2 units, sum
+    int4* where;                      // [token row][kv head]: first row of its prefix's first part, how many parts there are, the
+                                      // place of its rows in them, and a part's rows
+    int own_row;                      // the first row behind the prefixes' parts
+};
+
+struct SharedPlan {
+    const int *count, *first, *pages, *lead, *rows, *pages_of, *group_of, *member_of;
+    int cap;
+    __device__ __forceinline__ SharedPlan(const SharedArgs& a)
+        : count(a.plan), first(a.plan + 4), pages(first + a.cap + 1), lead(pages + a.cap), rows(lead + a.cap), pages_of(rows + a.cap),
+          group_of(pages_of + a.cap), member_of(group_of + a.cap), cap(a.cap) {}
+    static __device__ __forceinline__ int tiles(int members, int G) {
+        const int most = ROWS / G;
+        return (members + most - 1) / most;
+    }
+    // members of each tile but the last
+    static __device__ __forceinline__ int tile_members(int members, int G) {
+        const int n = tiles(members, G);
+        return (members + n - 1) / n;
+    }
+    // units of a run: as many for each
+    static __device__ __forceinline__ int per(int total, int runs) { return max(1, (total + runs - 1) / runs); }
+
+    // All units, and the group that unit u is of (u < 0: group `which`), by a whole warp: a lane a group.
+    struct Group { int before, pages, first, members, lead; };
+    __device__ __forceinline__ Group find(int u, int which, int nkv, int G, int lane, int& total) const {
+        Group found = {};
+        int groups = 1;
+        total = 0;
+        for (int g0 = 0; g0 < groups; g0 += 32) {
+            const int g = min(g0 + lane, cap - 1);
+            // (asked for before the number of groups is known: beyond the last one stands something that is not used)
+            const int pg = pages[g], f = first[g], m = first[g + 1] - f, head = lead[g];
+            if (g0 == 0) groups = *count;
+            const int units = g0 + lane < groups ? pg * tiles(m, G) * nkv : 0;
+            int upto = units;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            upto += total;
+            const bool it = u < 0 ? g0 + lane == which : u >= upto - units && u < upto;
+            const unsigned mine = __ballot_sync(0xffffffffu, it && units > 0);
+            if (mine != 0) {
+                const int from = __ffs(mine) - 1;
+                found.before = __shfl_sync(0xffffffffu, upto - units, from);
+                found.pages = __shfl_sync(0xffffffffu, pg, from);
+                found.first = __shfl_sync(0xffffffffu, f, from);
+                found.members = __shfl_sync(0xffffffffu, m, from);
+                found.lead = __shfl_sync(0xffffffffu, head, from);
+            }
+            total = __shfl_sync(0xffffffffu, upto, 31);
+        }
+        return found;
+    }
+    // where the parts of a token row and kv head are (see SharedArgs), by a whole warp
+    __device__ __forceinline__ int4 where(int tok, int kvh, int nkv, int G, int runs, int lane) const {
+        const int which = group_of[tok], mine = member_of[tok];
+        if (which < 0) return make_int4(0, 0, 0, 0);
+        int total;
+        const Group g = find(-1, which, nkv, G, lane, total);
+        const int tm = tile_members(g.members, G), p = per(total, runs), tile = mine / tm;
+        const int u0 = g.before + (tile * nkv + kvh) * g.pages, c0 = u0 / p, c1 = (u0 + g.pages - 1) / p;
+        const int members = min(tm, g.members - tile * tm);
+        return make_int4(nkv * G * (g.first + tile * tm) + kvh * G * members + c0 * ROWS, c1 - c0 + 1, (mine - tile * tm) * G, members * G);
+    }
+};
 
 // 32 bytes, a whole sector, at a time
 __device__ __forceinline__ void store8(float* dst, const uint32_t* v) {
@@ -26,19 +112,28 @@ __device__ __forceinline__ void store8(float* dst, const uint32_t* v) {
                  "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
+// What both kinds of CTA are given.
+struct SharedStep {
+    const bf16* q;
+    const int *positions, *seq_of_token, *page_table;
+    int max_pages, nq, nkv, d, dv, n_pages;
+    float scale_log2;
+    int* status;
+};
+
 template <int DK, int DV, bool EXACT>
-__global__ void __launch_bounds__(192, 2) shared_prefix_kernel(
-    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const bf16* q, const int* __restrict__ page_table,
-    const int* __restrict__ seq_of_token, int max_pages, int nq, int nkv, float scale_log2, int n_pages, int* __restrict__ status,
-    int d_, int dv_, const AttnShared shared) {
+__global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                                                                   const SharedStep st, const SharedArgs args) {
+    // (the dynamic segment is the only shared memory and is asked to start on a 1024-byte boundary: two CTAs share an SM)
+    extern __shared__ __align__(1024) uint8_t smem[];
     constexpr int HK = DK / 64, HV = DV / 64;
-    const int d = EXACT ? DK : d_, dv = EXACT ? DV : dv_, G = nq / nkv;
-    constexpr int QBOX = SHARED_ROWS * 64 * 2;             // [64 columns x 128 rows] of Q: 16 KB
+    const int d = EXACT ? DK : st.d, dv = EXACT ? DV : st.dv, nkv = st.nkv, nq = st.nq, G = nq / nkv;
+    const float scale_log2 = st.scale_log2;
+    int* status = st.status;
+    constexpr int QBOX = ROWS * 64 * 2;             // [64 columns x 128 rows] of Q: 16 KB
     constexpr int KBOX = 64 * 64 * 2;               // [64 columns x 64 keys] of K or V: 8 KB
     constexpr int Q_BYTES = HK * QBOX, K_STAGE = HK * KBOX, V_STAGE = HV * KBOX;
     constexpr int TMEM_COLS = 256;                  // two score buffers of 64 columns, then O
-    // (the dynamic segment is the only shared memory and is asked to start on a 1024-byte boundary: two CTAs share an SM)
-    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* Qs = smem;
     uint8_t* Ks = Qs + Q_BYTES;                     // two stages
     uint8_t* Vs = Ks + 2 * K_STAGE;                 // two stages
@@ -55,13 +150,13 @@ __global__ void __launch_bounds__(192, 2) shared_prefix_kernel(
     uint32_t* tmem_slot = (uint32_t*)(bars + 15);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
-    pdl_launch();                                   // (the whole grid is resident at once: the rule in common.cuh)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, run = (int)blockIdx.x;
-    const SharedPlan plan(shared);
+    const SharedPlan plan(args);
     int total;
     plan.find(-1, -1, nkv, G, lane, total);
-    const int per = plan.per(total, shared.runs), u_begin = min(run * per, total), u_end = min(u_begin + per, total);
-    if (u_begin >= u_end) {                         // (every kernel of a step waits for the one before it: common.cuh)
+    const int per = plan.per(total, args.runs), u_begin = min(run * per, total), u_end = min(u_begin + per, total);
+    // The next kernel's CTAs are let in when q is there, which they need and this kernel's work they do not.
+    if (u_begin >= u_end) {
         pdl_wait();
         return;
     }
@@ -101,7 +196,7 @@ __global__ void __launch_bounds__(192, 2) shared_prefix_kernel(
         r.first = g.first + tile * tm;
         r.members = min(tm, g.members - tile * tm);
         r.lead = g.lead;
-        r.row0 = (size_t)nkv * G * r.first + (size_t)r.head * G * r.members + (size_t)run * SHARED_ROWS;
+        r.row0 = (size_t)nkv * G * r.first + (size_t)r.head * G * r.members + (size_t)run * ROWS;
         return r;
     };
     // (a warp goes on or leaves as a whole: what follows a wait is for whole warps)
@@ -109,6 +204,7 @@ __global__ void __launch_bounds__(192, 2) shared_prefix_kernel(
         return __all_sync(0xffffffffu, tma::mbar_wait(bar, phase, abort_flag, status, code));
     };
 
+    if (warp == 5 || (warp == 4 && lane != 0)) { pdl_wait(); pdl_launch(); }
     int j = 0;                                      // pages so far
     if (warp == 4) {
         // The prefix's pages were written by earlier steps (this step's tokens go to pages of the rows' own), so they are
@@ -117,11 +213,11 @@ __global__ void __launch_bounds__(192, 2) shared_prefix_kernel(
             const Piece r = piece_at(u);
             u += r.pages;
             if (lane == 0 && ok) {
-                const int* pt = page_table + (size_t)seq_of_token[r.lead] * max_pages;
+                const int* pt = st.page_table + (size_t)st.seq_of_token[r.lead] * st.max_pages;
                 for (int i = 0; i < r.pages; ++i, ++j) {
                     const int s = j & 1;
                     const uint32_t ph = (uint32_t)((j >> 1) & 1) ^ 1u;
-                    const int row = (gg_page(pt, r.page0 + i, max_pages, PageBounds{n_pages, status}, 54) * nkv + r.head) * PAGE;
+                    const int row = (gg_page(pt, r.page0 + i, st.max_pages, PageBounds{st.n_pages, status}, 54) * nkv + r.head) * PAGE;
                     if (!(ok = tma::mbar_wait(&k_empty[s], ph, abort_flag, status, 71))) break;
                     tma::mbar_expect_tx(&k_full[s], K_STAGE);
 #pragma unroll
@@ -130,12 +226,13 @@ __global__ void __launch_bounds__(192, 2) shared_prefix_kernel(
                     tma::mbar_expect_tx(&v_full[s], V_STAGE);
 #pragma unroll
                     for (int hf = 0; hf < HV; ++hf) tma::load_2d(Vs + s * V_STAGE + hf * KBOX, &tmV, &v_full[s], hf * 64, row);
+                    if (j == 1 || u >= u_end && i + 1 == r.pages) { pdl_wait(); pdl_launch(); }
                 }
             }
             __syncwarp();
         }
     } else if (warp == 5) {
-        const uint32_t idesc_qk = tc5::idesc_bf16(SHARED_ROWS, 64, 0), idesc_pv = tc5::idesc_bf16(SHARED_ROWS, EXACT ? DV : (dv + 15) & ~15, 1);
+        const uint32_t idesc_qk = tc5::idesc_bf16(ROWS, 64, 0), idesc_pv = tc5::idesc_bf16(ROWS, EXACT ? DV : (dv + 15) & ~15, 1);
         // A matrix descriptor's upper word is the same for all; of the lower one an operand's place is added, in 16 bytes.
         const uint64_t dq = tc5::smem_desc(tma::smem_u32(Qs), 16, 1024), dk = tc5::smem_desc(tma::smem_u32(Ks), 16, 1024);
         const uint64_t dw = tc5::smem_desc(tma::smem_u32(Vs), KBOX, 1024);
@@ -194,8 +291,8 @@ __global__ void __launch_bounds__(192, 2) shared_prefix_kernel(
             const int rows = r.members * G;
             const bool live = row < rows, idle = warp * 32 >= rows;     // (a warp without rows only keeps the pace)
             const int member = live ? row / G : 0;
-            const bf16* src = q + ((size_t)plan.rows[r.first + member] * nq + (size_t)r.head * G + (row - member * G)) * d;
-            if (pieces == 0) pdl_wait();                       // q, and the scratch is free
+            const bf16* src = st.q + ((size_t)plan.rows[r.first + member] * nq + (size_t)r.head * G + (row - member * G)) * d;
+            if (pieces == 0) { pdl_wait(); pdl_launch(); }     // q, and the scratch is free
             if (!idle) {
                 // Q into its swizzled tile: row r of a box is 128 bytes, 16-byte chunk c at place c ^ (r & 7)
 #pragma unroll
@@ -295,7 +392,8 @@ __global__ void __launch_bounds__(192, 2) shared_prefix_kernel(
             if (!ok || !(ok = wait(o_done, (uint32_t)(pieces & 1), 79))) break;
             tc5::fence_after();
             if (!idle) {
-                float* dst = shared.part_o + (r.row0 + row) * dv;
+                // (a lane's 32 bytes lie beside its neighbours', a row's do not: rows in one piece took three times as long to write)
+                float* dst = args.part_o + r.row0 * dv + row * 8;
 #pragma unroll 1
                 for (int c0 = 0; c0 < (EXACT ? DV : dv); c0 += 32) {
                     uint32_t o[32];
@@ -304,15 +402,15 @@ __global__ void __launch_bounds__(192, 2) shared_prefix_kernel(
                     if (live) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 8)
-                            if (EXACT || c0 + c < dv) store8(dst + c0 + c, o + c);
+                            if (EXACT || c0 + c < dv) store8(dst + (size_t)(c0 + c) * rows, o + c);
                     }
                 }
-                if (live) shared.part_ml[r.row0 + row] = make_float2(m_used, l);
+                if (live) args.part_ml[r.row0 + row] = make_float2(m_used, l);
                 tc5::fence_before();
             }
         }
     }
-    pdl_wait();
+    pdl_wait();                                     // (every kernel of a step waits for the one before it: common.cuh)
     tc5::fence_before();
     __syncthreads();
     if (*abort_flag) {
@@ -326,76 +424,318 @@ __global__ void __launch_bounds__(192, 2) shared_prefix_kernel(
     }
 }
 
+// One share of the pages that only row `tok` reads, for the query heads of one kv head: four warps take 16 keys of every page
+// (fragments as in attention_fast.cu), their results are merged in shared memory.
+// This kernel starts when the prefix kernel's CTAs have all seen the kernel before them complete, and waits for the prefix kernel
+// only at its end: what it reads, q and the newest position among it, was there when it started.
 template <int DK, int DV, bool EXACT>
-int launch_prefix(const CUtensorMap& tk, const CUtensorMap& tv, const void* q, const int* page_table, const int* seq_of_token, int max_pages,
-                  int nq, int nkv, float scale_log2, int n_pages, int* status, int d, int dv, const AttnShared& shared, cudaStream_t stream) {
+__global__ void __launch_bounds__(256, 2) shared_own_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                                                                const SharedStep st, const SharedArgs args) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int pair = (int)blockIdx.x / args.shares, tok = pair / st.nkv, kvh = pair % st.nkv, share = (int)blockIdx.x % args.shares;
+    constexpr int HK = DK / 64, HV = DV / 64;
+    constexpr int BOX_BYTES = 64 * 64 * 2;                 // 8 KB
+    constexpr int STAGE_BYTES = (HK + HV) * BOX_BYTES;     // K halves then V halves
+    constexpr int STAGES = OWN_STAGES_BYTES / STAGE_BYTES > 4 ? 4 : OWN_STAGES_BYTES / STAGE_BYTES;
+    constexpr int KS = DK / 16, NT = DV / 8;
+    const int d = EXACT ? DK : st.d, dv = EXACT ? DV : st.dv, nkv = st.nkv, nq = st.nq, G = nq / nkv;
+    const float scale_log2 = st.scale_log2;
+    int* status = st.status;
+    uint64_t* full = (uint64_t*)(smem + STAGES * STAGE_BYTES);
+    uint64_t* empty = full + STAGES;
+    volatile int* abort_flag = (volatile int*)(empty + STAGES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { tma::mbar_init(&full[s], 1); tma::mbar_init(&empty[s], 4); }
+        *abort_flag = 0;
+        tma::mbar_fence_init();
+        tma::prefetch_map(&tmK);
+        tma::prefetch_map(&tmV);
+    }
+    __syncthreads();
+    const int b = st.seq_of_token[tok], pos = b >= 0 ? st.positions[tok] : -1;
+    const SharedPlan plan(args);
+    int p_begin = 0, npg = 0;
+    if (b >= 0) {
+        const int first = plan.pages_of[tok], n = max(0, pos / PAGE + 1 - first), each = (n + args.shares - 1) / args.shares;
+        p_begin = first + share * each;
+        npg = max(0, min(each, n - share * each));
+    }
+    float o[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f; }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    int4 where = make_int4(0, 0, 0, 0);
+    if (warp == 4) {
+        if (lane == 0) {
+            const int* pt = st.page_table + (size_t)b * st.max_pages;
+            for (int i = 0; i < npg; ++i) {
+                const int s = i % STAGES;
+                const uint32_t ph = (uint32_t)(i / STAGES) & 1u;
+                if (!tma::mbar_wait(&empty[s], ph ^ 1u, abort_flag, status, 11)) break;
+                tma::mbar_expect_tx(&full[s], STAGE_BYTES);
+                const int row = (gg_page(pt, p_begin + i, st.max_pages, PageBounds{st.n_pages, status}, 54) * nkv + kvh) * PAGE;
+                uint8_t* dst = smem + s * STAGE_BYTES;
+#pragma unroll
+                for (int hf = 0; hf < HK; ++hf) tma::load_2d(dst + hf * BOX_BYTES, &tmK, &full[s], hf * 64, row);
+#pragma unroll
+                for (int hf = 0; hf < HV; ++hf) tma::load_2d(dst + (HK + hf) * BOX_BYTES, &tmV, &full[s], hf * 64, row);
+            }
+        }
+    } else if (warp == 5) {
+        if (share == 0) where = plan.where(tok, kvh, nkv, G, args.runs, lane);
+    } else if (npg > 0) {
+        // Q fragments in the standard A layout: row = head of the group, k = head dimension
+        uint32_t qa[KS][4];
+        {
+            const bf16* q0 = st.q + ((size_t)tok * nq + (size_t)kvh * G) * d;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int c = ks * 16 + 2 * t;
+                const bool in0 = EXACT || c < d, in1 = EXACT || c + 8 < d;
+                qa[ks][0] = g < G && in0 ? __ldcg(reinterpret_cast<const unsigned int*>(q0 + (size_t)g * d + c)) : 0u;
+                qa[ks][1] = g + 8 < G && in0 ? __ldcg(reinterpret_cast<const unsigned int*>(q0 + (size_t)(g + 8) * d + c)) : 0u;
+                qa[ks][2] = g < G && in1 ? __ldcg(reinterpret_cast<const unsigned int*>(q0 + (size_t)g * d + c + 8)) : 0u;
+                qa[ks][3] = g + 8 < G && in1 ? __ldcg(reinterpret_cast<const unsigned int*>(q0 + (size_t)(g + 8) * d + c + 8)) : 0u;
+            }
+        }
+        const int krow = warp * 16;     // this warp's 16 keys of every page
+        for (int i = 0; i < npg; ++i) {
+            const int s = i % STAGES;
+            const uint32_t ph = (uint32_t)(i / STAGES) & 1u;
+            if (!tma::mbar_wait(&full[s], ph, abort_flag, status, 12)) break;
+            const uint8_t* st = smem + s * STAGE_BYTES;
+            const int key0 = (p_begin + i) * PAGE + krow;
+            float sc[2][4];
+            sc[0][0] = sc[0][1] = sc[0][2] = sc[0][3] = 0.f;
+            sc[1][0] = sc[1][1] = sc[1][2] = sc[1][3] = 0.f;
+            if (key0 <= pos) {      // whole-warp decision: any visible key among these 16?
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const bf16* box = reinterpret_cast<const bf16*>(st + (ks >> 2) * BOX_BYTES);
+                    uint32_t kb[4];
+                    ldsm_x4(kb, sw<64>(const_cast<bf16*>(box), krow + (lane & 7) + ((lane >> 4) << 3), (ks & 3) * 2 + ((lane >> 3) & 1)));
+                    mma16816(sc[0], qa[ks], kb[0], kb[1]);
+                    mma16816(sc[1], qa[ks], kb[2], kb[3]);
+                }
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int kidx = key0 + j * 8 + 2 * t + (e & 1);
+                        const float v = kidx <= pos ? sc[j][e] * scale_log2 : -INFINITY;
+                        sc[j][e] = v;
+                        mx[e >> 1] = fmaxf(mx[e >> 1], v);
+                    }
+                uint32_t pa[4];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                    const float mn = fmaxf(m[r], mx[r]);
+                    const float mu = mn == -INFINITY ? 0.f : mn;
+                    const float corr = fast_exp2(m[r] - mu);
+                    m[r] = mn;
+                    const float p00 = fast_exp2(sc[0][2 * r] - mu), p01 = fast_exp2(sc[0][2 * r + 1] - mu);
+                    const float p10 = fast_exp2(sc[1][2 * r] - mu), p11 = fast_exp2(sc[1][2 * r + 1] - mu);
+                    l[r] = l[r] * corr + (p00 + p01 + p10 + p11);
+                    pa[r] = pack_bf16(p00, p01);
+                    pa[2 + r] = pack_bf16(p10, p11);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) { o[n][2 * r] *= corr; o[n][2 * r + 1] *= corr; }
+                }
+#pragma unroll
+                for (int np = 0; np < NT / 2; ++np) {
+                    const bf16* box = reinterpret_cast<const bf16*>(st + (HK + (np >> 2)) * BOX_BYTES);
+                    uint32_t vb[4];
+                    ldsm_x4_trans(vb, sw<64>(const_cast<bf16*>(box), krow + (lane & 7) + (((lane >> 3) & 1) << 3), (np & 3) * 2 + (lane >> 4)));
+                    mma16816(o[2 * np], pa, vb[0], vb[1]);
+                    mma16816(o[2 * np + 1], pa, vb[2], vb[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) tma::mbar_arrive(&empty[s]);
+        }
+    }
+    __syncthreads();          // all pages consumed (or the CTA gave up): the ring can be reused for the merge
+    if (*abort_flag) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) { }       // let copies in flight land before the CTA goes away
+        __syncthreads();
+    }
+    if (warp == 5 && share == 0 && lane == 0) args.where[tok * nkv + kvh] = where;
+    float* sm_o = reinterpret_cast<float*>(smem);                 // [4][16][DV]
+    float* sm_ml = sm_o + 4 * 16 * DV;                            // [4][16][2]
+    if (warp < 4) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        }
+        // only the G rows that are query heads go on (the MMA tile has 16)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if (g + 8 * r >= G) continue;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                *reinterpret_cast<float2*>(&sm_o[(warp * 16 + g + 8 * r) * DV + n * 8 + 2 * t]) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+            if (t == 0) { sm_ml[(warp * 16 + g + 8 * r) * 2] = m[r]; sm_ml[(warp * 16 + g + 8 * r) * 2 + 1] = l[r]; }
+        }
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < G * dv; idx += THREADS) {
+        const int r = idx / dv, c = idx - r * dv;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_ml[(w * 16 + r) * 2]);
+        float L = 0.f, acc = 0.f;
+        if (M != -INFINITY) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = fast_exp2(sm_ml[(w * 16 + r) * 2] - M);
+                L += sm_ml[(w * 16 + r) * 2 + 1] * f;
+                acc += sm_o[(w * 16 + r) * DV + c] * f;
+            }
+        }
+        const size_t at = (size_t)args.own_row + ((size_t)tok * nq + (size_t)kvh * G + r) * args.shares + share;
+        args.part_o[at * dv + c] = acc;
+        if (c == 0) args.part_ml[at] = make_float2(M, L);
+    }
+    pdl_wait();                                     // (its end is the prefix kernel's end, too, for the kernel after it)
+}
+
+// Half a warp a row, eight columns a lane, or several (`team`, a power of two): its prefix's parts in the order of their runs, then its
+// own, each half warp every team-th, then the half warps' sums in their order.
+constexpr int JOIN_HALVES = 16;
+__global__ void __launch_bounds__(JOIN_HALVES * 16) shared_join_kernel(bf16* __restrict__ out, const int* __restrict__ seq_of_token, int ntok, int nq,
+                                                                       int nkv, int team, const float* __restrict__ sink, float out_scale,
+                                                                       const AttnShape sh, const SharedArgs args) {
+    __shared__ __align__(16) float sm_o[JOIN_HALVES][16][8];
+    __shared__ float2 sm_ml[JOIN_HALVES];
+    pdl_launch();
+    const int lane = threadIdx.x & 15, half = threadIdx.x >> 4, w = half & (team - 1), dv = sh.dv, c = 8 * lane;
+    const int row = ((int)blockIdx.x * JOIN_HALVES + half) / team, G = nq / nkv;
+    const bool in = row < ntok * nq;
+    const int tok = in ? row / nq : 0, h = row - tok * nq;
+    const bool real = in && seq_of_token[tok] >= 0;
+    pdl_wait();
+    float M = -INFINITY, L = 0.f, acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    auto add = [&](float2 ml, const float4& a, const float4& b) {
+        const float top = fmaxf(M, ml.x);
+        if (top == -INFINITY) return;
+        const float f = fast_exp2(M - top), g = fast_exp2(ml.x - top);
+        M = top;
+        L = fmaf(ml.y, g, L * f);
+        acc[0] = fmaf(a.x, g, acc[0] * f); acc[1] = fmaf(a.y, g, acc[1] * f); acc[2] = fmaf(a.z, g, acc[2] * f); acc[3] = fmaf(a.w, g, acc[3] * f);
+        acc[4] = fmaf(b.x, g, acc[4] * f); acc[5] = fmaf(b.y, g, acc[5] * f); acc[6] = fmaf(b.z, g, acc[6] * f); acc[7] = fmaf(b.w, g, acc[7] * f);
+    };
+    if (real) {
+        const int4 at = args.where[tok * nkv + h / G];
+        const int n = at.y + args.shares, r = at.z + h % G;
+        for (int k0 = w; k0 < n; k0 += 4 * team) {
+            float2 ml[4];
+            float4 a[4], b[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = k0 + k * team;
+                ml[k] = make_float2(-INFINITY, 0.f);
+                a[k] = b[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < n) {
+                    const size_t own = (size_t)args.own_row + (size_t)row * args.shares + (i - at.y), part = (size_t)at.x + (size_t)i * ROWS;
+                    ml[k] = args.part_ml[i < at.y ? part + r : own];
+                    const float4* src = reinterpret_cast<const float4*>(args.part_o + (i < at.y ? part * dv + ((size_t)lane * at.w + r) * 8 : own * dv + c));
+                    if (c < dv) { a[k] = src[0]; b[k] = src[1]; }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) add(ml[k], a[k], b[k]);
+        }
+    }
+    if (team > 1) {
+        float4* mine = reinterpret_cast<float4*>(sm_o[half][lane]);
+        mine[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        mine[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        if (lane == 0) sm_ml[half] = make_float2(M, L);
+        __syncthreads();
+        for (int k = 1; w == 0 && k < team; ++k) {
+            const float4* theirs = reinterpret_cast<const float4*>(sm_o[half + k][lane]);
+            add(sm_ml[half + k], theirs[0], theirs[1]);
+        }
+    }
+    if (w != 0 || !in || c >= dv) return;
+    L = attn_sink_sum(L, M, sink, h);
+    const float inv = L > 0.f ? out_scale / L : 0.f;
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        y[e] = pack_bf16(attn_gate(acc[2 * e] * inv, sh, tok, h * dv + c + 2 * e), attn_gate(acc[2 * e + 1] * inv, sh, tok, h * dv + c + 2 * e + 1));
+    *reinterpret_cast<uint4*>(out + ((size_t)tok * nq + h) * dv + c) = make_uint4(y[0], y[1], y[2], y[3]);
+}
+
+template <int DK, int DV, bool EXACT>
+int launch_shared(const CUtensorMap& tk, const CUtensorMap& tv, int ntok, const SharedStep& st, const SharedArgs& args, cudaStream_t stream) {
     // Q, K x 2, V x 2 (boxes of 64 columns: 16 KB of Q, 8 KB of K or V), barriers
     constexpr int smem = (DK / 64) * (16384 + 2 * 8192) + (DV / 64) * 2 * 8192 + 256;
-    static int known[GG_MAX_DEVICES];
-    auto kern = shared_prefix_kernel<DK, DV, EXACT>;
-    int resident = 0;
-    const int rc = gg_resident(kern, 192, smem, known, resident);
-    if (rc != 0) return rc;
-    return gg_launch(kern, dim3(shared.runs), dim3(192), smem, stream, 1, tk, tv, (const bf16*)q, page_table, seq_of_token, max_pages, nq,
-                     nkv, scale_log2, n_pages, status, d, dv, shared);
+    // the ring of a row's own pages, over which its warps' results are merged; barriers
+    constexpr int stage = (DK + DV) / 64 * 8192, ring = (OWN_STAGES_BYTES / stage > 4 ? 4 : OWN_STAGES_BYTES / stage) * stage, own = ring + 256;
+    static_assert(own >= 4 * 16 * (DV + 2) * 4, "the merge lies where the ring was");
+    static int known[2][GG_MAX_DEVICES];
+    int resident = 0, rc;
+    if ((rc = gg_resident(shared_prefix_kernel<DK, DV, EXACT>, THREADS, smem, known[0], resident)) != 0) return rc;
+    if ((rc = gg_resident(shared_own_kernel<DK, DV, EXACT>, THREADS, own, known[1], resident)) != 0) return rc;
+    if ((rc = gg_launch(shared_prefix_kernel<DK, DV, EXACT>, dim3(args.runs), dim3(THREADS), smem, stream, 1, tk, tv, st, args)) != 0) return rc;
+    return gg_launch(shared_own_kernel<DK, DV, EXACT>, dim3(ntok * st.nkv * args.shares), dim3(THREADS), own, stream, 1, tk, tv, st, args);
 }
-
-template <int DK, int DV, int STAGES, bool EXACT>
-int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const void* q, void* out, const int* positions, const int* seq_of_token,
-                const int* page_table, int max_pages, int ntok, int nq, int nkv, float scale_log2, int splits, const float* sink,
-                float out_scale, int n_pages, int* status, const AttnShape& sh, const AttnShared& shared, cudaStream_t stream) {
-    constexpr int smem = decode_tma_smem<DK, DV, STAGES>(9);
-    static int known[GG_MAX_DEVICES];
-    auto kern = attn_decode_tma_kernel<DK, DV, STAGES, EXACT, true>;
-    int resident = 0;
-    const int rc = gg_resident(kern, 160, smem, known, resident);
-    if (rc != 0) return rc;
-    const long long ctas = (long long)ntok * nkv * splits;
-    return gg_launch(kern, dim3(ntok, nkv, splits), dim3(160), smem, stream, splits, tk, tv, (const bf16*)q, (bf16*)out, (float*)nullptr,
-                     (float*)nullptr, positions, seq_of_token, page_table, max_pages, nq, nkv, scale_log2, 0, splits, splits > 1 ? 1 : 0,
-                     ctas <= resident ? 1 : 0, sink, out_scale, n_pages, status, sh, shared);
-}
-
-long long part_rows(int ntok, int nq) { return (long long)nq * ntok + (long long)SHARED_ROWS * SHARED_RUNS; }
 
 }  // namespace
 
-// Decode attention (see gg_attn_decode_tma) of a step with shared prefixes: plan as at AttnShared, part: scratch of
-// (nq ntok + 128 * 296) (dv + 2) floats, on a 32-byte boundary.  splits: 1, 2, 4 or 8 CTAs share a row's own pages.
-// status: codes 71-79 name the prefix kernel's wait that ran out, 11 and 12 the other's.
+// Decode attention (see gg_attn_decode_tma) of a step with shared prefixes: plan as at SharedArgs; runs (1 to 296): CTAs over
+// the prefixes; shares (1 to 64): CTAs that share a row's own pages; part: scratch of (nq ntok (1 + shares) + 128 runs) (dv + 2) + 4 ntok nkv floats, on a 32-byte boundary.
+// status: codes 71-79 (prefixes), 11 and 12 (own pages) name the wait that ran out.
 GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_pool, void* out, const int* positions,
                              const int* seq_of_token, const int* page_table, int max_pages, int page_size, int n_pages, const int* plan,
-                             int ntok, int nq, int nkv, int d, int dv, float scale, int splits, const float* sink, float out_scale,
+                             int ntok, int nq, int nkv, int d, int dv, float scale, int runs, int shares, const float* sink, float out_scale,
                              const void* gate, long long ldg, float* part, long long part_floats, int* status, cudaStream_t stream) {
     if (ntok <= 0) return 0;
-    if (page_size != PAGE || nq <= 0 || nkv <= 0 || nq % nkv || nq / nkv > 16 || !attn_shape_ok(d, dv, 0, gate, ldg) || nkv > 65535 ||
-        n_pages <= 0 || status == nullptr || plan == nullptr || !(splits == 1 || splits == 2 || splits == 4 || splits == 8))
+    if (page_size != PAGE || nq <= 0 || nkv <= 0 || nq % nkv || nq / nkv > 16 || !attn_shape_ok(d, dv, 0, gate, ldg) || shares < 1 || shares > 64 || runs < 1 || runs > MAX_RUNS ||
+        n_pages <= 0 || max_pages <= 0 || status == nullptr || plan == nullptr)
         return GG_ERR_ARG;
-    if ((((uintptr_t)q) & 15) || (((uintptr_t)k_pool) & 15) || (((uintptr_t)v_pool) & 15) || (((uintptr_t)part) & 31)) return GG_ERR_ARG;
-    const long long rows = part_rows(ntok, nq);
-    if (part == nullptr || part_floats < rows * (dv + 2) || rows > 0x7fffffffll) return GG_ERR_ARG;
+    if ((((uintptr_t)q) & 15) || (((uintptr_t)k_pool) & 15) || (((uintptr_t)v_pool) & 15) || (((uintptr_t)out) & 15) || (((uintptr_t)part) & 31))
+        return GG_ERR_ARG;
+    const long long prefix_rows = (long long)nq * ntok + (long long)ROWS * runs, rows = prefix_rows + (long long)nq * ntok * shares;
+    if (part == nullptr || part_floats < rows * (dv + 2) + 4ll * ntok * nkv || rows > 0x7fffffffll) return GG_ERR_ARG;
+    // (units, blocks and the rows of the pools are counted in 32 bits: a row lists at most max_pages pages)
+    const unsigned long long pool_rows = (unsigned long long)n_pages * nkv * PAGE;
+    if (pool_rows > 0x7fffffffull || (unsigned long long)ntok * max_pages * nkv > 0x7fffffffull || (long long)ntok * nkv * shares > 0x3fffffffll)
+        return GG_ERR_ARG;
     CUtensorMap tk, tv;
     int rc;
-    const unsigned long long pool_rows = (unsigned long long)n_pages * nkv * PAGE;
-    if (pool_rows > 0x7fffffffull) return GG_ERR_ARG;
     if ((rc = tma::make_map_bf16(&tk, k_pool, pool_rows, d, d, PAGE)) != 0) return rc;
     if ((rc = tma::make_map_bf16(&tv, v_pool, pool_rows, dv, dv, PAGE)) != 0) return rc;
-    const float scale_log2 = scale * 1.4426950408889634f;
+    const SharedStep st = {(const bf16*)q, positions, seq_of_token, page_table, max_pages, nq, nkv, d, dv, n_pages, scale * 1.4426950408889634f,
+                           status};
+    float* where = part + rows * dv;
+    const SharedArgs args = {plan, ntok, runs, shares, part, reinterpret_cast<float2*>(where + 4ll * ntok * nkv), reinterpret_cast<int4*>(where),
+                             (int)prefix_rows};
+#define GG_SHARED(DK_, DV_, EX_) launch_shared<DK_, DV_, EX_>(tk, tv, ntok, st, args, stream)
+    if (d == 128 && dv == 128) rc = GG_SHARED(128, 128, true);
+    else if (d == 64 && dv == 64) rc = GG_SHARED(64, 64, true);
+    else if (d <= 64 && dv <= 64) rc = GG_SHARED(64, 64, false);
+    else if (d <= 64) rc = GG_SHARED(64, 128, false);
+    else if (dv <= 64) rc = GG_SHARED(128, 64, false);
+    else rc = GG_SHARED(128, 128, false);
+#undef GG_SHARED
+    if (rc != 0) return rc;
     const AttnShape sh = {d, dv, 0, (const bf16*)gate, ldg};
-    const AttnShared shared = {plan, ntok, SHARED_RUNS, part, reinterpret_cast<float2*>(part + rows * dv)};
-#define GG_PREFIX(DK_, DV_, EX_) \
-    launch_prefix<DK_, DV_, EX_>(tk, tv, q, page_table, seq_of_token, max_pages, nq, nkv, scale_log2, n_pages, status, d, dv, shared, stream)
-#define GG_ROWS(DK_, DV_, ST_, EX_)                                                                                                      \
-    launch_rows<DK_, DV_, ST_, EX_>(tk, tv, q, out, positions, seq_of_token, page_table, max_pages, ntok, nq, nkv, scale_log2, splits, sink, \
-                                    out_scale, n_pages, status, sh, shared, stream)
-    if (d == 128 && dv == 128) return (rc = GG_PREFIX(128, 128, true)) != 0 ? rc : GG_ROWS(128, 128, 3, true);
-    if (d == 64 && dv == 64) return (rc = GG_PREFIX(64, 64, true)) != 0 ? rc : GG_ROWS(64, 64, 4, true);
-    if (d <= 64 && dv <= 64) return (rc = GG_PREFIX(64, 64, false)) != 0 ? rc : GG_ROWS(64, 64, 4, false);
-    if (d <= 64) return (rc = GG_PREFIX(64, 128, false)) != 0 ? rc : GG_ROWS(64, 128, 4, false);
-    if (dv <= 64) return (rc = GG_PREFIX(128, 64, false)) != 0 ? rc : GG_ROWS(128, 64, 4, false);
-    return (rc = GG_PREFIX(128, 128, false)) != 0 ? rc : GG_ROWS(128, 128, 3, false);
-#undef GG_PREFIX
-#undef GG_ROWS
+    // half warps a row: as many as fill the device once (a part read behind another takes 1 us longer), eight CTAs of 16 an SM
+    int team = 1;
+    while (team < JOIN_HALVES && (long long)ntok * nq * team * 2 <= 148 * 4 * JOIN_HALVES) team *= 2;
+    const long long halves = (long long)ntok * nq * team;
+    return gg_launch(shared_join_kernel, dim3((unsigned)((halves + JOIN_HALVES - 1) / JOIN_HALVES)), dim3(JOIN_HALVES * 16), 0, stream, 1, (bf16*)out,
+                     seq_of_token, ntok, nq, nkv, team, sink, out_scale, sh, args);
 }
 
 // 1 if this library was built with checked page tables (the debug build), else 0.

@@ -53,15 +53,30 @@ def attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page
         status_word(q.device).data_ptr(), stream_ptr())
 
 
-# Runs over the prefixes and rows of a tile of the shared-prefix kernel (csrc/attention_shared.cu).
-SHARED_RUNS, SHARED_ROWS = 296, 128
+# The most runs over the prefixes, rows of a tile, and the most CTAs that may share a row's own pages (csrc/attention_shared.cu).
+SHARED_RUNS, SHARED_ROWS, SHARED_SHARES = 296, 128, 8
 
 
 def shared_scratch(n_tokens: int, nq: int, nkv: int, dv: int) -> int:
-    """Floats of scratch that `attn_decode_shared` needs: the parts' rows, and two numbers beside each."""
+    """Floats of scratch that `attn_decode_shared` needs: the parts' rows, two numbers beside each, and where a row's parts are."""
     if n_tokens <= 0 or nkv <= 0 or nq <= 0 or nq % nkv or dv <= 0:
         raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {dv}, {n_tokens} tokens")
-    return (nq * n_tokens + SHARED_ROWS * SHARED_RUNS) * (dv + 2)
+    return (nq * n_tokens * (1 + SHARED_SHARES) + SHARED_ROWS * SHARED_RUNS) * (dv + 2) + 4 * n_tokens * nkv
+
+
+def shared_shares(n_tokens: int, nkv: int, own_pages: int) -> int:
+    """CTAs that share a row's own pages, of which the longest row has `own_pages`: what one wave of the device holds, and two pages
+    each at least."""
+    return max(1, min(296 // (n_tokens * nkv), own_pages // 2, SHARED_SHARES))
+
+
+def shared_runs(groups: Sequence[Tuple[int, int]], nq: int, nkv: int) -> int:
+    """CTAs over the prefixes of groups of (members, pages): one an SM, which leaves room for the CTAs of the rows' own pages beside
+    it, until a CTA has more than six pages (measured, us, one against two an SM: 64 rows of 32 heads on 32 pages 34 / 39; 12 rows of
+    32 heads on 2 kv heads, 256 pages 23 / 21; 64 rows on 512 pages 85 / 68)."""
+    most = SHARED_ROWS // (nq // nkv)
+    units = sum(pages * -(-members // most) for members, pages in groups) * nkv
+    return SHARED_RUNS // 2 if units <= 6 * (SHARED_RUNS // 2) else SHARED_RUNS
 
 
 def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[int], int]]:
@@ -107,18 +122,21 @@ class PrefixPlan:
         self.n_tokens = n_tokens
         self.words = host.to(device)
         self.own_pages = own_pages
+        self.groups = [(len(rows), int(pages)) for rows, pages in groups]
 
     @staticmethod
     def words_for(n_tokens: int) -> int:
         return 5 + 7 * n_tokens
 
     @classmethod
-    def over(cls, words: torch.Tensor, n_tokens: int, own_pages: Optional[int] = None) -> "PrefixPlan":
-        """A plan whose words are (or will be) on the device already, packed by `pack`."""
+    def over(cls, words: torch.Tensor, n_tokens: int, own_pages: Optional[int] = None,
+             groups: Sequence[Tuple[int, int]] = ()) -> "PrefixPlan":
+        """A plan whose words are (or will be) on the device already, packed by `pack`; `groups`: (members, pages) of those it will
+        hold, which choose the launch (any others are right, too)."""
         plan = cls.__new__(cls)
         if words.dtype != torch.int32 or words.numel() != cls.words_for(n_tokens) or not words.is_contiguous():
             raise KernelError(f"shared attention: a plan of {n_tokens} tokens has {cls.words_for(n_tokens)} int32 words")
-        plan.n_tokens, plan.words, plan.own_pages = n_tokens, words, own_pages
+        plan.n_tokens, plan.words, plan.own_pages, plan.groups = n_tokens, words, own_pages, list(groups)
         return plan
 
     @classmethod
@@ -170,10 +188,11 @@ class PrefixPlan:
 
 
 def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, page_size, plan: PrefixPlan, scratch, nq, nkv, d, scale,
-                       sink=None, out_scale: float = 1.0, dv: Optional[int] = None, gate=None, splits: Optional[int] = None) -> None:
+                       sink=None, out_scale: float = 1.0, dv: Optional[int] = None, gate=None, runs: Optional[int] = None, shares: Optional[int] = None) -> None:
     """Decode attention (`attn_decode_tma`, without windows and chunks) of the plan's token rows: the keys and values of a prefix
-    that several rows share are read once for all of them, in two kernels.  scratch: float32, `shared_scratch` of it; two launches
-    that may run at the same time need scratch of their own.  splits (1, 2, 4, 8): CTAs that share a row's own pages."""
+    that several rows share are read once for all of them, in three kernels.  scratch: float32, `shared_scratch` of it; two launches
+    that may run at the same time need scratch of their own.  runs: CTAs over the prefixes (default:
+    `shared_runs`); shares: CTAs that share a row's own pages (default: `shared_shares`)."""
     from .tcgen05_gemm import status_word
     dv = d if dv is None else int(dv)
     T = plan.n_tokens
@@ -208,12 +227,17 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
                 or gate.get_device() != here):
             raise KernelError(f"shared attention: a gate is bfloat16 with {T} rows of {nq * dv}, on the current CUDA device")
         p_gate, ldg = gate.data_ptr(), gate.stride(0)
-    if splits is None:
-        own = table.shape[1] if plan.own_pages is None else plan.own_pages
-        splits = min(8, decode_tma_splits(T, nkv, own * page_size, cluster=True))
+    if shares is None:
+        shares = shared_shares(T, nkv, table.shape[1] if plan.own_pages is None else plan.own_pages)
+    elif not 1 <= shares <= SHARED_SHARES:
+        raise KernelError(f"shared attention: 1 to {SHARED_SHARES} shares, not {shares}")
+    if runs is None:
+        runs = shared_runs(plan.groups, nq, nkv)
+    elif not 1 <= runs <= SHARED_RUNS:
+        raise KernelError(f"shared attention: 1 to {SHARED_RUNS} runs, not {runs}")
     kernel("attention_shared", "gg_attn_decode_shared")(
         p_q, p_k, p_v, p_out, p_pos, p_seq, p_table, table.shape[1], page_size, k_pool.shape[0], p_plan, T, nq, nkv, d, dv, float(scale),
-        int(splits), p_sink, float(out_scale), p_gate, ldg, p_scratch, scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
+        int(runs), int(shares), p_sink, float(out_scale), p_gate, ldg, p_scratch, scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
 
 
 def attn_prefill(q, k_pool, v_pool, out, cu_seqlens, ctx_lens, seq_of_token, table, page_size, n_seqs,

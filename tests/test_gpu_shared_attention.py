@@ -129,8 +129,8 @@ def test_matches_the_formula(case):
                                 dict(groups=[300], prefix=[1], own=(1, 4), nq=4, nkv=4, d=64)])
 def test_own_pages_and_a_factor(kw):
     s = Setup(**kw)
-    for splits in (None, 1, 2, 4, 8):
-        check(s.run(out_scale=0.5, splits=splits), *s.want(out_scale=0.5))
+    for runs, shares in ((None, None), (1, 1), (3, 3), (296, 8)):
+        check(s.run(out_scale=0.5, runs=runs, shares=shares), *s.want(out_scale=0.5))
 
 
 def test_rows_that_share_nothing():
@@ -206,8 +206,10 @@ def test_refusals_on_the_device():
         s.run(scratch=torch.empty(100, device="cuda"))
     with pytest.raises(KernelError, match="plan of"):
         A.PrefixPlan.over(plan.words, 3)
-    with pytest.raises(KernelError):
-        s.run(plan=plan, splits=3)
+    with pytest.raises(KernelError, match="shares"):
+        s.run(plan=plan, shares=9)
+    with pytest.raises(KernelError, match="runs"):
+        s.run(plan=plan, runs=297)
     with pytest.raises(KernelError, match="plan"):
         s.run(plan=A.PrefixPlan.of_pages(s.lists, s.lengths, PAGE, "cpu"))
     with pytest.raises(KernelError, match="sink"):

@@ -82,9 +82,11 @@ def test_plan_words():
     assert empty == [0] * 20 + [-1] * 3 + [0] * 3
 
 
-def test_own_pages():
+def test_own_pages_and_their_shares():
     assert A.PrefixPlan.of_pages([[0, 1, 2], [0, 1, 3], [5]], [140, 170, 3], 64, "cpu").own_pages == 1
     assert A.PrefixPlan.of_pages([[0, 1, 2, 7], [0, 1, 3], [5]], [193, 170, 3], 64, "cpu").own_pages == 2
+    assert A.shared_shares(64, 8, 100) == 1 and A.shared_shares(2, 8, 100) == 8 and A.shared_shares(2, 8, 3) == 1 and A.shared_shares(8, 8, 9) == 4
+    assert A.shared_shares(4000, 8, 100) == 1
 
 
 @pytest.mark.parametrize("groups, n", [([([0, 5], 2)], 5), ([([-1, 2], 2)], 5), ([([1, 1], 2)], 5), ([([0, 1], 2), ([1, 2], 2)], 5),
