@@ -70,14 +70,26 @@ class Context:
             from .engine.timing import PhaseTimer
             self.generator.timer = PhaseTimer(model.rt.device)
 
-    def generate(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]],
-                 params: Optional[GenerateParams] = None) -> Union[GenerationResult, List[GenerationResult]]:
-        """One prompt (a list of ids) gives one result; a list of prompts gives a list."""
+    def generate(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]], params: Optional[GenerateParams] = None,
+                 prefix: Optional["SharedPrefix"] = None) -> Union[GenerationResult, List[GenerationResult]]:
+        """One prompt (a list of ids) gives one result; a list of prompts gives a list.  With `params.answers` above one every
+        prompt gives that many results, side by side, and one prompt gives a list, too.  `prefix`: the prompts go on from its
+        tokens, which are not run again (the results count them among their prompt's)."""
         single = len(prompts) > 0 and isinstance(prompts[0], int)
+        lists = [list(prompts)] if single else [list(p) for p in prompts]
+        slot = None
+        if prefix is not None:
+            if prefix.ctx is not self or prefix._slot is None:
+                raise ValueError("the prefix is closed, or another context's")
+            lists, slot = [prefix.tokens + p for p in lists], prefix._slot
         if self.generator.timer is not None:
             self.generator.timer.reset()
-        res = self.generator.generate([list(prompts)] if single else [list(p) for p in prompts], params)
-        return res[0] if single else res
+        res = self.generator.generate(lists, params, prefix=slot)
+        return res[0] if single and (params is None or params.answers == 1) else res
+
+    def new_prefix(self, tokens: Sequence[int]) -> "SharedPrefix":
+        """Run `tokens` once and keep them in the cache for prompts that begin with them (`generate(..., prefix=...)`)."""
+        return SharedPrefix(self, tokens)
 
     def last_timing(self):
         """The `PhaseReport` of the last `generate` call (LoadOptions(timing=True)): prefill, time to the first
@@ -106,6 +118,43 @@ class Context:
             return out.clone()
         finally:
             self.cache.close(slot)
+
+
+class SharedPrefix:
+    """Tokens that many prompts begin with, run once and held in a cache slot (`Context.new_prefix`).  Requests go on from it in
+    slots of their own, which share its pages; closing it gives back the pages that no running request holds."""
+
+    def __init__(self, ctx: "Context", tokens: Sequence[int]):
+        self.ctx = ctx
+        self.tokens: List[int] = [int(t) for t in tokens]
+        self._slot: Optional[int] = None
+        if not self.tokens:
+            raise ValueError("empty prefix")
+        if not ctx.cache.can_fork:
+            raise ValueError("a layer of this model keeps something that other sequences cannot go on from")
+        slot = ctx.cache.open()
+        try:
+            most = ctx.generator.prefill_tokens
+            for a in range(0, len(self.tokens), most):
+                ctx.stepper.step([StepEntry(slot, self.tokens[a:a + most])])
+        except BaseException:
+            ctx.cache.close(slot)
+            raise
+        self._slot = slot
+
+    def token_count(self) -> int:
+        return len(self.tokens)
+
+    def close(self) -> None:
+        if self._slot is not None:
+            self.ctx.cache.close(self._slot)
+            self._slot = None
+
+    def __enter__(self) -> "SharedPrefix":
+        return self
+
+    def __exit__(self, *exc) -> None:
+        self.close()
 
 
 class Conversation:

@@ -32,6 +32,10 @@ two-phase rule as the reference's cache, whose Append does not move Len() until 
 (cache.go:4-29) and its GPU mirror as [max_seq, kv_dim] per layer (pkg/gpu/cuda/driver.c:534-565);
 slots, pages and groups are this library's own.
 
+A sequence may be *forked*: the new slot goes on from the same tokens.  Pages are then held by several sequences and counted
+once; a page that a step is about to write to is copied first where others hold it too (so a fork costs no page until it goes
+on), a fixed-size state is copied at once.  Sequences that share pages may be read together (`PagedStore.shared`).
+
 Capacity is counted in tokens: `max_tokens` is the most that live sequences may hold, each
 sequence's count rounded up to a whole page.
 
@@ -138,6 +142,18 @@ class CacheStore:
     def check(self, is_open) -> None:             # bookkeeping invariants, for tests
         pass
 
+    can_fork = False              # True: `fork` is implemented
+
+    def fork(self, slot: int, new: int) -> None:  # `new`, just opened, goes on from what `slot` holds
+        raise CacheError(f"{type(self).__name__} cannot go on from another sequence")
+
+    def copies_needed(self, slots: Sequence[int], lengths: Sequence[int]) -> int:
+        """Pages that a step of these slots must copy before it writes to them."""
+        return 0
+
+    def own_tail(self, slot: int, length: int) -> None:
+        """Before a step writes from position `length` on: what it writes to becomes the slot's own."""
+
     def save(self, slots: Sequence[int]):
         """What a step would change for these slots beyond writing its own positions, for `load` to put back:
         a caller that runs a step twice (a warm-up before a graph capture) brackets the first run with the two.
@@ -165,16 +181,22 @@ class PagedStore(CacheStore):
         self.chunk = chunk
         self.pages = FreeList(n_pages, "page")
         self.seq_pages: Dict[int, List[int]] = {}   # slot -> page id per page index (-1 once given back)
+        self.more_holders: Dict[int, int] = {}      # page -> sequences that hold it beside the first (none: not listed)
+        self.sharing = 0                            # counts the changes in which pages are whose, beyond a sequence's growth
         self.index = -1                        # position among the cache's paged stores (set by the cache):
         #                                        a step's page table of this store is ctx.page_tables[index]
 
     def check(self, is_open) -> None:
         self.pages.check()
-        held = [p for pl in self.seq_pages.values() for p in pl if p >= 0]
-        if len(held) != len(set(held)):
-            raise CacheError("a page is held by two sequences")
-        if len(held) != self.pages.held_count:
-            raise CacheError(f"{self.pages.held_count} pages are held but sequences list {len(held)}")
+        holders: Dict[int, int] = {}
+        for pl in self.seq_pages.values():
+            for p in pl:
+                if p >= 0:
+                    holders[p] = holders.get(p, 0) + 1
+        if {p: n - 1 for p, n in holders.items() if n > 1} != self.more_holders:
+            raise CacheError("a page is held by two sequences without being counted so, or the other way round")
+        if len(holders) != self.pages.held_count:
+            raise CacheError(f"{self.pages.held_count} pages are held but sequences list {len(holders)}")
         for s in self.seq_pages:
             if not is_open(s):
                 raise CacheError(f"pages are listed for slot {s}, which is not open")
@@ -198,6 +220,64 @@ class PagedStore(CacheStore):
         if n:
             self.seq_pages.setdefault(slot, []).extend(self.pages.take_many(n))
 
+    # ------------------------------------------------------------------ pages of several sequences
+    @property
+    def shared(self) -> bool:
+        """Are there pages that several sequences hold?"""
+        return bool(self.more_holders)
+
+    def give_back(self, page: int) -> None:
+        """One holder less; the last one's page is free."""
+        self.sharing += 1
+        more = self.more_holders.get(page, 0)
+        if more > 1:
+            self.more_holders[page] = more - 1
+        elif more == 1:
+            del self.more_holders[page]
+        else:
+            self.pages.give(page)
+
+    def copy_page(self, page: int, to: int) -> None:
+        """Copy a page's contents in every layer (a subclass that can be forked)."""
+        raise CacheError(f"{type(self).__name__} cannot copy a page")
+
+    @property
+    def can_fork(self) -> bool:
+        return type(self).copy_page is not PagedStore.copy_page
+
+    def fork(self, slot: int, new: int) -> None:
+        if not self.can_fork:
+            raise CacheError(f"{type(self).__name__} cannot go on from another sequence: it does not say how to copy a page")
+        self.sharing += 1
+        pl = self.seq_pages.get(slot, [])
+        for pg in pl:
+            if pg >= 0:
+                self.more_holders[pg] = self.more_holders.get(pg, 0) + 1
+        if pl:
+            self.seq_pages[new] = list(pl)
+
+    def copies_needed(self, slots: Sequence[int], lengths: Sequence[int]) -> int:
+        if not self.more_holders:
+            return 0
+        writers: Dict[int, int] = {}
+        for s, n in zip(slots, lengths):
+            for pg in self.seq_pages.get(s, [])[n // self.page_size:]:
+                if pg in self.more_holders:
+                    writers[pg] = writers.get(pg, 0) + 1
+        # (the last holder of a page writes to it where it is)
+        return sum(min(n, self.more_holders[pg]) for pg, n in writers.items())
+
+    def own_tail(self, slot: int, length: int) -> None:
+        if not self.more_holders:
+            return
+        pl = self.seq_pages.get(slot, [])
+        for idx in range(length // self.page_size, len(pl)):
+            if pl[idx] in self.more_holders:
+                new = self.pages.take()
+                self.copy_page(pl[idx], new)
+                self.give_back(pl[idx])
+                pl[idx] = new
+
     def trim(self, slot: int, length: int) -> None:
         """Windowed or chunked group: give back pages all of whose positions lie before what the next token reads."""
         if self.window is None and self.chunk is None:
@@ -208,7 +288,7 @@ class PagedStore(CacheStore):
             if (idx + 1) * self.page_size > first_needed:
                 break
             if pg >= 0:
-                self.pages.give(pg)
+                self.give_back(pg)
                 pl[idx] = -1
 
     def can_shorten(self, slot: int, length: int) -> bool:
@@ -226,13 +306,13 @@ class PagedStore(CacheStore):
         keep = (length + self.page_size - 1) // self.page_size
         for pg in pl[keep:]:
             if pg >= 0:
-                self.pages.give(pg)
+                self.give_back(pg)
         del pl[keep:]
 
     def release(self, slot: int) -> None:
         for pg in self.seq_pages.pop(slot, []):
             if pg >= 0:
-                self.pages.give(pg)
+                self.give_back(pg)
 
     def table_row(self, slot: int, width: int) -> List[int]:
         pl = self.seq_pages.get(slot, [])
@@ -262,6 +342,10 @@ class KVGroup(PagedStore):
     def view(self, entry: int) -> "KVView":
         li = self.entries.index(entry)
         return KVView(group=self.index, k=self.k[li], v=self.v[li], page_size=self.page_size, request=self.request)
+
+    def copy_page(self, page: int, to: int) -> None:
+        for pool in (self.k, self.v):
+            pool[:, to].copy_(pool[:, page])
 
 
 @dataclass
@@ -311,6 +395,9 @@ class LatentStore(PagedStore):
         li = self.entries.index(entry)
         return LatentView(group=self.index, pool=self.pool[li], page_size=self.page_size, request=self.request)
 
+    def copy_page(self, page: int, to: int) -> None:
+        self.pool[:, to].copy_(self.pool[:, page])
+
 
 @dataclass
 class StateView:
@@ -338,6 +425,11 @@ class StateStore(CacheStore):
 
     def can_shorten(self, slot: int, length: int) -> bool:
         return False
+
+    can_fork = True
+
+    def fork(self, slot: int, new: int) -> None:
+        self.state[new].copy_(self.state[slot])
 
     def save(self, slots: Sequence[int]):
         idx = torch.as_tensor(list(slots), dtype=torch.long, device=self.state.device)
@@ -469,6 +561,25 @@ class SequenceCache:
         self.lengths[slot] = 0
         self.slots.give(slot)
 
+    @property
+    def can_fork(self) -> bool:
+        """Can every store go on from another sequence (`fork`)?"""
+        return all(st.can_fork for st in self.stores)
+
+    def fork(self, slot: int) -> int:
+        """A new slot that goes on from the tokens that `slot` holds: pages are shared until one of the two writes to them,
+        fixed-size states are copied.  The two are equals from then on; either may be cut back or closed."""
+        if not self.slots.is_held(slot):
+            raise CacheError(f"slot {slot} is not open")
+        if not self.can_fork:
+            raise CacheError("a layer's storage cannot go on from another sequence: "
+                             + ", ".join(sorted({type(st).__name__ for st in self.stores if not st.can_fork})))
+        new = self.slots.take()
+        for st in self.stores:
+            st.fork(slot, new)
+        self.lengths[new] = self.lengths[slot]
+        return new
+
     def length(self, slot: int) -> int:
         if not self.slots.is_held(slot):
             raise CacheError(f"slot {slot} is not open")
@@ -519,20 +630,26 @@ class SequenceCache:
             if n <= 0:
                 raise CacheError(f"slot {s}: a step must bring at least one token")
         for g in self.groups:
-            need = sum(g.pages_needed(s, self.lengths[s] + n) for s, n in zip(slots, counts))
+            need = self._pages_for(g, slots, counts)
             if need > g.pages.free_count:
                 raise CacheFull(
                     f"the step needs {need} more pages of {self.page_size} tokens but only "
                     f"{g.pages.free_count} of {g.n_pages} are free (cache sized for {self.max_tokens} tokens)")
         for g in self.groups:
             for s, n in zip(slots, counts):
+                g.own_tail(s, self.lengths[s])
                 g.reserve(s, self.lengths[s] + n)
+
+    def _pages_for(self, g: CacheStore, slots: Sequence[int], counts: Sequence[int]) -> int:
+        """Pages of group g that a step takes: those that the sequences grow by, and copies of shared ones that it writes to."""
+        return (sum(g.pages_needed(s, self.lengths[s] + n) for s, n in zip(slots, counts))
+                + g.copies_needed(slots, [self.lengths[s] for s in slots]))
 
     def pages_short(self, slots: Sequence[int], counts: Sequence[int]) -> int:
         """How many pages the fullest group lacks for `counts[i]` new tokens of `slots[i]` (<= 0: it fits)."""
         short = -self.n_pages
         for g in self.groups:
-            need = sum(g.pages_needed(s, self.lengths[s] + n) for s, n in zip(slots, counts))
+            need = self._pages_for(g, slots, counts)
             short = max(short, need - g.pages.free_count)
         return short if self.groups else 0
 

@@ -40,6 +40,18 @@ def _ids(text: str) -> List[int]:
         raise SystemExit(f"prompt must be token ids separated by spaces or commas, got {text!r}")
 
 
+def _biases(texts) -> dict:
+    """ID=VALUE, any number of times."""
+    out = {}
+    for text in texts or []:
+        try:
+            t, b = text.split("=")
+            out[int(t)] = float(b)
+        except ValueError:
+            raise SystemExit(f"--logit-bias takes ID=VALUE, not {text!r}")
+    return out
+
+
 def cmd_run(a) -> int:
     import gogguf_b200 as gg
     if not a.m and not a.random:
@@ -52,6 +64,8 @@ def cmd_run(a) -> int:
             prompts += [_ids(line) for line in f if line.strip()]
     if not prompts and not a.i:
         raise SystemExit("give a prompt with -p (token ids) or --prompt-file, or use -i")
+    if a.answers < 1 or (a.i and a.answers != 1):
+        raise SystemExit("--answers is at least 1, and a conversation (-i) goes on with one answer")
     t_load = time.perf_counter()
     options = gg.LoadOptions(dtype=a.dtype, max_tokens=a.cache_tokens, max_batch=a.max_batch, timing=a.timing)
     engine = gg.load(a.m, options) if a.m else gg.load_random(a.random, a.weights_seed, options)
@@ -60,7 +74,8 @@ def cmd_run(a) -> int:
     params = gg.GenerateParams(
         max_tokens=a.n,
         sampler=gg.SamplerConfig(temp=a.temp, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p, seed=a.seed),
-        repeat_penalty=a.repeat_penalty, repeat_last_n=a.repeat_last_n,
+        repeat_penalty=a.repeat_penalty, repeat_last_n=a.repeat_last_n, answers=a.answers,
+        frequency_penalty=a.frequency_penalty, presence_penalty=a.presence_penalty, logit_bias=_biases(a.logit_bias),
         stop_token_ids=None if a.stop_ids is None else _ids(a.stop_ids))
     if a.i:
         return run_interactive(ctx, params, prompts, sys.stdin, sys.stdout)
@@ -280,7 +295,11 @@ def build_parser() -> argparse.ArgumentParser:
     r.add_argument("--top-p", type=float, default=1.0, help="nucleus sampling (1 = off)")
     r.add_argument("--min-p", type=float, default=0.0, help="min-p sampling (0 = off)")
     r.add_argument("--repeat-penalty", type=float, default=1.0, help="penalty for repeated tokens (1 = off)")
-    r.add_argument("--repeat-last-n", type=int, default=64, help="history window of the repeat penalty")
+    r.add_argument("--repeat-last-n", type=int, default=64, help="history window of the penalties")
+    r.add_argument("--frequency-penalty", type=float, default=0.0, help="subtracted from a logit per time its id stands in the window")
+    r.add_argument("--presence-penalty", type=float, default=0.0, help="subtracted once from the logits of ids that stand in the window")
+    r.add_argument("--logit-bias", action="append", metavar="ID=VALUE", help="number added to an id's logit (-inf: never); may be repeated")
+    r.add_argument("--answers", type=int, default=1, help="answers per prompt, which is run once for all of them")
     r.add_argument("--seed", type=int, default=0, help="seed of the sampling draws")
     r.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     r.add_argument("--stop-ids", default=None, help="stop token ids (default: the model's eos_token_id)")

@@ -57,17 +57,26 @@ def attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page
 SHARED_RUNS, SHARED_ROWS, SHARED_SHARES = 296, 128, 8
 
 
-def shared_scratch(n_tokens: int, nq: int, nkv: int, dv: int) -> int:
-    """Floats of scratch that `attn_decode_shared` needs: the parts' rows, two numbers beside each, and where a row's parts are."""
+def shared_scratch(n_tokens: int, nq: int, nkv: int, dv: int, shares: Optional[int] = None) -> int:
+    """Floats of scratch that `attn_decode_shared` needs (for whatever `shares` it chooses itself, or for a given number): the parts'
+    rows, two numbers beside each, and where a row's parts are."""
     if n_tokens <= 0 or nkv <= 0 or nq <= 0 or nq % nkv or dv <= 0:
         raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {dv}, {n_tokens} tokens")
-    return (nq * n_tokens * (1 + SHARED_SHARES) + SHARED_ROWS * SHARED_RUNS) * (dv + 2) + 4 * n_tokens * nkv
+    if shares is None:
+        shares = shared_shares(n_tokens, nkv, 2 * SHARED_SHARES)
+    return (nq * n_tokens * (1 + shares) + SHARED_ROWS * SHARED_RUNS) * (dv + 2) + 4 * n_tokens * nkv
 
 
 def shared_shares(n_tokens: int, nkv: int, own_pages: int) -> int:
     """CTAs that share a row's own pages, of which the longest row has `own_pages`: what one wave of the device holds, and two pages
     each at least."""
     return max(1, min(296 // (n_tokens * nkv), own_pages // 2, SHARED_SHARES))
+
+
+def prefix_pays(groups: Sequence[Tuple[int, int]], nkv: int, d: int, dv: int) -> bool:
+    """Is reading the prefixes of groups of (members, pages) once worth the kernels more that it takes?  Saved is what all members
+    but one of each group would read."""
+    return sum((members - 1) * pages for members, pages in groups) * nkv * (d + dv) >= 1 << 19
 
 
 def shared_runs(groups: Sequence[Tuple[int, int]], nq: int, nkv: int) -> int:
@@ -211,9 +220,6 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
     p_q, p_k, p_v, p_out = need(q, bf16, "q"), need(k_pool, bf16, "k_pool"), need(v_pool, bf16, "v_pool"), need(out, bf16, "out")
     p_pos, p_seq, p_table = need(positions, i32, "positions"), need(seq_of_token, i32, "seq_of_token"), need(table, i32, "table")
     p_plan, p_scratch = need(plan.words, i32, "plan"), need(scratch, torch.float32, "scratch")
-    room = shared_scratch(T, nq, nkv, dv)
-    if scratch.numel() < room:
-        raise KernelError(f"shared attention: scratch must have {room} elements")
     if (q.numel() < T * nq * d or out.numel() < T * nq * dv or positions.numel() < T or seq_of_token.numel() < T or table.dim() != 2
             or k_pool.shape != (k_pool.shape[0], nkv, page_size, d) or v_pool.shape != (k_pool.shape[0], nkv, page_size, dv)):
         raise KernelError("shared attention: shapes disagree")
@@ -231,6 +237,9 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
         shares = shared_shares(T, nkv, table.shape[1] if plan.own_pages is None else plan.own_pages)
     elif not 1 <= shares <= SHARED_SHARES:
         raise KernelError(f"shared attention: 1 to {SHARED_SHARES} shares, not {shares}")
+    room = shared_scratch(T, nq, nkv, dv, shares)
+    if scratch.numel() < room:
+        raise KernelError(f"shared attention: scratch must have {room} elements")
     if runs is None:
         runs = shared_runs(plan.groups, nq, nkv)
     elif not 1 <= runs <= SHARED_RUNS:
@@ -304,19 +313,25 @@ def takes(nq: int, nkv: int, d: int, dv: int) -> bool:
 
 def try_make(nq: int, nkv: int, d: int, scale: float, window: int, dv: Optional[int] = None,
              chunk: int = 0) -> Optional[Callable]:
-    """f(q, k_pool, v_pool, out, ctx, table, page_size, sink=None, out_scale=1.0, gate=None) for bfloat16, or None when
-    the sizes are outside what the tensor-core kernels take; then the plain kernel serves."""
+    """f(q, k_pool, v_pool, out, ctx, table, page_size, sink=None, out_scale=1.0, gate=None, prefix=None) for bfloat16, or
+    None when the sizes are outside what the tensor-core kernels take; then the plain kernel serves.  prefix: the `PrefixPlan` of
+    a decode step whose sequences share pages (not read by windowed or chunked attention)."""
     dv = d if dv is None else dv
     if not takes(nq, nkv, d, dv):
         return None
     exact = d == dv and d in (64, 128)
 
-    def run(q, k_pool, v_pool, out, ctx, table, page_size, sink=None, out_scale=1.0, gate=None):
+    def run(q, k_pool, v_pool, out, ctx, table, page_size, sink=None, out_scale=1.0, gate=None, prefix=None):
         T = ctx.n_tokens
         kw = dict(sink=sink, out_scale=out_scale, dv=dv, chunk=chunk, gate=gate)
         if page_size != 64 or q.dtype != torch.bfloat16:
             K.attention_plain(q, k_pool, v_pool, out, ctx.positions, ctx.seq_of_token, table, page_size,
                               T, nq, nkv, d, scale, window, **kw)
+            return
+        if ctx.decode and prefix is not None and not window and not chunk:
+            scratch = ctx.ws.get("attn_prefix_parts", (shared_scratch(T, nq, nkv, dv),), torch.float32)
+            attn_decode_shared(q, k_pool, v_pool, out, ctx.positions, ctx.seq_of_token, table, page_size, prefix, scratch, nq, nkv, d,
+                               scale, sink=sink, out_scale=out_scale, dv=dv, gate=gate)
             return
         if ctx.decode:
             # (what lies before a window or a chunk is not read: no more splits than the pages that are)

@@ -1506,6 +1506,34 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, hi
     return out
 
 
+def shape_advance(tokens: torch.Tensor, ring_rows: Optional[torch.Tensor], rows: int, hist: Optional[torch.Tensor] = None,
+                  hist_len: Optional[torch.Tensor] = None, hist_pos: Optional[torch.Tensor] = None, states: Optional[torch.Tensor] = None,
+                  classes: Optional[torch.Tensor] = None, next: Optional[torch.Tensor] = None) -> None:
+    """What the drawn ids tokens[:rows] change for their requests (ring_rows[r], default r; a request in one row at most): they join
+    `hist` as `history_append` appends them, and move the grammar states `states` [requests] to next[state, classes[id]]; an id that
+    leads to -1 becomes -1 in `tokens` and joins nothing."""
+    if hist is None and states is None:
+        return
+    for t, what in ((tokens, "tokens"), (ring_rows, "ring_rows"), (hist, "hist"), (hist_len, "hist_len"), (hist_pos, "hist_pos"), (states, "states"),
+                    (classes, "classes"), (next, "next")):
+        if t is not None:
+            _need(t, torch.int32, what)
+    if hist is not None and (hist_len is None or hist_pos is None or hist.dim() != 2 or hist_len.numel() != hist.shape[0]
+                             or hist_pos.numel() != hist.shape[0]):
+        raise KernelError("shape_advance: hist goes with hist_len and hist_pos, one number a request")
+    if states is not None and (classes is None or next is None or next.dim() != 2):
+        raise KernelError("shape_advance: states go with classes and next")
+    rings = hist.shape[0] if hist is not None else states.numel()
+    if states is not None and states.numel() != rings:
+        raise KernelError("shape_advance: hist and states are for different numbers of requests")
+    if rows > tokens.numel() or rows > (rings if ring_rows is None else ring_rows.numel()):
+        raise KernelError(f"shape_advance: {rows} rows of {tokens.numel()} tokens for {rings} requests")
+    kernel("logit_shaping", "gg_shape_advance")(
+        _p(tokens), _p(ring_rows), rows, rings, _p(hist), _p(hist_len), _p(hist_pos), hist.shape[1] if hist is not None else 0, _p(states),
+        _p(classes), _p(next), next.shape[0] if states is not None else 0, next.shape[1] if states is not None else 0,
+        classes.numel() if states is not None else 0, _stream())
+
+
 TOPK_MAX = 1024      # largest top-k the on-device chain takes (csrc/sampling.cu)
 
 

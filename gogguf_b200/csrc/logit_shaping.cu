@@ -140,6 +140,30 @@ __global__ void __launch_bounds__(THREADS) shape_logits_kernel(const float* logi
     }
 }
 
+// What a drawn id changes for its request: the last ids, the grammar's state; an id that the state does not allow becomes -1.
+__global__ void shape_advance_kernel(int* tokens, const int* __restrict__ ring_rows, int R, int rings, int* hist, int* hist_len, int* hist_pos,
+                                     int last_n, int* states, const int* classes, const int* next, int n_states, int n_classes, int V) {
+    pdl_launch();
+    pdl_wait();
+    const int r = blockIdx.x * blockDim.x + threadIdx.x;
+    if (r >= R) return;
+    const int ring = ring_rows != nullptr ? ring_rows[r] : r;
+    if (ring < 0 || ring >= rings) return;
+    int id = tokens[r];
+    if (states != nullptr && states[ring] >= 0) {
+        const int s = states[ring];
+        const int to = s < n_states && id >= 0 && id < V ? next[(size_t)s * n_classes + classes[id]] : -1;
+        if (to < 0) tokens[r] = id = -1;
+        else states[ring] = to;
+    }
+    if (hist != nullptr && id >= 0) {
+        const int p = hist_pos[ring];
+        hist[(size_t)ring * last_n + p] = id;
+        hist_pos[ring] = p + 1 == last_n ? 0 : p + 1;
+        if (hist_len[ring] < last_n) hist_len[ring] += 1;
+    }
+}
+
 }  // namespace
 
 // out[r] = the shaped logits[r] for R rows of V; out == logits (and ldo == ld): in place, where only what changes is touched.
@@ -163,4 +187,16 @@ GG_API gg_shape_logits(const float* logits, long long ld, float* out, long long 
     auto kern = in_place ? (vec ? shape_logits_kernel<true, 4> : shape_logits_kernel<true, 1>)
                          : (vec ? shape_logits_kernel<false, 4> : shape_logits_kernel<false, 1>);
     return gg_launch(kern, grid, dim3(THREADS), 0, stream, 1, logits, ld, out, ldo, V, ring_rows, rings, s);
+}
+
+// R drawn ids (in place); the requests' last ids (hist null: none are kept) as gg_history_append appends to them; their grammar states
+// (null: none; negative: that request has none) over `next` [n_states, n_classes] and a class per id.  A request stands in one row
+// at most.
+GG_API gg_shape_advance(int* tokens, const int* ring_rows, int R, int rings, int* hist, int* hist_len, int* hist_pos, int last_n, int* states,
+                        const int* classes, const int* next, int n_states, int n_classes, int V, cudaStream_t stream) {
+    if (R <= 0) return 0;
+    if (rings <= 0 || (hist != nullptr && (hist_len == nullptr || hist_pos == nullptr || last_n <= 0))) return GG_ERR_ARG;
+    if (states != nullptr && (classes == nullptr || next == nullptr || n_states <= 0 || n_classes <= 0 || V <= 0)) return GG_ERR_ARG;
+    return gg_launch(shape_advance_kernel, dim3((R + 127) / 128), dim3(128), 0, stream, 1, tokens, ring_rows, R, rings, hist, hist_len, hist_pos,
+                     last_n, states, classes, next, n_states, n_classes, V);
 }

@@ -16,9 +16,11 @@ with reason "length" and the others go on).  Stop *strings* need a tokenizer and
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Callable, List, Optional, Sequence, Tuple
+from typing import Callable, List, Mapping, Optional, Sequence, Tuple
 
+from ..sampling.grammar import TokenGrammar
 from ..sampling.sampler import SamplerConfig, make_sampler
+from ..sampling.shaping import LogitShaping
 from .step import StepEntry
 
 
@@ -31,6 +33,11 @@ class GenerateParams:
     repeat_last_n: int = 64
     stop_token_ids: Optional[Sequence[int]] = None     # None: the model's own (eos_token_id)
     on_token: Optional[Callable[[int, int], bool]] = None   # (request index, token) -> go on?
+    answers: int = 1               # results per prompt: answer a of prompt i is result i * answers + a, drawn as that request
+    frequency_penalty: float = 0.0 # subtracted from a logit for every time its id stands among the last repeat_last_n
+    presence_penalty: float = 0.0  # subtracted once from the logits of the ids that stand there
+    logit_bias: Optional[Mapping[int, float]] = None   # id -> number added to its logit (-inf: never)
+    grammar: Optional[TokenGrammar] = None             # the ids that an answer may go on with, from one id to the next
     keep_logits: bool = False      # results carry the float32 logits every sampled token was drawn from (host copies)
 
 
@@ -64,6 +71,35 @@ def plan_batches(prompt_lens: Sequence[int], max_new: int, max_batch: int, capac
         if cur and (len(cur) >= max_batch or used + need > capacity_tokens):
             batches.append(cur)
             cur, used = [], 0
+        cur.append(i)
+        used += need
+    if cur:
+        batches.append(cur)
+    return batches
+
+
+def plan_shared_batches(prompt_lens: Sequence[int], sources: Sequence[int], max_new: int, max_batch: int, capacity_tokens: int,
+                        page_size: int, context: int, prefix_tokens: int = 0) -> List[List[int]]:
+    """`plan_batches` where request i has the prompt of request `sources[i]` (<= i) and all prompts begin with `prefix_tokens`
+    tokens that the cache holds already: the whole pages of a prompt are counted once in a batch, those of the prefix not at all."""
+    if max_batch <= 0:
+        raise ValueError("max_batch must be positive")
+    batches: List[List[int]] = []
+    cur: List[int] = []
+    used = 0
+    for i, n in enumerate(prompt_lens):
+        if n <= 0:
+            raise ValueError(f"request {i}: empty prompt")
+        if n > context:
+            raise ValueError(f"request {i}: prompt of {n} tokens exceeds the context of {context}")
+        pages = -(-min(n + max(max_new, 0), context) // page_size)
+        alone = pages - min(prefix_tokens, n) // page_size
+        if alone * page_size > capacity_tokens:
+            raise ValueError(f"request {i}: needs room for {alone * page_size} tokens but the cache holds {capacity_tokens}")
+        need = pages - n // page_size if sources[i] in cur else alone
+        if cur and (len(cur) >= max_batch or (used + need) * page_size > capacity_tokens):
+            batches.append(cur)
+            cur, used, need = [], 0, alone
         cur.append(i)
         used += need
     if cur:
@@ -130,19 +166,39 @@ class Generator:
         return torch.cat([outs[i] for i in live], dim=0)
 
     def generate(self, prompts: Sequence[Sequence[int]], params: Optional[GenerateParams] = None,
-                 held: Optional[dict] = None) -> List[GenerationResult]:
+                 held: Optional[dict] = None, prefix: Optional[int] = None) -> List[GenerationResult]:
         """`held` maps a request's index to a slot that is open already and holds the first tokens of its
         prompt (as many as the cache says): only the rest of the prompt is run, and when the request ends
         the slot stays open, cut back to the tokens of prompt + result that it holds (a conversation,
         pkg/runtime/conversation.go:87-133).  A prompt that is wholly in its slot gives its last token
-        back first, so that there are logits to sample from (conversation.go:120-126)."""
+        back first, so that there are logits to sample from (conversation.go:120-126).
+
+        `prefix` is an open slot that holds the first tokens of every prompt: every request goes on from it in a slot of its own,
+        and it stays as it is.  With `params.answers` above one the answers to a prompt go on from one run of it.  Either way the
+        requests' slots share the pages of what they have in common (where the model's storage can be shared; otherwise every
+        request's prompt is run for itself)."""
         params = params or GenerateParams()
         max_new = params.max_tokens if params.max_tokens > 0 else 128      # session.go:134-137
+        answers = int(params.answers)
+        if answers < 1:
+            raise ValueError(f"answers must be at least 1, not {params.answers}")
+        if answers > 1 and held:
+            raise ValueError("a conversation goes on with one answer")
+        sources = list(range(len(prompts)))
+        if answers > 1:
+            sources = [i * answers for i in range(len(prompts)) for _ in range(answers)]
+            prompts = [p for p in prompts for _ in range(answers)]
         results: List[Optional[GenerationResult]] = [None] * len(prompts)
-        batches = plan_batches([len(p) for p in prompts], max_new, self.max_batch,
-                               self._room(held), self.cache.page_size, self.context)
+        lens = [len(p) for p in prompts]
+        if (answers > 1 or prefix is not None) and self.cache.can_fork:
+            batches = plan_shared_batches(lens, sources, max_new, self.max_batch, self._room(held), self.cache.page_size, self.context,
+                                          self.cache.length(prefix) if prefix is not None else 0)
+        else:
+            batches = plan_batches(lens, max_new, self.max_batch, self._room(held), self.cache.page_size, self.context)
+            sources = list(range(len(prompts)))
+            prefix = None
         for batch in batches:
-            self._run_batch(batch, prompts, params, max_new, results, held or {})
+            self._run_batch(batch, prompts, params, max_new, results, held or {}, sources, prefix)
         return [r for r in results if r is not None]
 
     def _room(self, held: Optional[dict] = None) -> int:
@@ -182,26 +238,38 @@ class Generator:
         return None
 
     def _run_batch(self, batch: List[int], prompts, params: GenerateParams, max_new: int, results,
-                   held=None) -> None:
+                   held=None, sources=None, prefix=None) -> None:
         held = held or {}
+        # the first request of the batch with a prompt runs it, the others go on from its slot
+        first = {}
+        for i in batch:
+            first.setdefault(sources[i] if sources is not None else i, i)
+        runs = [i for i in batch if first[sources[i] if sources is not None else i] == i]
         stop = set(self.default_stop if params.stop_token_ids is None else params.stop_token_ids)
-        sampler = make_sampler(params.sampler, params.repeat_penalty, params.repeat_last_n, self.vocab_size)
+        sampler = make_sampler(params.sampler, params.repeat_penalty, params.repeat_last_n, self.vocab_size,
+                               LogitShaping.of(params, self.vocab_size))
         cache = self.cache
         slots, cached = {}, {}
         generated = {i: [] for i in batch}
         live: List[int] = list(batch)
         try:
-            for i in batch:
-                if i in held:
-                    slots[i] = held[i]
-                    have = min(cache.length(held[i]), len(prompts[i]) - 1)
-                    if not cache.truncate(held[i], have):
-                        cache.restart(held[i])
+            for i in runs:
+                if i in held or prefix is not None:
+                    s = slots[i] = held[i] if i in held else cache.fork(prefix)
+                    have = min(cache.length(s), len(prompts[i]) - 1)
+                    if not cache.truncate(s, have):
+                        cache.restart(s)
                         have = 0
                     cached[i] = have
                 else:
                     slots[i] = cache.open()
-            logits = self._prefill(live, prompts, slots, cached)
+            logits = self._prefill(runs, prompts, slots, cached)
+            if len(runs) < len(batch):
+                row = {i: r for r, i in enumerate(runs)}
+                for i in batch:
+                    if i not in slots:
+                        slots[i] = cache.fork(slots[first[sources[i]]])
+                logits = logits[[row[first[sources[i]]] for i in batch]]
             # a step ahead of the host needs a stepper that replays captured decode steps
             # (and no copies of every step's logits to the host, which the loop below makes)
             ahead = (hasattr(self.stepper, "decode_from_device") and getattr(self.stepper, "capturable", True)
@@ -214,7 +282,7 @@ class Generator:
                                        held)
                 return
             while live:
-                hist = [list(prompts[i]) + generated[i] for i in live] if sampler.penalised else None
+                hist = [list(prompts[i]) + generated[i] for i in live] if sampler.penalised or sampler.shaped else None
                 self._tic("sample", len(live))
                 nxt = sampler.sample(logits, streams=live, steps=[len(generated[i]) for i in live],
                                      histories=hist)
@@ -349,13 +417,16 @@ class GenerationSession:
         out = [-1] * len(self.prompts)
         if not self._live:
             return out
-        key = (params.sampler, params.repeat_penalty, params.repeat_last_n)
+        if params.answers != 1:
+            raise ValueError("a session gives one answer to each of its prompts")
+        shaping = LogitShaping.of(params, self._gen.vocab_size)
+        key = (params.sampler, params.repeat_penalty, params.repeat_last_n, shaping.key() if shaping is not None else None)
         sampler = self._samplers.get(key)
         if sampler is None:
             sampler = self._samplers[key] = make_sampler(params.sampler, params.repeat_penalty, params.repeat_last_n,
-                                                         self._gen.vocab_size)
+                                                         self._gen.vocab_size, shaping)
         live = self._live
-        hist = [self.prompts[i] + self.generated[i] for i in live] if sampler.penalised else None
+        hist = [self.prompts[i] + self.generated[i] for i in live] if sampler.penalised or sampler.shaped else None
         nxt = sampler.sample(self._logits, streams=live, steps=[len(self.generated[i]) for i in live], histories=hist)
         go_on: List[int] = []
         for i, t in zip(live, nxt):

@@ -50,7 +50,7 @@ class GraphStepper(Stepper):
     def __init__(self, model, cache, min_width: int = 16):
         super().__init__(model, cache)
         self.min_width = min_width
-        self._graphs: Dict[Tuple[int, int], _Captured] = {}
+        self._graphs: Dict[Tuple, _Captured] = {}       # by batch bucket, width bucket and what the sequences share
         self.replays = 0
         # a part that reads back to the host or allocates while it runs declares `capturable = False`;
         # such a model is stepped eagerly, and `decode_from_device` is not offered for it
@@ -60,9 +60,9 @@ class GraphStepper(Stepper):
         w = max(self.cache.table_width(slots), self.min_width)
         return 1 << (w - 1).bit_length()
 
-    def _capture(self, entries: Sequence[StepEntry], bucket: int, width: int) -> _Captured:
+    def _capture(self, entries: Sequence[StepEntry], bucket: int, width: int, prefixes=None) -> _Captured:
         dev_t = self.model.rt.device
-        lay = StepLayout(bucket, bucket, bucket, [width] * len(self.cache.groups))
+        lay = StepLayout(bucket, bucket, bucket, [width] * len(self.cache.groups), sorted(prefixes.groups) if prefixes else ())
         host = torch.empty(lay.total, dtype=torch.int32, pin_memory=True)
         dev = torch.empty(lay.total, dtype=torch.int32, device=dev_t)
         ws = Workspace(dev_t)
@@ -70,7 +70,7 @@ class GraphStepper(Stepper):
 
         def run():
             ctx, lay2, rows = self.build_context(entries, host=host, dev=dev, pad_seqs=bucket,
-                                                 table_width=width, ws=ws)
+                                                 table_width=width, ws=ws, prefixes=prefixes)
             ctx.max_ctx = width * self.cache.page_size      # an upper bound: lengths change between replays
             x = self.run_layers(ctx)
             return self.run_head(ctx, x, rows, bucket)
@@ -90,7 +90,7 @@ class GraphStepper(Stepper):
         n0 = build.launch_count()
         with torch.cuda.graph(cap.graph):
             # the copy of the integer inputs stays outside the graph: it is re-issued before every replay
-            ctx, lay2, rows = self._context_for_capture(entries, cap, bucket, width)
+            ctx, lay2, rows = self._context_for_capture(entries, cap, bucket, width, prefixes)
             x = self.run_layers(ctx)
             cap.logits = self.run_head(ctx, x, rows, bucket)
         cap.kernels = build.launch_count() - n0
@@ -98,7 +98,7 @@ class GraphStepper(Stepper):
         cap.copied = [None, None]
         return cap
 
-    def _context_for_capture(self, entries, cap: _Captured, bucket: int, width: int):
+    def _context_for_capture(self, entries, cap: _Captured, bucket: int, width: int, prefixes=None):
         # same views as build_context makes, without touching host memory or copying
         from ..parts.base import StepContext
         lay, dev = cap.layout, cap.dev
@@ -109,7 +109,7 @@ class GraphStepper(Stepper):
             seq_of_token=lay.view(dev, "seq_of_token"), cu_seqlens=lay.view(dev, "cu_seqlens"),
             slots=lay.view(dev, "slots"), ctx_lens=lay.view(dev, "ctx_lens"),
             page_tables={g: lay.view(dev, f"pages{g}").view(B, width) for g in range(len(self.cache.groups))},
-            max_new=1, max_ctx=width * self.cache.page_size, decode=True)
+            max_new=1, max_ctx=width * self.cache.page_size, decode=True, prefixes=self.prefix_plans(lay, dev, prefixes))
         return ctx, lay, lay.view(dev, "logit_rows")
 
     def _run(self, entries: Sequence[StepEntry], taps=None) -> Optional[torch.Tensor]:
@@ -149,10 +149,11 @@ class GraphStepper(Stepper):
 
     def _replay(self, entries, slots, counts, bucket, sampled, rows):
         width = self._width_bucket(slots)
-        key = (bucket, width)
+        prefixes = self.shared_prefixes(slots)
+        key = (bucket, width) if prefixes is None else (bucket, width, prefixes.key())
         cap = self._graphs.get(key)
         if cap is None:
-            cap = self._graphs[key] = self._capture(entries, bucket, width)
+            cap = self._graphs[key] = self._capture(entries, bucket, width, prefixes)
         # two pinned buffers in turn: the one filled now was last copied from two steps ago
         t = cap.turn
         cap.turn ^= 1
@@ -160,7 +161,7 @@ class GraphStepper(Stepper):
         if cap.copied[t] is not None:
             cap.copied[t].synchronize()
         self.build_context(entries, host=host, dev=cap.dev, pad_seqs=bucket, table_width=width, ws=cap.ws,
-                           token_src=rows, wait_host=False)
+                           token_src=rows, wait_host=False, prefixes=prefixes)
         if cap.copied[t] is None:
             cap.copied[t] = torch.cuda.Event()
         cap.copied[t].record()

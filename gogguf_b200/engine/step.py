@@ -28,6 +28,7 @@ import numpy as np
 import torch
 
 from ..cache.sequence_cache import SequenceCache
+from ..cache.sequence_cache import KVGroup
 from ..parts.base import StepContext, Workspace
 from .model import Model
 
@@ -81,10 +82,28 @@ def _pad4(n: int) -> int:
     return (n + 3) & ~3
 
 
+def plan_words(n_tokens: int) -> int:
+    from ..csrc.fast_attention import PrefixPlan
+    return PrefixPlan.words_for(n_tokens)
+
+
+@dataclass
+class SharedPrefixes:
+    """The prefixes that a decode step's sequences share, by KV group: groups of (rows of the step, pages), and the most pages that a
+    sequence reads beside them."""
+    groups: Dict[int, List[Tuple[List[int], int]]]
+    own_pages: int
+
+    def key(self) -> Tuple:
+        """What a captured step's launches depend on: the groups' weight and the own pages, each up to a power of two."""
+        return tuple((g, sum(len(rows) * pages for rows, pages in gs).bit_length()) for g, gs in sorted(self.groups.items())) + (
+            self.own_pages.bit_length(),)
+
+
 class StepLayout:
     """Packs the integer inputs of a step into one host buffer and one device buffer."""
 
-    def __init__(self, n_tokens: int, n_seqs: int, n_want: int, group_widths: Sequence[int]):
+    def __init__(self, n_tokens: int, n_seqs: int, n_want: int, group_widths: Sequence[int], prefix_groups: Sequence[int] = ()):
         self.n_tokens, self.n_seqs, self.n_want = n_tokens, n_seqs, n_want
         self.group_widths = list(group_widths)
         off = 0
@@ -97,6 +116,9 @@ class StepLayout:
         for g, w in enumerate(self.group_widths):
             self.off[f"pages{g}"] = (off, n_seqs * w)
             off += _pad4(n_seqs * w)
+        for g in prefix_groups:               # groups whose pages several sequences share: the plan of a decode step
+            self.off[f"prefix{g}"] = (off, plan_words(n_seqs))
+            off += _pad4(plan_words(n_seqs))
         self.total = off
 
     def view(self, buf, name: str):
@@ -114,6 +136,7 @@ class Stepper:
         self._host: Optional[torch.Tensor] = None
         self._dev: Optional[torch.Tensor] = None
         self._copied: Optional[torch.cuda.Event] = None
+        self._found: Dict[int, Tuple] = {}          # KV group -> (its count of changes, slots, what they share)
 
     # ------------------------------------------------------------------ host side
     def _check_entry(self, e: StepEntry, seen: set) -> Optional[StepError]:
@@ -162,10 +185,43 @@ class Stepper:
             self._dev = torch.empty(cap, dtype=torch.int32, device=self.model.rt.device)
         return self._host, self._dev
 
+    def shared_prefixes(self, slots: Sequence[int]) -> Optional[SharedPrefixes]:
+        """What a decode step of these slots (pages reserved) should read once for several sequences, or None."""
+        stores = [st for st in self.cache.groups if isinstance(st, KVGroup) and st.shared and st.window is None and st.chunk is None]
+        if not stores or len(slots) < 2 or not (self.model.rt.fast and self.model.rt.dtype == torch.bfloat16):
+            return None
+        from ..csrc.fast_attention import prefix_pays, shared_groups
+        starts = [self.cache.lengths[s] for s in slots]
+        found, own = {}, 0
+        for st in stores:
+            # (what sequences share does not change while they grow)
+            known = self._found.get(st.index)
+            if known is None or known[0] != st.sharing or known[1] != list(slots):
+                rows = np.asarray(self.cache.page_table(st.index, slots, self.cache.table_width(slots)), dtype=np.int64)
+                known = self._found[st.index] = (st.sharing, list(slots), shared_groups(rows, [n // st.page_size for n in starts]))
+            groups = known[2]
+            rq = st.request
+            if groups and prefix_pays([(len(r), pages) for r, pages in groups], rq.num_kv_heads, rq.head_dim, rq.value_dim or rq.head_dim):
+                found[st.index] = groups
+                have = [n // st.page_size + 1 for n in starts]
+                for r, pages in groups:
+                    for i in r:
+                        have[i] -= pages
+                own = max(own, max(have))
+        return SharedPrefixes(found, own) if found else None
+
+    def prefix_plans(self, lay: StepLayout, dev: torch.Tensor, prefixes: Optional[SharedPrefixes]) -> Dict[int, object]:
+        """The plans as the parts take them, over the words of the step's device buffer."""
+        if prefixes is None:
+            return {}
+        from ..csrc.fast_attention import PrefixPlan
+        return {g: PrefixPlan.over(lay.view(dev, f"prefix{g}"), lay.n_seqs, prefixes.own_pages, [(len(r), pages) for r, pages in gs])
+                for g, gs in prefixes.groups.items()}
+
     def build_context(self, entries: Sequence[StepEntry], host: Optional[torch.Tensor] = None,
                       dev: Optional[torch.Tensor] = None, pad_seqs: int = 0, table_width: Optional[int] = None,
                       ws: Optional[Workspace] = None, token_src: Optional[Sequence[int]] = None,
-                      wait_host: bool = True) -> Tuple[StepContext, StepLayout, torch.Tensor]:
+                      wait_host: bool = True, prefixes: Optional[SharedPrefixes] = None) -> Tuple[StepContext, StepLayout, torch.Tensor]:
         """Fill the integer inputs for `entries` (pages must be reserved already) and copy them to the device.
 
         `pad_seqs` > len(entries) pads the batch with empty rows (one padding token each), which the
@@ -181,7 +237,9 @@ class Stepper:
         T = sum(counts) + n_pad
         n_want = sum(len(e.want) for e in entries)
         width = table_width if table_width is not None else cache.table_width(slots)
-        lay = StepLayout(T, B, max(n_want, pad_seqs), [width] * len(cache.groups))
+        if prefixes is None and decode and host is None:
+            prefixes = self.shared_prefixes(slots)          # (a captured step's are found before its graph is looked up)
+        lay = StepLayout(T, B, max(n_want, pad_seqs), [width] * len(cache.groups), sorted(prefixes.groups) if prefixes else ())
         if host is None:
             host, dev = self._buffers(lay.total)
         if self._copied is not None and wait_host:
@@ -224,6 +282,9 @@ class Stepper:
             pt[:] = 0
             if entries:
                 pt[:len(entries)] = np.asarray(cache.page_table(g, slots, width), dtype=np.int32)
+        for g, gs in (prefixes.groups.items() if prefixes else ()):
+            from ..csrc.fast_attention import PrefixPlan
+            PrefixPlan.pack(gs, B, lay.view(h, f"prefix{g}"))
         dev[:lay.total].copy_(host[:lay.total], non_blocking=True)
         if dev.is_cuda:
             if self._copied is None:
@@ -240,6 +301,7 @@ class Stepper:
             decode=decode,
             fresh=bool(entries) and not any(starts),
             lengths=() if decode else list(zip(starts, counts)),
+            prefixes=self.prefix_plans(lay, dev, prefixes),
         )
         return ctx, lay, lay.view(dev, "logit_rows")
 

@@ -226,7 +226,8 @@ class AttentionMixer:
                                  cache.k if writes_cache else None, cache.v if writes_cache else None,
                                  T, nq, nkv, d, self.rot)
         if self._fast is not None:
-            self._fast(q, cache.k, cache.v, o, ctx, table, cache.page_size, sink=self.sink, out_scale=self.out_scale, gate=gate)
+            self._fast(q, cache.k, cache.v, o, ctx, table, cache.page_size, sink=self.sink, out_scale=self.out_scale, gate=gate,
+                       prefix=ctx.prefixes.get(cache.group))
         else:
             # (tiles share the keys' reads; asked once a step for layers of one size)
             asked = ("attention_tiles", nq, nkv, d, dv, self.window, self.chunk)

@@ -24,6 +24,8 @@ from typing import List, Optional, Sequence
 import numpy as np
 import torch
 
+from .shaping import LogitShaping, ShapingState, shape_host
+
 _M64 = (1 << 64) - 1
 
 
@@ -167,8 +169,10 @@ class Sampler:
     TOPK_SLICE, TOPK_SMEM = 8192, 160 * 1024
 
     def __init__(self, cfg: SamplerConfig, repeat_penalty: float = 1.0, repeat_last_n: int = 64,
-                 vocab_size: Optional[int] = None):
+                 vocab_size: Optional[int] = None, shaping: Optional[LogitShaping] = None):
         self.cfg = cfg
+        self.shaping = shaping    # penalties, biases and a grammar; the repeat penalty is then part of it
+        self._state = None        # what of it is on the device (`begin`)
         # The chain with a top-k has a kernel as long as the slices' candidates fit its shared memory (top-k
         # 1,024 up to a vocabulary of 163,840); beyond that the host chain takes the rows, as it does for
         # every configuration without a kernel.
@@ -189,15 +193,21 @@ class Sampler:
     @property
     def device_only(self) -> bool:
         """True when every row can be sampled by kernels alone (with a repeat penalty: after `begin`)."""
-        return self.on_device and (not self.penalised or self._rings is not None)
+        return self.on_device and (not (self.penalised or self.shaped) or self._rings is not None)
 
     def begin(self, streams: Sequence[int], prompts: Sequence[Sequence[int]], device) -> None:
         """Put the last `repeat_last_n` ids of each request's prompt on the device, one ring per request, so
         that the penalty can be applied, and every sampled id appended, without the host.  Only needed (and
         only done) with a repeat penalty and a configuration whose sampling runs on the device."""
-        if not (self.penalised and self.on_device):
+        if not ((self.penalised or self.shaped) and self.on_device):
             return
         n, rows = self.repeat_last_n, len(streams)
+        if self.shaped:
+            self._state = ShapingState(self.shaping, prompts, [()] * rows, device)
+            self._rings = ()
+            self._ring_rows = self._ring_pairs(rows, device)
+            self._ring_of = {int(s): r for r, s in enumerate(streams)}
+            return
         hist = torch.full((rows, n), -1, dtype=torch.int32)
         lens = torch.zeros(rows, dtype=torch.int32)
         for r, p in enumerate(prompts):
@@ -207,8 +217,12 @@ class Sampler:
         pos = lens % n
         self._rings = (hist.to(device), lens.to(device), pos.to(torch.int32).to(device))
         self._ring_of = {int(s): r for r, s in enumerate(streams)}
-        self._ring_rows = [(torch.empty(max(rows, 1), dtype=torch.int32, pin_memory=True),
-                            torch.empty(max(rows, 1), dtype=torch.int32, device=device)) for _ in range(2)]
+        self._ring_rows = self._ring_pairs(rows, device)
+
+    @staticmethod
+    def _ring_pairs(rows: int, device):
+        return [(torch.empty(max(rows, 1), dtype=torch.int32, pin_memory=True),
+                 torch.empty(max(rows, 1), dtype=torch.int32, device=device)) for _ in range(2)]
 
     def sample_async(self, logits: torch.Tensor, streams: Sequence[int], steps: Sequence[int]) -> PendingSample:
         """Greedy or temperature sampling on the device without waiting for the result: the ids stay in
@@ -228,13 +242,16 @@ class Sampler:
                            torch.empty(cap, dtype=torch.float32, device=logits.device)) for _ in range(2)]
         out, pinned, u_host, u_dev, temps = self._outs[self._turn]
         ring_rows = None
-        if self.penalised:
+        if self.penalised or self.shaped:
             # the rows' rings: the penalty edits the logits in place before the sampling kernel reads them
             rr_host, rr_dev = self._ring_rows[self._turn]
             rr_host[:rows] = torch.tensor([self._ring_of[int(s)] for s in streams], dtype=torch.int32)
             rr_dev[:rows].copy_(rr_host[:rows], non_blocking=True)
             ring_rows = rr_dev
-            K.repeat_penalty(logits, self._rings[0], self._rings[1], ring_rows, self.repeat_penalty, rows)
+            if self.shaped:
+                self._state.apply(logits, ring_rows, rows)
+            else:
+                K.repeat_penalty(logits, self._rings[0], self._rings[1], ring_rows, self.repeat_penalty, rows)
         self._turn ^= 1
         if self.cfg.greedy:
             K.argmax(logits, out, rows)
@@ -246,7 +263,9 @@ class Sampler:
             else:
                 temps[:rows].fill_(float(self.cfg.temp))
                 K.sample(logits, temps, u_dev, out, rows)
-        if ring_rows is not None:
+        if self.shaped:
+            self._state.advance(out, ring_rows, rows)
+        elif ring_rows is not None:
             K.history_append(out, ring_rows, self._rings[0], self._rings[1], self._rings[2], rows)
         pinned[:rows].copy_(out[:rows], non_blocking=True)
         ev = torch.cuda.Event()
@@ -255,13 +274,20 @@ class Sampler:
 
     @property
     def penalised(self) -> bool:
-        return self.repeat_penalty > 0 and self.repeat_penalty != 1
+        """A repeat penalty alone (with others it is part of the shaping)."""
+        return self.repeat_penalty > 0 and self.repeat_penalty != 1 and self.shaping is None
+
+    @property
+    def shaped(self) -> bool:
+        return self.shaping is not None
 
     def sample(self, logits: torch.Tensor, streams: Sequence[int], steps: Sequence[int],
                histories: Optional[Sequence[Sequence[int]]] = None) -> List[int]:
         """`streams[r]`: request index of row r; `steps[r]`: tokens it has generated so far;
-        `histories[r]`: prompt + generated ids (only read when a repeat penalty is set)."""
+        `histories[r]`: prompt + generated ids (only read with penalties or a grammar)."""
         rows = len(streams)
+        if self.shaped:
+            return self._sample_shaped(logits, streams, steps, histories)
         if rows and logits.is_cuda and self.on_device and self.device_chain and not self.cfg.greedy and not self.penalised:
             from ..csrc import kernels as K
             if self._ids is None or self._ids.numel() < rows:
@@ -307,6 +333,30 @@ class Sampler:
         return res
 
 
+    def _sample_shaped(self, logits: torch.Tensor, streams: Sequence[int], steps: Sequence[int],
+                       histories: Optional[Sequence[Sequence[int]]]) -> List[int]:
+        """`sample` with the rows shaped first, beside the logits, which stay as they are."""
+        rows = len(streams)
+        if histories is None or len(histories) < rows:
+            raise ValueError("penalties, biases and grammars need the rows' histories")
+        if not rows:
+            return []
+        made = [list(h)[len(h) - k:] for h, k in zip(histories, steps)]
+        if logits.is_cuda:
+            state = ShapingState(self.shaping, histories[:rows], made, logits.device)
+            x = state.apply(logits, None, rows, out=torch.empty((rows, logits.shape[1]), dtype=torch.float32, device=logits.device))
+        else:
+            x = logits[:rows].detach().to(torch.float32).clone()
+            for r in range(rows):
+                shape_host(x[r].numpy(), self.shaping, histories[r], made[r])
+        plain = Sampler(self.cfg, vocab_size=logits.shape[1])
+        got = plain.sample(x, streams, steps)
+        if self.shaping.grammar is not None:
+            g = self.shaping.grammar
+            got = [t if g.step(g.walk(m), int(t)) >= 0 else -1 for t, m in zip(got, made)]
+        return got
+
+
 class FunctionSampler:
     """A caller's own sampling function in the place of the chain: `fn(logits) -> id`, with the row's float32
     logits as a numpy array (sampler.Func, pkg/sampler/temperature.go:9; GenerateParams.Sampler,
@@ -315,14 +365,19 @@ class FunctionSampler:
 
     device_only = False
 
-    def __init__(self, fn, repeat_penalty: float = 1.0, repeat_last_n: int = 64):
+    def __init__(self, fn, repeat_penalty: float = 1.0, repeat_last_n: int = 64, shaping: Optional[LogitShaping] = None):
         self.fn = fn
+        self.shaping = shaping
         self.repeat_penalty = float(repeat_penalty)
         self.repeat_last_n = int(repeat_last_n) if repeat_last_n else 64
 
     @property
     def penalised(self) -> bool:
-        return self.repeat_penalty > 0 and self.repeat_penalty != 1
+        return self.repeat_penalty > 0 and self.repeat_penalty != 1 and self.shaping is None
+
+    @property
+    def shaped(self) -> bool:
+        return self.shaping is not None
 
     def begin(self, streams, prompts, device) -> None:
         pass
@@ -336,15 +391,25 @@ class FunctionSampler:
             row = host[r].copy()
             if self.penalised and histories is not None:
                 apply_repeat_penalty(row, histories[r], self.repeat_penalty, self.repeat_last_n)
-            res.append(int(self.fn(row)))
+            made = ()
+            if self.shaped:
+                if histories is None:
+                    raise ValueError("penalties, biases and grammars need the rows' histories")
+                made = list(histories[r])[len(histories[r]) - steps[r]:]
+                shape_host(row, self.shaping, histories[r], made)
+            t = int(self.fn(row))
+            if self.shaped and self.shaping.grammar is not None and self.shaping.grammar.walk(made + [t]) < 0:
+                t = -1
+            res.append(t)
         return res
 
 
-def make_sampler(sampler, repeat_penalty: float = 1.0, repeat_last_n: int = 64, vocab_size: Optional[int] = None):
+def make_sampler(sampler, repeat_penalty: float = 1.0, repeat_last_n: int = 64, vocab_size: Optional[int] = None,
+                 shaping: Optional[LogitShaping] = None):
     """The sampler of a request: a `SamplerConfig` gives the chain, a function is called as it is.
     `vocab_size`, where known, lets the sampler decide at once which of its kernels take rows of that length."""
     if isinstance(sampler, SamplerConfig):
-        return Sampler(sampler, repeat_penalty, repeat_last_n, vocab_size)
+        return Sampler(sampler, repeat_penalty, repeat_last_n, vocab_size, shaping)
     if callable(sampler):
-        return FunctionSampler(sampler, repeat_penalty, repeat_last_n)
+        return FunctionSampler(sampler, repeat_penalty, repeat_last_n, shaping)
     raise TypeError(f"a sampler is a SamplerConfig or a function of a row of logits, not {type(sampler).__name__}")

@@ -82,7 +82,7 @@ class Setup:
         if plan is None:
             plan = A.PrefixPlan.of_pages(self.lists, self.lengths, PAGE, "cuda")
         if scratch is None:
-            scratch = torch.full((A.shared_scratch(self.T, self.nq, self.nkv, self.dv),), math.nan, device="cuda")
+            scratch = torch.full((A.shared_scratch(self.T, self.nq, self.nkv, self.dv, kw.get("shares")),), math.nan, device="cuda")
         kw = {"sink": self.sink, "gate": self.gate, "dv": self.dv, **kw}
         A.attn_decode_shared(self.q, self.k, self.v, self.out, self.positions, self.rows, self.table, PAGE, plan, scratch, self.nq,
                              self.nkv, self.d, self.scale, **kw)
