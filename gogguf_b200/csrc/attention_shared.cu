@@ -6,7 +6,7 @@
 // by side, so that what computes and what waits for memory share the SMs; a third adds them, always in the same order.
 //
 // Prefixes: a tile is up to 128 rows of a tensor-core product, members of a group times the query heads of a kv head.  Per page
-// of 64 keys S = Q K^T (tcgen05.mma 128 x 64 x 16) lands in tensor memory, four warps take a row per thread, leave P as bfloat16
+// of 64 keys S = Q K^T (tcgen05.mma 128 x 128 x 16, two pages at once) lands in tensor memory, four warps take a row per thread, leave P as bfloat16
 // where S was and O += P V accumulates in tensor memory, as in the prefill kernel (attention_fast.cu), without its masks: every
 // reader sees every key of the prefix.  All (group, tile, kv head)s' pages are one line of work cut into equal runs, one per CTA,
 // so that neither the number of readers nor that of kv heads leaves an SM without work, and the grid is the same for every plan:
@@ -132,22 +132,21 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     int* status = st.status;
     constexpr int QBOX = ROWS * 64 * 2;             // [64 columns x 128 rows] of Q: 16 KB
     constexpr int KBOX = 64 * 64 * 2;               // [64 columns x 64 keys] of K or V: 8 KB
-    constexpr int Q_BYTES = HK * QBOX, K_STAGE = HK * KBOX, V_STAGE = HV * KBOX;
-    constexpr int TMEM_COLS = 256;                  // two score buffers of 64 columns, then O
+    constexpr int Q_BYTES = HK * QBOX, COL = 2 * KBOX;      // a step's two pages of K or V: 64 columns of both, then the next 64
+    constexpr int TMEM_COLS = 256;                  // scores of 128 keys, then O
     uint8_t* Qs = smem;
-    uint8_t* Ks = Qs + Q_BYTES;                     // two stages
-    uint8_t* Vs = Ks + 2 * K_STAGE;                 // two stages
-    uint64_t* bars = (uint64_t*)(Vs + 2 * V_STAGE);
-    uint64_t* q_full = bars;                        // the four softmax warps have written a run's Q
-    uint64_t* k_full = bars + 1;                    // [2]
-    uint64_t* k_empty = bars + 3;                   // [2]
-    uint64_t* v_full = bars + 5;                    // [2]
-    uint64_t* v_empty = bars + 7;                   // [2]
-    uint64_t* s_full = bars + 9;                    // [2]
-    uint64_t* p_ready = bars + 11;                  // [2] (two in turn: a warp may be a page ahead of another)
-    uint64_t* pv_done = bars + 13;
-    uint64_t* o_done = bars + 14;                   // every P V of a run's (tile, kv head) is complete
-    uint32_t* tmem_slot = (uint32_t*)(bars + 15);
+    uint8_t* Ks = Qs + Q_BYTES;
+    uint8_t* Vs = Ks + HK * COL;
+    uint64_t* bars = (uint64_t*)(Vs + HV * COL);
+    uint64_t* q_full = bars;                        // the four softmax warps have written a piece's Q
+    uint64_t* k_full = bars + 1;
+    uint64_t* k_empty = bars + 2;
+    uint64_t* v_full = bars + 3;
+    uint64_t* v_empty = bars + 4;
+    uint64_t* s_full = bars + 5;
+    uint64_t* p_ready = bars + 6;
+    uint64_t* o_done = bars + 7;                    // every P V of a piece is complete
+    uint32_t* tmem_slot = (uint32_t*)(bars + 8);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, run = (int)blockIdx.x;
@@ -162,12 +161,9 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     }
     if (threadIdx.x == 0) {
         tma::mbar_init(q_full, 4);
-        for (int i = 0; i < 2; ++i) {
-            tma::mbar_init(&k_full[i], 1); tma::mbar_init(&k_empty[i], 1);
-            tma::mbar_init(&v_full[i], 1); tma::mbar_init(&v_empty[i], 1);
-            tma::mbar_init(&s_full[i], 1); tma::mbar_init(&p_ready[i], 4);
-        }
-        tma::mbar_init(pv_done, 1);
+        tma::mbar_init(k_full, 1); tma::mbar_init(k_empty, 1);
+        tma::mbar_init(v_full, 1); tma::mbar_init(v_empty, 1);
+        tma::mbar_init(s_full, 1); tma::mbar_init(p_ready, 4);
         tma::mbar_init(o_done, 1);
         *abort_flag = 0;
         tma::mbar_fence_init();
@@ -205,7 +201,7 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     };
 
     if (warp == 5 || (warp == 4 && lane != 0)) { pdl_wait(); pdl_launch(); }
-    int j = 0;                                      // pages so far
+    int j = 0;                                      // steps of two pages (a piece's last may be one) so far
     if (warp == 4) {
         // The prefix's pages were written by earlier steps (this step's tokens go to pages of the rows' own), so they are
         // streamed before the kernel before this one has finished.
@@ -214,44 +210,34 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
             u += r.pages;
             if (lane == 0 && ok) {
                 const int* pt = st.page_table + (size_t)st.seq_of_token[r.lead] * st.max_pages;
-                for (int i = 0; i < r.pages; ++i, ++j) {
-                    const int s = j & 1;
-                    const uint32_t ph = (uint32_t)((j >> 1) & 1) ^ 1u;
-                    const int row = (gg_page(pt, r.page0 + i, st.max_pages, PageBounds{st.n_pages, status}, 54) * nkv + r.head) * PAGE;
-                    if (!(ok = tma::mbar_wait(&k_empty[s], ph, abort_flag, status, 71))) break;
-                    tma::mbar_expect_tx(&k_full[s], K_STAGE);
+                for (int i = 0; i < r.pages; i += 2, ++j) {
+                    const int n = min(2, r.pages - i);
+                    const uint32_t ph = (uint32_t)(j & 1) ^ 1u;
+                    int at[2];
+                    for (int g = 0; g < n; ++g)
+                        at[g] = (gg_page(pt, r.page0 + i + g, st.max_pages, PageBounds{st.n_pages, status}, 54) * nkv + r.head) * PAGE;
+                    if (!(ok = tma::mbar_wait(k_empty, ph, abort_flag, status, 71))) break;
+                    tma::mbar_expect_tx(k_full, (uint32_t)(n * HK * KBOX));
+                    for (int g = 0; g < n; ++g)
 #pragma unroll
-                    for (int hf = 0; hf < HK; ++hf) tma::load_2d(Ks + s * K_STAGE + hf * KBOX, &tmK, &k_full[s], hf * 64, row);
-                    if (!(ok = tma::mbar_wait(&v_empty[s], ph, abort_flag, status, 72))) break;
-                    tma::mbar_expect_tx(&v_full[s], V_STAGE);
+                        for (int hf = 0; hf < HK; ++hf) tma::load_2d(Ks + hf * COL + g * KBOX, &tmK, k_full, hf * 64, at[g]);
+                    if (!(ok = tma::mbar_wait(v_empty, ph, abort_flag, status, 72))) break;
+                    tma::mbar_expect_tx(v_full, (uint32_t)(n * HV * KBOX));
+                    for (int g = 0; g < n; ++g)
 #pragma unroll
-                    for (int hf = 0; hf < HV; ++hf) tma::load_2d(Vs + s * V_STAGE + hf * KBOX, &tmV, &v_full[s], hf * 64, row);
-                    if (j == 1 || u >= u_end && i + 1 == r.pages) { pdl_wait(); pdl_launch(); }
+                        for (int hf = 0; hf < HV; ++hf) tma::load_2d(Vs + hf * COL + g * KBOX, &tmV, v_full, hf * 64, at[g]);
+                    if (j == 0) { pdl_wait(); pdl_launch(); }
                 }
             }
             __syncwarp();
         }
     } else if (warp == 5) {
-        const uint32_t idesc_qk = tc5::idesc_bf16(ROWS, 64, 0), idesc_pv = tc5::idesc_bf16(ROWS, EXACT ? DV : (dv + 15) & ~15, 1);
+        const uint32_t idesc_qk[2] = {tc5::idesc_bf16(ROWS, 64, 0), tc5::idesc_bf16(ROWS, 128, 0)};
+        const uint32_t idesc_pv = tc5::idesc_bf16(ROWS, EXACT ? DV : (dv + 15) & ~15, 1);
         // A matrix descriptor's upper word is the same for all; of the lower one an operand's place is added, in 16 bytes.
         const uint64_t dq = tc5::smem_desc(tma::smem_u32(Qs), 16, 1024), dk = tc5::smem_desc(tma::smem_u32(Ks), 16, 1024);
-        const uint64_t dw = tc5::smem_desc(tma::smem_u32(Vs), KBOX, 1024);
+        const uint64_t dw = tc5::smem_desc(tma::smem_u32(Vs), COL, 1024);
         auto moved = [](uint64_t desc, uint32_t bytes) -> uint64_t { return desc & 0xffffffff00000000ull | (uint32_t)desc + (bytes >> 4); };
-        auto issue_scores = [&](int j) -> bool {
-            const int s = j & 1;
-            if (!tma::mbar_wait(&k_full[s], (uint32_t)((j >> 1) & 1), abort_flag, status, 73)) return false;
-            tc5::fence_after();
-            const uint64_t dks = moved(dk, (uint32_t)(s * K_STAGE));
-#pragma unroll
-            for (int ks = 0; ks < DK / 16; ++ks) {
-                if (!EXACT && ks * 16 >= d) break;
-                tc5::mma(S_t + (uint32_t)(s * 64), moved(dq, (uint32_t)((ks >> 2) * QBOX + (ks & 3) * 32)),
-                         moved(dks, (uint32_t)((ks >> 2) * KBOX + (ks & 3) * 32)), idesc_qk, ks > 0 ? 1u : 0u);
-            }
-            tc5::commit(&s_full[s]);
-            tc5::commit(&k_empty[s]);
-            return true;
-        };
         int pieces = 0;
         for (int u = u_begin; u < u_end; ++pieces) {
             const Piece r = piece_at(u);
@@ -259,23 +245,30 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
             if (lane == 0 && ok) {
                 // (a piece's first scores come after the last P V of the piece before: its Q is written when that is read)
                 ok = tma::mbar_wait(q_full, (uint32_t)(pieces & 1), abort_flag, status, 74);
-                if (ok) ok = issue_scores(j);
-                for (int i = 0; i < r.pages && ok; ++i, ++j) {
-                    // The next page's scores do not wait for this page's softmax: their buffer was last read by the
-                    // softmax of page j - 1, whose p_ready this thread has already seen.
-                    if (i + 1 < r.pages && !(ok = issue_scores(j + 1))) break;
-                    const int s = j & 1;
-                    const uint32_t ph = (uint32_t)((j >> 1) & 1);
-                    if (!(ok = tma::mbar_wait(&v_full[s], ph, abort_flag, status, 76))) break;
-                    if (!(ok = tma::mbar_wait(&p_ready[s], ph, abort_flag, status, 75))) break;
+                for (int i = 0; i < r.pages && ok; i += 2, ++j) {
+                    const int n = min(2, r.pages - i);
+                    const uint32_t ph = (uint32_t)(j & 1);
+                    if (!(ok = tma::mbar_wait(k_full, ph, abort_flag, status, 73))) break;
                     tc5::fence_after();
-                    const uint64_t dvs = moved(dw, (uint32_t)(s * V_STAGE));
+                    // (over the P of the step before, which the products before these have read: the tensor core works in order)
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        // P of page j lies in the first 32 columns of score buffer j & 1: 16 keys are 8 columns
-                        tc5::mma_a_tmem(O_t, S_t + (uint32_t)(s * 64 + kk * 8), moved(dvs, (uint32_t)(kk * 2048)), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
-                    tc5::commit(pv_done);
-                    tc5::commit(&v_empty[s]);
+                    for (int ks = 0; ks < DK / 16; ++ks) {
+                        if (!EXACT && ks * 16 >= d) break;
+                        tc5::mma(S_t, moved(dq, (uint32_t)((ks >> 2) * QBOX + (ks & 3) * 32)), moved(dk, (uint32_t)((ks >> 2) * COL + (ks & 3) * 32)),
+                                 idesc_qk[n - 1], ks > 0 ? 1u : 0u);
+                    }
+                    tc5::commit(s_full);
+                    tc5::commit(k_empty);
+                    if (!(ok = tma::mbar_wait(v_full, ph, abort_flag, status, 76))) break;
+                    if (!(ok = tma::mbar_wait(p_ready, ph, abort_flag, status, 75))) break;
+                    tc5::fence_after();
+                    for (int g = 0; g < n; ++g)
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            // P lies in the first columns of the scores: 16 keys are 8 columns
+                            tc5::mma_a_tmem(O_t, S_t + (uint32_t)(g * 32 + kk * 8), moved(dw, (uint32_t)(g * KBOX + kk * 2048)), idesc_pv,
+                                            (i > 0 || g > 0 || kk > 0) ? 1u : 0u);
+                    tc5::commit(v_empty);
                 }
                 if (ok) tc5::commit(o_done);
             }
@@ -291,14 +284,23 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
             const int rows = r.members * G;
             const bool live = row < rows, idle = warp * 32 >= rows;     // (a warp without rows only keeps the pace)
             const int member = live ? row / G : 0;
-            const bf16* src = st.q + ((size_t)plan.rows[r.first + member] * nq + (size_t)r.head * G + (row - member * G)) * d;
+            const int from = live ? (plan.rows[r.first + member] * nq + r.head * G + (row - member * G)) : -1;      // row of q
             if (pieces == 0) { pdl_wait(); pdl_launch(); }     // q, and the scratch is free
             if (!idle) {
-                // Q into its swizzled tile: row r of a box is 128 bytes, 16-byte chunk c at place c ^ (r & 7)
+                // Q into its swizzled tile: row r of a box is 128 bytes, 16-byte chunk c at place c ^ (r & 7).  Half a warp reads a
+                // row (a row per lane instead asked the L1 for 32 lines at a time, 3 us of 128 rows)
+                constexpr int LANES = DK / 8, ROWS_AT_ONCE = 32 / LANES;
+                const int c = lane % LANES;
+                uint4 x[32 / ROWS_AT_ONCE];
 #pragma unroll
-                for (int c = 0; c < DK / 8; ++c) {
-                    const uint4 x = live && (EXACT || c * 8 < d) ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-                    *reinterpret_cast<uint4*>(Qs + (c >> 3) * QBOX + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = x;
+                for (int k = 0; k < 32 / ROWS_AT_ONCE; ++k) {
+                    const int src = __shfl_sync(0xffffffffu, from, k * ROWS_AT_ONCE + lane / LANES);
+                    x[k] = src >= 0 && (EXACT || c * 8 < d) ? *reinterpret_cast<const uint4*>(st.q + (size_t)src * d + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+                }
+#pragma unroll
+                for (int k = 0; k < 32 / ROWS_AT_ONCE; ++k) {
+                    const int to = warp * 32 + k * ROWS_AT_ONCE + lane / LANES;
+                    *reinterpret_cast<uint4*>(Qs + (c >> 3) * QBOX + to * 128 + (((c & 7) ^ (to & 7)) << 4)) = x[k];
                 }
             }
             tc5::fence_proxy_async_smem();
@@ -306,14 +308,15 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
             __syncwarp();
             if (lane == 0) tma::mbar_arrive(q_full);
             float m_used = -INFINITY, l = 0.f;
-            for (int i = 0; i < r.pages; ++i, ++j) {
-                const int s = j & 1;
-                if (!(ok = wait(&s_full[s], (uint32_t)((j >> 1) & 1), 77))) break;
+            for (int i = 0; i < r.pages; i += 2, ++j) {
+                const int pages = min(2, r.pages - i);
+                if (!(ok = wait(s_full, (uint32_t)(j & 1), 77))) break;
                 tc5::fence_after();
-                if (!idle) {
+#pragma unroll 1
+                for (int g = 0; g < pages && !idle; ++g) {
                     uint32_t sr[64], pk[32];
-                    tc5::ld32(S_t + lane_off + (uint32_t)(s * 64), sr);
-                    tc5::ld32(S_t + lane_off + (uint32_t)(s * 64) + 32, sr + 32);
+                    tc5::ld32(S_t + lane_off + (uint32_t)(g * 64), sr);
+                    tc5::ld32(S_t + lane_off + (uint32_t)(g * 64) + 32, sr + 32);
                     tc5::wait_ld();
                     // P = 2^(score scale - maximum in use) as bfloat16 pairs; returns the sum of the page's P
                     auto exponentials = [&]() -> float {
@@ -332,8 +335,9 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
                         unpack2(add2(add2(l4[0], l4[1]), add2(l4[2], l4[3])), la, lb);
                         return la + lb;
                     };
-                    // The maximum in use is that of the pages before (any is exact while nothing overflows): only where a row
-                    // has none yet, or the page's sum says that a score lies more than 2^64 above it, is the page's own found, O rescaled where it has grown by more than 2^8, and the page computed again.
+                    // The maximum in use is that of the pages before (any is exact while nothing overflows): only where a row has none
+                    // yet, or the page's sum says that a score lies more than 2^64 above it, is the page's own found, what was summed
+                    // rescaled where it has grown by more than 2^8, and the page computed again.
                     float lpage = 0.f;
                     bool again = m_used == -INFINITY;
                     if (!__any_sync(0xffffffffu, again)) {
@@ -358,37 +362,44 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
                                 m_used = mx;
                                 l *= corr;
                             }
-                            if (i > 0 && __any_sync(0xffffffffu, had)) {
-                                // P V of the page before must be complete before O is rescaled (that of this page waits for
-                                // this warp's p_ready, that of two pages ago came before these scores: the phase is the one meant)
-                                if (!(ok = wait(pv_done, (uint32_t)((j - 1) & 1), 78))) break;
-                                tc5::fence_after();
-#pragma unroll 1
-                                for (int c0 = 0; c0 < (EXACT ? DV : dv); c0 += 32) {
-                                    uint32_t o[32];
-                                    tc5::ld32(O_t + lane_off + c0, o);
-                                    tc5::wait_ld();
+                            auto rescale = [&](uint32_t at, bool pairs) {
+                                uint32_t o[32];
+                                tc5::ld32(at + lane_off, o);
+                                tc5::wait_ld();
 #pragma unroll
-                                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
-                                    tc5::st32(O_t + lane_off + c0, o);
+                                for (int c = 0; c < 32; ++c) {
+                                    if (pairs) {
+                                        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&o[c]));
+                                        o[c] = pack_bf16(f.x * corr, f.y * corr);
+                                    } else {
+                                        o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+                                    }
                                 }
+                                tc5::st32(at + lane_off, o);
+                            };
+                            if (__any_sync(0xffffffffu, had)) {
+                                // O is complete: the P V of the step before was issued before these scores.  The P of this step's
+                                // first page is rescaled as the bfloat16 it is (rounded once more, where a maximum grows by 2^8)
+                                if (i > 0)
+#pragma unroll 1
+                                    for (int c0 = 0; c0 < (EXACT ? DV : dv); c0 += 32) rescale(O_t + (uint32_t)c0, false);
+                                if (g > 0) rescale(S_t, true);
                                 tc5::wait_st();
                             }
                         }
                         lpage = exponentials();
                     }
                     l += lpage;
-                    // P over this thread's own row of the scores it has read: nothing else uses this buffer now (the P V of
-                    // two pages ago was issued before these scores, and the tensor core works in order)
-                    tc5::st32(S_t + lane_off + (uint32_t)(s * 64), pk);
+                    // P over this thread's own row of scores it has read: the first page's takes half the columns of the first page's
+                    // scores, the second's the other half
+                    tc5::st32(S_t + lane_off + (uint32_t)(g * 32), pk);
                     tc5::wait_st();
                 }
                 tc5::fence_before();
                 __syncwarp();
-                if (lane == 0) tma::mbar_arrive(&p_ready[s]);
+                if (lane == 0) tma::mbar_arrive(p_ready);
             }
-            // The last P V (on a barrier of its own: by pv_done's parity, two phases not yet complete would look like the last one
-            // being so), then the part
+            // the last P V, then the part
             if (!ok || !(ok = wait(o_done, (uint32_t)(pieces & 1), 79))) break;
             tc5::fence_after();
             if (!idle) {
@@ -445,6 +456,8 @@ __global__ void __launch_bounds__(256, 2) shared_own_kernel(const __grid_constan
     uint64_t* empty = full + STAGES;
     volatile int* abort_flag = (volatile int*)(empty + STAGES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const SharedPlan plan(args);
+    const int b = st.seq_of_token[tok], at = st.positions[tok], first = plan.pages_of[tok];
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { tma::mbar_init(&full[s], 1); tma::mbar_init(&empty[s], 4); }
         *abort_flag = 0;
@@ -453,11 +466,10 @@ __global__ void __launch_bounds__(256, 2) shared_own_kernel(const __grid_constan
         tma::prefetch_map(&tmV);
     }
     __syncthreads();
-    const int b = st.seq_of_token[tok], pos = b >= 0 ? st.positions[tok] : -1;
-    const SharedPlan plan(args);
+    const int pos = b >= 0 ? at : -1;
     int p_begin = 0, npg = 0;
     if (b >= 0) {
-        const int first = plan.pages_of[tok], n = max(0, pos / PAGE + 1 - first), each = (n + args.shares - 1) / args.shares;
+        const int n = max(0, pos / PAGE + 1 - first), each = (n + args.shares - 1) / args.shares;
         p_begin = first + share * each;
         npg = max(0, min(each, n - share * each));
     }
@@ -584,23 +596,24 @@ __global__ void __launch_bounds__(256, 2) shared_own_kernel(const __grid_constan
         }
     }
     __syncthreads();
-    for (int idx = threadIdx.x; idx < G * dv; idx += THREADS) {
-        const int r = idx / dv, c = idx - r * dv;
-        float M = -INFINITY;
+    for (int idx = threadIdx.x; idx < G * dv / 4; idx += THREADS) {
+        const int r = idx / (dv / 4), c = (idx - r * (dv / 4)) * 4;
+        float m4[4], M = -INFINITY, L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_ml[(w * 16 + r) * 2]);
-        float L = 0.f, acc = 0.f;
+        for (int w = 0; w < 4; ++w) { m4[w] = sm_ml[(w * 16 + r) * 2]; M = fmaxf(M, m4[w]); }
         if (M != -INFINITY) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float f = fast_exp2(sm_ml[(w * 16 + r) * 2] - M);
-                L += sm_ml[(w * 16 + r) * 2 + 1] * f;
-                acc += sm_o[(w * 16 + r) * DV + c] * f;
+                const float f = fast_exp2(m4[w] - M);
+                const float4 v = *reinterpret_cast<const float4*>(&sm_o[(w * 16 + r) * DV + c]);
+                L = fmaf(sm_ml[(w * 16 + r) * 2 + 1], f, L);
+                acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
             }
         }
-        const size_t at = (size_t)args.own_row + ((size_t)tok * nq + (size_t)kvh * G + r) * args.shares + share;
-        args.part_o[at * dv + c] = acc;
-        if (c == 0) args.part_ml[at] = make_float2(M, L);
+        const size_t to = (size_t)args.own_row + ((size_t)tok * nq + (size_t)kvh * G + r) * args.shares + share;
+        *reinterpret_cast<float4*>(args.part_o + to * dv + c) = acc;
+        if (c == 0) args.part_ml[to] = make_float2(M, L);
     }
     pdl_wait();                                     // (its end is the prefix kernel's end, too, for the kernel after it)
 }

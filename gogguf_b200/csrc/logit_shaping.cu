@@ -40,21 +40,20 @@ __device__ __forceinline__ float shaped(float x, int c, int b, const Shaping& s)
 }
 
 // VEC: logits of a load (4: rows on 16-byte boundaries).  A thread's logits lie THREADS * VEC apart, so that a warp's lie side by
-// side; they are asked for before the row's request is known, and its state's bits before its ids are counted.
-template <bool IN_PLACE, int VEC>
-__global__ void __launch_bounds__(THREADS) shape_logits_kernel(const float* logits, long long ld, float* out, long long ldo, int V,
+// side.  A slice is 4 us of waiting for loads that depend on one another (the row's request, its numbers, its ids and its state's
+// bits) around 32 KB of traffic, so what does not depend is asked for together, the logits first, and as many CTAs as fit an SM
+// share it: of a logit's word the lower half counts its id, the upper one is its bias's place in the request's list, plus one
+// (WIDE: two words, for windows or lists beyond 65,535).
+template <bool IN_PLACE, int VEC, bool WIDE>
+__global__ void __launch_bounds__(THREADS, 6) shape_logits_kernel(const float* logits, long long ld, float* out, long long ldo, int V,
                                                                const int* __restrict__ ring_rows, int rings, const Shaping s) {
     constexpr int GROUPS = PER / VEC;
-    __shared__ __align__(16) int count[SLICE];
-    __shared__ __align__(16) int bias_at[SLICE];
+    __shared__ __align__(16) unsigned seen[WIDE ? 2 : 1][SLICE];
     const int r = blockIdx.y, lo = blockIdx.x * SLICE, n = min(SLICE, V - lo);
     pdl_launch();
     const bool sparse = s.hist != nullptr || s.bias_start != nullptr;
     if (sparse) {
-        for (int i = threadIdx.x * 4; i < SLICE; i += THREADS * 4) {
-            *reinterpret_cast<int4*>(count + i) = make_int4(0, 0, 0, 0);
-            *reinterpret_cast<int4*>(bias_at + i) = make_int4(0, 0, 0, 0);
-        }
+        for (int i = threadIdx.x * 4; i < (WIDE ? 2 : 1) * SLICE; i += THREADS * 4) *reinterpret_cast<uint4*>(seen[0] + i) = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
     }
     pdl_wait();
@@ -76,7 +75,14 @@ __global__ void __launch_bounds__(THREADS) shape_logits_kernel(const float* logi
     }
     const int ring = ring_rows != nullptr ? ring_rows[r] : r;
     const bool known = ring >= 0 && ring < rings;
+    const int ids = known && s.hist != nullptr ? min(s.hist_len[ring], s.last_n) : 0;
     const int state = known && s.masks != nullptr ? s.mask_rows[ring] : -1;
+    const int b0 = known && s.bias_start != nullptr ? max(s.bias_start[ring], 0) : 0;
+    const int b1 = known && s.bias_start != nullptr ? min(s.bias_start[ring + 1], s.biases) : 0;
+    const int* h = s.hist + (size_t)ring * s.last_n;
+    int first_id = -1, first_bias = -1;
+    if ((int)threadIdx.x < ids) first_id = h[threadIdx.x];
+    if (b0 + (int)threadIdx.x < b1) first_bias = s.bias_ids[b0 + threadIdx.x];
     // bits of allowed ids, a thread's groups'  (a state beyond the table allows nothing)
     unsigned allowed[GROUPS];
 #pragma unroll
@@ -86,20 +92,29 @@ __global__ void __launch_bounds__(THREADS) shape_logits_kernel(const float* logi
     }
     bool any = false;                               // an id of this slice is penalised or has a bias
     if (sparse) {
-        if (known && s.hist != nullptr) {
-            const int* h = s.hist + (size_t)ring * s.last_n;
-            const int m = min(s.hist_len[ring], s.last_n);
-            for (int t = threadIdx.x; t < m; t += THREADS) {
-                const int id = h[t];
-                if (id >= lo && id - lo < n) { atomicAdd(&count[id - lo], 1); any = true; }
-            }
+        auto count = [&](int id) {
+            if (id >= lo && id - lo < n) { atomicAdd(&seen[0][id - lo], 1u); any = true; }
+        };
+        count(first_id);
+        int t = threadIdx.x + THREADS;
+        for (; t + 3 * THREADS < ids; t += 4 * THREADS) {
+            const int a = h[t], b = h[t + THREADS], c = h[t + 2 * THREADS], d = h[t + 3 * THREADS];
+            count(a); count(b); count(c); count(d);
         }
-        if (known && s.bias_start != nullptr) {
-            const int e = min(s.bias_start[ring + 1], s.biases);
-            for (int t = max(s.bias_start[ring], 0) + threadIdx.x; t < e; t += THREADS) {
-                const int id = s.bias_ids[t];
-                // (of an id that is listed twice, the last entry)
-                if (id >= lo && id - lo < n) { atomicMax(&bias_at[id - lo], t + 1); any = true; }
+        for (; t < ids; t += THREADS) count(h[t]);
+        for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
+            const int id = e < b0 + THREADS ? first_bias : s.bias_ids[e];
+            if (id < lo || id - lo >= n) continue;
+            any = true;
+            // (of an id that is listed twice, the last entry)
+            if (WIDE) {
+                atomicMax(&seen[1][id - lo], (unsigned)(e - b0 + 1));
+            } else {
+                unsigned old = seen[0][id - lo], was;
+                do {
+                    was = old;
+                    old = atomicCAS(&seen[0][id - lo], was, max(was >> 16, (unsigned)(e - b0 + 1)) << 16 | (was & 0xffffu));
+                } while (old != was);
             }
         }
         any = __syncthreads_or(any);
@@ -108,27 +123,45 @@ __global__ void __launch_bounds__(THREADS) shape_logits_kernel(const float* logi
     for (int k = 0; k < GROUPS; ++k) {
         const int i = (k * THREADS + threadIdx.x) * VEC;
         if (i >= n) break;
-        int c[VEC] = {}, b[VEC] = {};
+        unsigned w[VEC] = {}, u[VEC] = {};
+        bool some = false;                          // of this group is seen or has a bias
         if (any) {
             if (VEC == 4) {
-                const int4 c4 = *reinterpret_cast<const int4*>(count + i), b4 = *reinterpret_cast<const int4*>(bias_at + i);
-                c[0] = c4.x; c[1 % VEC] = c4.y; c[2 % VEC] = c4.z; c[3 % VEC] = c4.w;
-                b[0] = b4.x; b[1 % VEC] = b4.y; b[2 % VEC] = b4.z; b[3 % VEC] = b4.w;
-            } else { c[0] = count[i]; b[0] = bias_at[i]; }
+                const uint4 w4 = *reinterpret_cast<const uint4*>(seen[0] + i);
+                w[0] = w4.x; w[1 % VEC] = w4.y; w[2 % VEC] = w4.z; w[3 % VEC] = w4.w;
+                if (WIDE) {
+                    const uint4 u4 = *reinterpret_cast<const uint4*>(seen[WIDE ? 1 : 0] + i);
+                    u[0] = u4.x; u[1 % VEC] = u4.y; u[2 % VEC] = u4.z; u[3 % VEC] = u4.w;
+                }
+            } else {
+                w[0] = seen[0][i];
+                if (WIDE) u[0] = seen[WIDE ? 1 : 0][i];
+            }
+            unsigned both = 0u;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) both |= w[e] | u[e];
+            some = both != 0u;
         }
+        auto one = [&](float z, int e) -> float {
+            const int c = WIDE ? (int)w[e] : (int)(w[e] & 0xffffu), b = WIDE ? (int)u[e] : (int)(w[e] >> 16);
+            return shaped(z, c, b > 0 ? b0 + b : 0, s);
+        };
         if (IN_PLACE) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 if (i + e >= n) break;
                 if (!(allowed[k] >> e & 1)) y[i + e] = -INFINITY;
-                else if (c[e] > 0 || b[e] > 0) y[i + e] = shaped(x[i + e], c[e], b[e], s);
+                else if (some && (w[e] | u[e]) != 0u) y[i + e] = one(x[i + e], e);
             }
         } else {
+            if (some) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                if (any && (c[e] > 0 || b[e] > 0)) v[k][e] = shaped(v[k][e], c[e], b[e], s);
-                if (!(allowed[k] >> e & 1)) v[k][e] = -INFINITY;
+                for (int e = 0; e < VEC; ++e)
+                    if ((w[e] | u[e]) != 0u) v[k][e] = one(v[k][e], e);
             }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (!(allowed[k] >> e & 1)) v[k][e] = -INFINITY;
             if (VEC == 4 && i + 4 <= n) {
                 __stcs(reinterpret_cast<float4*>(y + i), make_float4(v[k][0], v[k][1 % VEC], v[k][2 % VEC], v[k][3 % VEC]));
             } else {
@@ -184,8 +217,12 @@ GG_API gg_shape_logits(const float* logits, long long ld, float* out, long long 
     const bool in_place = out == logits;
     if (in_place && R > 1 && ld != ldo) return GG_ERR_ARG;
     if (in_place && hist == nullptr && bias_start == nullptr && masks == nullptr) return 0;
-    auto kern = in_place ? (vec ? shape_logits_kernel<true, 4> : shape_logits_kernel<true, 1>)
-                         : (vec ? shape_logits_kernel<false, 4> : shape_logits_kernel<false, 1>);
+    // (a request's own list is no longer than all of them)
+    const bool wide = (hist != nullptr && last_n > 65535) || biases > 65534;
+#define GG_SHAPE(WIDE_) (in_place ? (vec ? shape_logits_kernel<true, 4, WIDE_> : shape_logits_kernel<true, 1, WIDE_>) \
+                                  : (vec ? shape_logits_kernel<false, 4, WIDE_> : shape_logits_kernel<false, 1, WIDE_>))
+    auto kern = wide ? GG_SHAPE(true) : GG_SHAPE(false);
+#undef GG_SHAPE
     return gg_launch(kern, grid, dim3(THREADS), 0, stream, 1, logits, ld, out, ldo, V, ring_rows, rings, s);
 }
 

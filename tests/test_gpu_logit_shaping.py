@@ -104,6 +104,8 @@ SIZES = {
     "rows apart": dict(R=4, V=1001, ld=1030, window=17, biases=9, states=3, seed=3),
     "a wide vocabulary": dict(R=3, V=151936, window=64, biases=300, states=4, seed=4),
     "a long window": dict(R=2, V=5000, window=20000, biases=0, states=0, seed=5),
+    "a window beyond 65,535": dict(R=2, V=900, window=70000, biases=40, states=3, seed=7),
+    "biases beyond 65,534": dict(R=3, V=30011, window=20, biases=30011, states=0, seed=9),
     "rows of many requests": dict(R=5, V=700, window=30, biases=12, states=6, requests=19, seed=6),
     "penalties alone": dict(R=3, V=9000, window=50),
     "biases alone": dict(R=3, V=9000, biases=50),
