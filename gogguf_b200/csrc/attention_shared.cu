@@ -8,9 +8,10 @@
 // Prefixes: a tile is up to 128 rows of a tensor-core product, members of a group times the query heads of a kv head.  Per page
 // of 64 keys S = Q K^T (tcgen05.mma 128 x 128 x 16, two pages at once) lands in tensor memory, four warps take a row per thread, leave P as bfloat16
 // where S was and O += P V accumulates in tensor memory, as in the prefill kernel (attention_fast.cu), without its masks: every
-// reader sees every key of the prefix.  All (group, tile, kv head)s' pages are one line of work cut into equal runs, one per CTA,
-// so that neither the number of readers nor that of kv heads leaves an SM without work, and the grid is the same for every plan:
-// a captured step replays with other groups.
+// reader sees every key of the prefix.  The pages of a group's kv heads are one line of work cut into equal runs, one per CTA and
+// tile, so that neither the number of readers nor that of kv heads leaves an SM without work; the CTAs of a group's tiles that
+// read the same pages stand side by side, so that they read them once from memory (64 rows of 32 heads on 512 pages, each tile's
+// pages in a line of their own: 225 MB instead of 134).  The grid is the same for every plan: a captured step replays with others.
 //
 // A row's own positions: a CTA a (token row, kv head, share), on mma.sync with the query heads as rows, as the decode kernel of a
 // step without prefixes does it (attention_fast.cu).  (As rows of the prefix's product, a page of a member's own took the tensor
@@ -28,10 +29,10 @@ constexpr int OWN_STAGES_BYTES = 96 * 1024;
 // The plan, integers of a step, with room for `cap` token rows: how many groups; from word 4 on, per group the place of its first
 // member in `rows` (and one place beyond the last group's), its pages and its first member; `rows`, the members' token rows group
 // by group; per token row the pages that are its prefix (0: none), its group (-1: none) and its place among the group's members.
-// A group's members are cut into tiles of equal size; the units of work are the pages of (group, tile, kv head) in that order, and
-// run c takes `per` of them from c per on.  The part that run c leaves of a (tile, kv head) begins at row row0 + 128 c, with row0
-// the rows of all (tile, kv head)s before: later parts are later in c or in row0, and 128 is the most a part has, so no two
-// overlap.
+// A group's members are cut into tiles of equal size.  Its line of work is the pages of kv head 0, of kv head 1 and so on, cut into
+// segments of `per` pages; a run is a segment and a tile, and run c is CTA c's (and run c + CTAs, should there be more).  What a run
+// leaves of a kv head is a part of as many rows as its tile has.  A tile's parts lie one behind the other, the one of segment s and
+// head h as number s + h: later parts are later in s or in h, so no two are the same.
 struct SharedArgs {
     const int* plan;
     int cap, runs, shares;            // token rows that the plan has room for; runs; CTAs that share a row's own pages
@@ -57,52 +58,73 @@ struct SharedPlan {
         const int n = tiles(members, G);
         return (members + n - 1) / n;
     }
-    // units of a run: as many for each
-    static __device__ __forceinline__ int per(int total, int runs) { return max(1, (total + runs - 1) / runs); }
+    // A lane's group, and for all groups before it: runs, and rows of their parts.
+    struct Group { int before, rows, pages, first, members, lead, segments; };
 
-    // All units, and the group that unit u is of (u < 0: group `which`), by a whole warp: a lane a group.
-    struct Group { int before, pages, first, members, lead; };
-    __device__ __forceinline__ Group find(int u, int which, int nkv, int G, int lane, int& total) const {
-        Group found = {};
-        int groups = 1;
-        total = 0;
+    // Runs of all groups with segments of `per` pages (per 0: pages of all runs); by a whole warp.
+    __device__ __forceinline__ int runs(int per, int nkv, int G, int lane) const {
+        int groups = 1, sum = 0;
         for (int g0 = 0; g0 < groups; g0 += 32) {
             const int g = min(g0 + lane, cap - 1);
             // (asked for before the number of groups is known: beyond the last one stands something that is not used)
+            const int pg = pages[g], m = first[g + 1] - first[g];
+            if (g0 == 0) groups = *count;
+            if (g0 + lane < groups) sum += tiles(m, G) * (per > 0 ? (pg * nkv + per - 1) / per : pg * nkv);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        return sum;
+    }
+    // The shortest segments, or nearly, that give every CTA one run at most: one round more costs all that the others wait.
+    __device__ __forceinline__ int per(int ctas, int nkv, int G, int lane) const {
+        const int total = runs(0, nkv, G, lane), least = max(1, (total + ctas - 1) / ctas);
+        int n = least;
+        for (int tries = 0; tries < 8 && runs(n, nkv, G, lane) > ctas; ++tries) n += max(1, least / 8);
+        return n;
+    }
+    // The group that run c is of (c < 0: group `which`).
+    __device__ __forceinline__ Group find(int c, int which, int per, int nkv, int G, int lane) const {
+        Group found = {};
+        int groups = 1, runs_before = 0, rows_before = 0;
+        for (int g0 = 0; g0 < groups; g0 += 32) {
+            const int g = min(g0 + lane, cap - 1);
             const int pg = pages[g], f = first[g], m = first[g + 1] - f, head = lead[g];
             if (g0 == 0) groups = *count;
-            const int units = g0 + lane < groups ? pg * tiles(m, G) * nkv : 0;
-            int upto = units;
+            const bool is = g0 + lane < groups;
+            const int segs = is ? (pg * nkv + per - 1) / per : 0, n = is ? tiles(m, G) * segs : 0, rows = is ? m * G * (segs + nkv) : 0;
+            int upto = n, rows_upto = rows;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += x;
+                const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, rows_upto, o);
+                if (lane >= o) { upto += x; rows_upto += y; }
             }
-            upto += total;
-            const bool it = u < 0 ? g0 + lane == which : u >= upto - units && u < upto;
-            const unsigned mine = __ballot_sync(0xffffffffu, it && units > 0);
+            upto += runs_before;
+            rows_upto += rows_before;
+            const unsigned mine = __ballot_sync(0xffffffffu, is && (c < 0 ? g0 + lane == which : c >= upto - n && c < upto));
             if (mine != 0) {
                 const int from = __ffs(mine) - 1;
-                found.before = __shfl_sync(0xffffffffu, upto - units, from);
+                found.before = __shfl_sync(0xffffffffu, upto - n, from);
+                found.rows = __shfl_sync(0xffffffffu, rows_upto - rows, from);
                 found.pages = __shfl_sync(0xffffffffu, pg, from);
                 found.first = __shfl_sync(0xffffffffu, f, from);
                 found.members = __shfl_sync(0xffffffffu, m, from);
                 found.lead = __shfl_sync(0xffffffffu, head, from);
+                found.segments = __shfl_sync(0xffffffffu, segs, from);
             }
-            total = __shfl_sync(0xffffffffu, upto, 31);
+            runs_before = __shfl_sync(0xffffffffu, upto, 31);
+            rows_before = __shfl_sync(0xffffffffu, rows_upto, 31);
         }
         return found;
     }
     // where the parts of a token row and kv head are (see SharedArgs), by a whole warp
-    __device__ __forceinline__ int4 where(int tok, int kvh, int nkv, int G, int runs, int lane) const {
+    __device__ __forceinline__ int4 where(int tok, int kvh, int nkv, int G, int ctas, int lane) const {
         const int which = group_of[tok], mine = member_of[tok];
         if (which < 0) return make_int4(0, 0, 0, 0);
-        int total;
-        const Group g = find(-1, which, nkv, G, lane, total);
-        const int tm = tile_members(g.members, G), p = per(total, runs), tile = mine / tm;
-        const int u0 = g.before + (tile * nkv + kvh) * g.pages, c0 = u0 / p, c1 = (u0 + g.pages - 1) / p;
-        const int members = min(tm, g.members - tile * tm);
-        return make_int4(nkv * G * (g.first + tile * tm) + kvh * G * members + c0 * ROWS, c1 - c0 + 1, (mine - tile * tm) * G, members * G);
+        const int n = per(ctas, nkv, G, lane);
+        const Group g = find(-1, which, n, nkv, G, lane);
+        const int tm = tile_members(g.members, G), tile = mine / tm, rows = min(tm, g.members - tile * tm) * G;
+        const int s0 = kvh * g.pages / n, s1 = ((kvh + 1) * g.pages - 1) / n;
+        return make_int4(g.rows + tile * tm * G * (g.segments + nkv) + (s0 + kvh) * rows, s1 - s0 + 1, (mine - tile * tm) * G, rows);
     }
 };
 
@@ -149,13 +171,11 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     uint32_t* tmem_slot = (uint32_t*)(bars + 8);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, run = (int)blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const SharedPlan plan(args);
-    int total;
-    plan.find(-1, -1, nkv, G, lane, total);
-    const int per = plan.per(total, args.runs), u_begin = min(run * per, total), u_end = min(u_begin + per, total);
+    const int per = plan.per((int)gridDim.x, nkv, G, lane), runs = plan.runs(per, nkv, G, lane);
     // The next kernel's CTAs are let in when q is there, which they need and this kernel's work they do not.
-    if (u_begin >= u_end) {
+    if ((int)blockIdx.x >= runs) {
         pdl_wait();
         return;
     }
@@ -178,22 +198,38 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     bool ok = (tma::smem_u32(smem) & 1023u) == 0;
     if (!ok && threadIdx.x == 0) atomicCAS(status, 0, 29);
 
-    // The run is cut where the (tile, kv head) changes.  Every role walks the same cuts.
+    // A run is cut where the kv head changes.  Every role walks the same cuts.
     struct Piece { int first, members, head, page0, pages, lead; size_t row0; };
-    auto piece_at = [&](int u) -> Piece {
-        int all;
-        const SharedPlan::Group g = plan.find(u, -1, nkv, G, lane, all);
-        const int tm = plan.tile_members(g.members, G), rel = u - g.before;
-        const int th = rel / g.pages, tile = th / nkv;
-        Piece r;
-        r.head = th - tile * nkv;
-        r.page0 = rel - th * g.pages;
-        r.pages = min(g.pages - r.page0, u_end - u);
-        r.first = g.first + tile * tm;
-        r.members = min(tm, g.members - tile * tm);
-        r.lead = g.lead;
-        r.row0 = (size_t)nkv * G * r.first + (size_t)r.head * G * r.members + (size_t)run * ROWS;
-        return r;
+    struct Walk {
+        SharedPlan::Group g;
+        int c, at, end, tile, segment;
+    };
+    auto start = [&](int c) -> Walk {
+        Walk w;
+        w.c = c;
+        w.g = plan.find(c, -1, per, nkv, G, lane);
+        const int nt = plan.tiles(w.g.members, G), local = c - w.g.before;
+        w.segment = local / nt;
+        w.tile = local - w.segment * nt;
+        w.at = w.segment * per;
+        w.end = min(w.at + per, w.g.pages * nkv);
+        return w;
+    };
+    auto next = [&](Walk& w, Piece& r) -> bool {
+        if (w.at >= w.end) {
+            if (w.c + (int)gridDim.x >= runs) return false;
+            w = start(w.c + (int)gridDim.x);
+        }
+        const int tm = plan.tile_members(w.g.members, G);
+        r.head = w.at / w.g.pages;
+        r.page0 = w.at - r.head * w.g.pages;
+        r.pages = min(w.g.pages - r.page0, w.end - w.at);
+        r.first = w.g.first + w.tile * tm;
+        r.members = min(tm, w.g.members - w.tile * tm);
+        r.lead = w.g.lead;
+        r.row0 = (size_t)w.g.rows + (size_t)w.tile * tm * G * (w.g.segments + nkv) + (size_t)(w.segment + r.head) * r.members * G;
+        w.at += r.pages;
+        return true;
     };
     // (a warp goes on or leaves as a whole: what follows a wait is for whole warps)
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) -> bool {
@@ -201,13 +237,12 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     };
 
     if (warp == 5 || (warp == 4 && lane != 0)) { pdl_wait(); pdl_launch(); }
+    Piece r;
     int j = 0;                                      // steps of two pages (a piece's last may be one) so far
     if (warp == 4) {
         // The prefix's pages were written by earlier steps (this step's tokens go to pages of the rows' own), so they are
         // streamed before the kernel before this one has finished.
-        for (int u = u_begin; u < u_end;) {
-            const Piece r = piece_at(u);
-            u += r.pages;
+        for (Walk w = start((int)blockIdx.x); next(w, r);) {
             if (lane == 0 && ok) {
                 const int* pt = st.page_table + (size_t)st.seq_of_token[r.lead] * st.max_pages;
                 for (int i = 0; i < r.pages; i += 2, ++j) {
@@ -239,9 +274,7 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
         const uint64_t dw = tc5::smem_desc(tma::smem_u32(Vs), COL, 1024);
         auto moved = [](uint64_t desc, uint32_t bytes) -> uint64_t { return desc & 0xffffffff00000000ull | (uint32_t)desc + (bytes >> 4); };
         int pieces = 0;
-        for (int u = u_begin; u < u_end; ++pieces) {
-            const Piece r = piece_at(u);
-            u += r.pages;
+        for (Walk w = start((int)blockIdx.x); next(w, r); ++pieces) {
             if (lane == 0 && ok) {
                 // (a piece's first scores come after the last P V of the piece before: its Q is written when that is read)
                 ok = tma::mbar_wait(q_full, (uint32_t)(pieces & 1), abort_flag, status, 74);
@@ -278,9 +311,7 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
         const int row = threadIdx.x;                           // row of the tile = tensor-memory lane
         const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
         int pieces = 0;
-        for (int u = u_begin; u < u_end && ok; ++pieces) {
-            const Piece r = piece_at(u);
-            u += r.pages;
+        for (Walk w = start((int)blockIdx.x); ok && next(w, r); ++pieces) {
             const int rows = r.members * G;
             const bool live = row < rows, idle = warp * 32 >= rows;     // (a warp without rows only keeps the pace)
             const int member = live ? row / G : 0;
@@ -657,7 +688,7 @@ __global__ void __launch_bounds__(JOIN_HALVES * 16) shared_join_kernel(bf16* __r
                 ml[k] = make_float2(-INFINITY, 0.f);
                 a[k] = b[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (i < n) {
-                    const size_t own = (size_t)args.own_row + (size_t)row * args.shares + (i - at.y), part = (size_t)at.x + (size_t)i * ROWS;
+                    const size_t own = (size_t)args.own_row + (size_t)row * args.shares + (i - at.y), part = (size_t)at.x + (size_t)i * at.w;
                     ml[k] = args.part_ml[i < at.y ? part + r : own];
                     const float4* src = reinterpret_cast<const float4*>(args.part_o + (i < at.y ? part * dv + ((size_t)lane * at.w + r) * 8 : own * dv + c));
                     if (c < dv) { a[k] = src[0]; b[k] = src[1]; }
@@ -706,7 +737,7 @@ int launch_shared(const CUtensorMap& tk, const CUtensorMap& tv, int ntok, const 
 }  // namespace
 
 // Decode attention (see gg_attn_decode_tma) of a step with shared prefixes: plan as at SharedArgs; runs (1 to 296): CTAs over
-// the prefixes; shares (1 to 64): CTAs that share a row's own pages; part: scratch of (nq ntok (1 + shares) + 128 runs) (dv + 2) + 4 ntok nkv floats, on a 32-byte boundary.
+// the prefixes; shares (1 to 64): CTAs that share a row's own pages; part: scratch of (nq ntok (2 + shares) + 128 runs) (dv + 2) + 4 ntok nkv floats, on a 32-byte boundary.
 // status: codes 71-79 (prefixes), 11 and 12 (own pages) name the wait that ran out.
 GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_pool, void* out, const int* positions,
                              const int* seq_of_token, const int* page_table, int max_pages, int page_size, int n_pages, const int* plan,
@@ -718,7 +749,7 @@ GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_po
         return GG_ERR_ARG;
     if ((((uintptr_t)q) & 15) || (((uintptr_t)k_pool) & 15) || (((uintptr_t)v_pool) & 15) || (((uintptr_t)out) & 15) || (((uintptr_t)part) & 31))
         return GG_ERR_ARG;
-    const long long prefix_rows = (long long)nq * ntok + (long long)ROWS * runs, rows = prefix_rows + (long long)nq * ntok * shares;
+    const long long prefix_rows = 2ll * nq * ntok + (long long)ROWS * runs, rows = prefix_rows + (long long)nq * ntok * shares;
     if (part == nullptr || part_floats < rows * (dv + 2) + 4ll * ntok * nkv || rows > 0x7fffffffll) return GG_ERR_ARG;
     // (units, blocks and the rows of the pools are counted in 32 bits: a row lists at most max_pages pages)
     const unsigned long long pool_rows = (unsigned long long)n_pages * nkv * PAGE;

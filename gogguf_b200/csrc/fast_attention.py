@@ -64,7 +64,7 @@ def shared_scratch(n_tokens: int, nq: int, nkv: int, dv: int, shares: Optional[i
         raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {dv}, {n_tokens} tokens")
     if shares is None:
         shares = shared_shares(n_tokens, nkv, 2 * SHARED_SHARES)
-    return (nq * n_tokens * (1 + shares) + SHARED_ROWS * SHARED_RUNS) * (dv + 2) + 4 * n_tokens * nkv
+    return (nq * n_tokens * (2 + shares) + SHARED_ROWS * SHARED_RUNS) * (dv + 2) + 4 * n_tokens * nkv
 
 
 def shared_shares(n_tokens: int, nkv: int, own_pages: int) -> int:
