@@ -6,12 +6,11 @@
 // by side, so that what computes and what waits for memory share the SMs; a third adds them, always in the same order.
 //
 // Prefixes: a tile is up to 128 rows of a tensor-core product, members of a group times the query heads of a kv head.  Per page
-// of 64 keys S = Q K^T (tcgen05.mma 128 x 128 x 16, two pages at once) lands in tensor memory, four warps take a row per thread, leave P as bfloat16
+// of 64 keys S = Q K^T (tcgen05.mma 128 x 64 x 16) lands in tensor memory, four warps take a row per thread, leave P as bfloat16
 // where S was and O += P V accumulates in tensor memory, as in the prefill kernel (attention_fast.cu), without its masks: every
-// reader sees every key of the prefix.  The pages of a group's kv heads are one line of work cut into equal runs, one per CTA and
-// tile, so that neither the number of readers nor that of kv heads leaves an SM without work; the CTAs of a group's tiles that
-// read the same pages stand side by side, so that they read them once from memory (64 rows of 32 heads on 512 pages, each tile's
-// pages in a line of their own: 225 MB instead of 134).  The grid is the same for every plan: a captured step replays with others.
+// reader sees every key of the prefix.  All (group, tile, kv head)s' pages are one line of work cut into equal runs, one per CTA,
+// so that neither the number of readers nor that of kv heads leaves an SM without work, and the grid is the same for every plan:
+// a captured step replays with other groups.
 //
 // A row's own positions: a CTA a (token row, kv head, share), on mma.sync with the query heads as rows, as the decode kernel of a
 // step without prefixes does it (attention_fast.cu).  (As rows of the prefix's product, a page of a member's own took the tensor
@@ -29,10 +28,10 @@ constexpr int OWN_STAGES_BYTES = 96 * 1024;
 // The plan, integers of a step, with room for `cap` token rows: how many groups; from word 4 on, per group the place of its first
 // member in `rows` (and one place beyond the last group's), its pages and its first member; `rows`, the members' token rows group
 // by group; per token row the pages that are its prefix (0: none), its group (-1: none) and its place among the group's members.
-// A group's members are cut into tiles of equal size.  Its line of work is the pages of kv head 0, of kv head 1 and so on, cut into
-// segments of `per` pages; a run is a segment and a tile, and run c is CTA c's (and run c + CTAs, should there be more).  What a run
-// leaves of a kv head is a part of as many rows as its tile has.  A tile's parts lie one behind the other, the one of segment s and
-// head h as number s + h: later parts are later in s or in h, so no two are the same.
+// A group's members are cut into tiles of equal size; the units of work are the pages of (group, tile, kv head) in that order, and
+// run c takes `per` of them from c per on.  The part that run c leaves of a (tile, kv head) begins at row row0 + 128 c, with row0
+// the rows of all (tile, kv head)s before: later parts are later in c or in row0, and 128 is the most a part has, so no two
+// overlap.
 struct SharedArgs {
     const int* plan;
     int cap, runs, shares;            // token rows that the plan has room for; runs; CTAs that share a row's own pages
@@ -58,73 +57,52 @@ struct SharedPlan {
         const int n = tiles(members, G);
         return (members + n - 1) / n;
     }
-    // A lane's group, and for all groups before it: runs, and rows of their parts.
-    struct Group { int before, rows, pages, first, members, lead, segments; };
+    // units of a run: as many for each
+    static __device__ __forceinline__ int per(int total, int runs) { return max(1, (total + runs - 1) / runs); }
 
-    // Runs of all groups with segments of `per` pages (per 0: pages of all runs); by a whole warp.
-    __device__ __forceinline__ int runs(int per, int nkv, int G, int lane) const {
-        int groups = 1, sum = 0;
+    // All units, and the group that unit u is of (u < 0: group `which`), by a whole warp: a lane a group.
+    struct Group { int before, pages, first, members, lead; };
+    __device__ __forceinline__ Group find(int u, int which, int nkv, int G, int lane, int& total) const {
+        Group found = {};
+        int groups = 1;
+        total = 0;
         for (int g0 = 0; g0 < groups; g0 += 32) {
             const int g = min(g0 + lane, cap - 1);
             // (asked for before the number of groups is known: beyond the last one stands something that is not used)
-            const int pg = pages[g], m = first[g + 1] - first[g];
-            if (g0 == 0) groups = *count;
-            if (g0 + lane < groups) sum += tiles(m, G) * (per > 0 ? (pg * nkv + per - 1) / per : pg * nkv);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        return sum;
-    }
-    // The shortest segments, or nearly, that give every CTA one run at most: one round more costs all that the others wait.
-    __device__ __forceinline__ int per(int ctas, int nkv, int G, int lane) const {
-        const int total = runs(0, nkv, G, lane), least = max(1, (total + ctas - 1) / ctas);
-        int n = least;
-        for (int tries = 0; tries < 8 && runs(n, nkv, G, lane) > ctas; ++tries) n += max(1, least / 8);
-        return n;
-    }
-    // The group that run c is of (c < 0: group `which`).
-    __device__ __forceinline__ Group find(int c, int which, int per, int nkv, int G, int lane) const {
-        Group found = {};
-        int groups = 1, runs_before = 0, rows_before = 0;
-        for (int g0 = 0; g0 < groups; g0 += 32) {
-            const int g = min(g0 + lane, cap - 1);
             const int pg = pages[g], f = first[g], m = first[g + 1] - f, head = lead[g];
             if (g0 == 0) groups = *count;
-            const bool is = g0 + lane < groups;
-            const int segs = is ? (pg * nkv + per - 1) / per : 0, n = is ? tiles(m, G) * segs : 0, rows = is ? m * G * (segs + nkv) : 0;
-            int upto = n, rows_upto = rows;
+            const int units = g0 + lane < groups ? pg * tiles(m, G) * nkv : 0;
+            int upto = units;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, rows_upto, o);
-                if (lane >= o) { upto += x; rows_upto += y; }
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
             }
-            upto += runs_before;
-            rows_upto += rows_before;
-            const unsigned mine = __ballot_sync(0xffffffffu, is && (c < 0 ? g0 + lane == which : c >= upto - n && c < upto));
+            upto += total;
+            const bool it = u < 0 ? g0 + lane == which : u >= upto - units && u < upto;
+            const unsigned mine = __ballot_sync(0xffffffffu, it && units > 0);
             if (mine != 0) {
                 const int from = __ffs(mine) - 1;
-                found.before = __shfl_sync(0xffffffffu, upto - n, from);
-                found.rows = __shfl_sync(0xffffffffu, rows_upto - rows, from);
+                found.before = __shfl_sync(0xffffffffu, upto - units, from);
                 found.pages = __shfl_sync(0xffffffffu, pg, from);
                 found.first = __shfl_sync(0xffffffffu, f, from);
                 found.members = __shfl_sync(0xffffffffu, m, from);
                 found.lead = __shfl_sync(0xffffffffu, head, from);
-                found.segments = __shfl_sync(0xffffffffu, segs, from);
             }
-            runs_before = __shfl_sync(0xffffffffu, upto, 31);
-            rows_before = __shfl_sync(0xffffffffu, rows_upto, 31);
+            total = __shfl_sync(0xffffffffu, upto, 31);
         }
         return found;
     }
     // where the parts of a token row and kv head are (see SharedArgs), by a whole warp
-    __device__ __forceinline__ int4 where(int tok, int kvh, int nkv, int G, int ctas, int lane) const {
+    __device__ __forceinline__ int4 where(int tok, int kvh, int nkv, int G, int runs, int lane) const {
         const int which = group_of[tok], mine = member_of[tok];
         if (which < 0) return make_int4(0, 0, 0, 0);
-        const int n = per(ctas, nkv, G, lane);
-        const Group g = find(-1, which, n, nkv, G, lane);
-        const int tm = tile_members(g.members, G), tile = mine / tm, rows = min(tm, g.members - tile * tm) * G;
-        const int s0 = kvh * g.pages / n, s1 = ((kvh + 1) * g.pages - 1) / n;
-        return make_int4(g.rows + tile * tm * G * (g.segments + nkv) + (s0 + kvh) * rows, s1 - s0 + 1, (mine - tile * tm) * G, rows);
+        int total;
+        const Group g = find(-1, which, nkv, G, lane, total);
+        const int tm = tile_members(g.members, G), p = per(total, runs), tile = mine / tm;
+        const int u0 = g.before + (tile * nkv + kvh) * g.pages, c0 = u0 / p, c1 = (u0 + g.pages - 1) / p;
+        const int members = min(tm, g.members - tile * tm);
+        return make_int4(nkv * G * (g.first + tile * tm) + kvh * G * members + c0 * ROWS, c1 - c0 + 1, (mine - tile * tm) * G, members * G);
     }
 };
 
@@ -154,36 +132,42 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     int* status = st.status;
     constexpr int QBOX = ROWS * 64 * 2;             // [64 columns x 128 rows] of Q: 16 KB
     constexpr int KBOX = 64 * 64 * 2;               // [64 columns x 64 keys] of K or V: 8 KB
-    constexpr int Q_BYTES = HK * QBOX, COL = 2 * KBOX;      // a step's two pages of K or V: 64 columns of both, then the next 64
-    constexpr int TMEM_COLS = 256;                  // scores of 128 keys, then O
+    constexpr int Q_BYTES = HK * QBOX, K_STAGE = HK * KBOX, V_STAGE = HV * KBOX;
+    constexpr int TMEM_COLS = 256;                  // two score buffers of 64 columns, then O
     uint8_t* Qs = smem;
-    uint8_t* Ks = Qs + Q_BYTES;
-    uint8_t* Vs = Ks + HK * COL;
-    uint64_t* bars = (uint64_t*)(Vs + HV * COL);
-    uint64_t* q_full = bars;                        // the four softmax warps have written a piece's Q
-    uint64_t* k_full = bars + 1;
-    uint64_t* k_empty = bars + 2;
-    uint64_t* v_full = bars + 3;
-    uint64_t* v_empty = bars + 4;
-    uint64_t* s_full = bars + 5;
-    uint64_t* p_ready = bars + 6;
-    uint64_t* o_done = bars + 7;                    // every P V of a piece is complete
-    uint32_t* tmem_slot = (uint32_t*)(bars + 8);
+    uint8_t* Ks = Qs + Q_BYTES;                     // two stages
+    uint8_t* Vs = Ks + 2 * K_STAGE;                 // two stages
+    uint64_t* bars = (uint64_t*)(Vs + 2 * V_STAGE);
+    uint64_t* q_full = bars;                        // the four softmax warps have written a run's Q
+    uint64_t* k_full = bars + 1;                    // [2]
+    uint64_t* k_empty = bars + 3;                   // [2]
+    uint64_t* v_full = bars + 5;                    // [2]
+    uint64_t* v_empty = bars + 7;                   // [2]
+    uint64_t* s_full = bars + 9;                    // [2]
+    uint64_t* p_ready = bars + 11;                  // [2] (two in turn: a warp may be a page ahead of another)
+    uint64_t* pv_done = bars + 13;
+    uint64_t* o_done = bars + 14;                   // every P V of a run's (tile, kv head) is complete
+    uint32_t* tmem_slot = (uint32_t*)(bars + 15);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, run = (int)blockIdx.x;
     const SharedPlan plan(args);
-    const int per = plan.per((int)gridDim.x, nkv, G, lane), runs = plan.runs(per, nkv, G, lane);
+    int total;
+    plan.find(-1, -1, nkv, G, lane, total);
+    const int per = plan.per(total, args.runs), u_begin = min(run * per, total), u_end = min(u_begin + per, total);
     // The next kernel's CTAs are let in when q is there, which they need and this kernel's work they do not.
-    if ((int)blockIdx.x >= runs) {
+    if (u_begin >= u_end) {
         pdl_wait();
         return;
     }
     if (threadIdx.x == 0) {
         tma::mbar_init(q_full, 4);
-        tma::mbar_init(k_full, 1); tma::mbar_init(k_empty, 1);
-        tma::mbar_init(v_full, 1); tma::mbar_init(v_empty, 1);
-        tma::mbar_init(s_full, 1); tma::mbar_init(p_ready, 4);
+        for (int i = 0; i < 2; ++i) {
+            tma::mbar_init(&k_full[i], 1); tma::mbar_init(&k_empty[i], 1);
+            tma::mbar_init(&v_full[i], 1); tma::mbar_init(&v_empty[i], 1);
+            tma::mbar_init(&s_full[i], 1); tma::mbar_init(&p_ready[i], 4);
+        }
+        tma::mbar_init(pv_done, 1);
         tma::mbar_init(o_done, 1);
         *abort_flag = 0;
         tma::mbar_fence_init();
@@ -198,38 +182,22 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     bool ok = (tma::smem_u32(smem) & 1023u) == 0;
     if (!ok && threadIdx.x == 0) atomicCAS(status, 0, 29);
 
-    // A run is cut where the kv head changes.  Every role walks the same cuts.
+    // The run is cut where the (tile, kv head) changes.  Every role walks the same cuts.
     struct Piece { int first, members, head, page0, pages, lead; size_t row0; };
-    struct Walk {
-        SharedPlan::Group g;
-        int c, at, end, tile, segment;
-    };
-    auto start = [&](int c) -> Walk {
-        Walk w;
-        w.c = c;
-        w.g = plan.find(c, -1, per, nkv, G, lane);
-        const int nt = plan.tiles(w.g.members, G), local = c - w.g.before;
-        w.segment = local / nt;
-        w.tile = local - w.segment * nt;
-        w.at = w.segment * per;
-        w.end = min(w.at + per, w.g.pages * nkv);
-        return w;
-    };
-    auto next = [&](Walk& w, Piece& r) -> bool {
-        if (w.at >= w.end) {
-            if (w.c + (int)gridDim.x >= runs) return false;
-            w = start(w.c + (int)gridDim.x);
-        }
-        const int tm = plan.tile_members(w.g.members, G);
-        r.head = w.at / w.g.pages;
-        r.page0 = w.at - r.head * w.g.pages;
-        r.pages = min(w.g.pages - r.page0, w.end - w.at);
-        r.first = w.g.first + w.tile * tm;
-        r.members = min(tm, w.g.members - w.tile * tm);
-        r.lead = w.g.lead;
-        r.row0 = (size_t)w.g.rows + (size_t)w.tile * tm * G * (w.g.segments + nkv) + (size_t)(w.segment + r.head) * r.members * G;
-        w.at += r.pages;
-        return true;
+    auto piece_at = [&](int u) -> Piece {
+        int all;
+        const SharedPlan::Group g = plan.find(u, -1, nkv, G, lane, all);
+        const int tm = plan.tile_members(g.members, G), rel = u - g.before;
+        const int th = rel / g.pages, tile = th / nkv;
+        Piece r;
+        r.head = th - tile * nkv;
+        r.page0 = rel - th * g.pages;
+        r.pages = min(g.pages - r.page0, u_end - u);
+        r.first = g.first + tile * tm;
+        r.members = min(tm, g.members - tile * tm);
+        r.lead = g.lead;
+        r.row0 = (size_t)nkv * G * r.first + (size_t)r.head * G * r.members + (size_t)run * ROWS;
+        return r;
     };
     // (a warp goes on or leaves as a whole: what follows a wait is for whole warps)
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) -> bool {
@@ -237,71 +205,77 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     };
 
     if (warp == 5 || (warp == 4 && lane != 0)) { pdl_wait(); pdl_launch(); }
-    Piece r;
-    int j = 0;                                      // steps of two pages (a piece's last may be one) so far
+    int j = 0;                                      // pages so far
     if (warp == 4) {
         // The prefix's pages were written by earlier steps (this step's tokens go to pages of the rows' own), so they are
         // streamed before the kernel before this one has finished.
-        for (Walk w = start((int)blockIdx.x); next(w, r);) {
+        for (int u = u_begin; u < u_end;) {
+            const Piece r = piece_at(u);
+            u += r.pages;
             if (lane == 0 && ok) {
                 const int* pt = st.page_table + (size_t)st.seq_of_token[r.lead] * st.max_pages;
-                for (int i = 0; i < r.pages; i += 2, ++j) {
-                    const int n = min(2, r.pages - i);
-                    const uint32_t ph = (uint32_t)(j & 1) ^ 1u;
-                    int at[2];
-                    for (int g = 0; g < n; ++g)
-                        at[g] = (gg_page(pt, r.page0 + i + g, st.max_pages, PageBounds{st.n_pages, status}, 54) * nkv + r.head) * PAGE;
-                    if (!(ok = tma::mbar_wait(k_empty, ph, abort_flag, status, 71))) break;
-                    tma::mbar_expect_tx(k_full, (uint32_t)(n * HK * KBOX));
-                    for (int g = 0; g < n; ++g)
+                for (int i = 0; i < r.pages; ++i, ++j) {
+                    const int s = j & 1;
+                    const uint32_t ph = (uint32_t)((j >> 1) & 1) ^ 1u;
+                    const int row = (gg_page(pt, r.page0 + i, st.max_pages, PageBounds{st.n_pages, status}, 54) * nkv + r.head) * PAGE;
+                    if (!(ok = tma::mbar_wait(&k_empty[s], ph, abort_flag, status, 71))) break;
+                    tma::mbar_expect_tx(&k_full[s], K_STAGE);
 #pragma unroll
-                        for (int hf = 0; hf < HK; ++hf) tma::load_2d(Ks + hf * COL + g * KBOX, &tmK, k_full, hf * 64, at[g]);
-                    if (!(ok = tma::mbar_wait(v_empty, ph, abort_flag, status, 72))) break;
-                    tma::mbar_expect_tx(v_full, (uint32_t)(n * HV * KBOX));
-                    for (int g = 0; g < n; ++g)
+                    for (int hf = 0; hf < HK; ++hf) tma::load_2d(Ks + s * K_STAGE + hf * KBOX, &tmK, &k_full[s], hf * 64, row);
+                    if (!(ok = tma::mbar_wait(&v_empty[s], ph, abort_flag, status, 72))) break;
+                    tma::mbar_expect_tx(&v_full[s], V_STAGE);
 #pragma unroll
-                        for (int hf = 0; hf < HV; ++hf) tma::load_2d(Vs + hf * COL + g * KBOX, &tmV, v_full, hf * 64, at[g]);
-                    if (j == 0) { pdl_wait(); pdl_launch(); }
+                    for (int hf = 0; hf < HV; ++hf) tma::load_2d(Vs + s * V_STAGE + hf * KBOX, &tmV, &v_full[s], hf * 64, row);
+                    if (j == 1 || u >= u_end && i + 1 == r.pages) { pdl_wait(); pdl_launch(); }
                 }
             }
             __syncwarp();
         }
     } else if (warp == 5) {
-        const uint32_t idesc_qk[2] = {tc5::idesc_bf16(ROWS, 64, 0), tc5::idesc_bf16(ROWS, 128, 0)};
-        const uint32_t idesc_pv = tc5::idesc_bf16(ROWS, EXACT ? DV : (dv + 15) & ~15, 1);
+        const uint32_t idesc_qk = tc5::idesc_bf16(ROWS, 64, 0), idesc_pv = tc5::idesc_bf16(ROWS, EXACT ? DV : (dv + 15) & ~15, 1);
         // A matrix descriptor's upper word is the same for all; of the lower one an operand's place is added, in 16 bytes.
         const uint64_t dq = tc5::smem_desc(tma::smem_u32(Qs), 16, 1024), dk = tc5::smem_desc(tma::smem_u32(Ks), 16, 1024);
-        const uint64_t dw = tc5::smem_desc(tma::smem_u32(Vs), COL, 1024);
+        const uint64_t dw = tc5::smem_desc(tma::smem_u32(Vs), KBOX, 1024);
         auto moved = [](uint64_t desc, uint32_t bytes) -> uint64_t { return desc & 0xffffffff00000000ull | (uint32_t)desc + (bytes >> 4); };
+        auto issue_scores = [&](int j) -> bool {
+            const int s = j & 1;
+            if (!tma::mbar_wait(&k_full[s], (uint32_t)((j >> 1) & 1), abort_flag, status, 73)) return false;
+            tc5::fence_after();
+            const uint64_t dks = moved(dk, (uint32_t)(s * K_STAGE));
+#pragma unroll
+            for (int ks = 0; ks < DK / 16; ++ks) {
+                if (!EXACT && ks * 16 >= d) break;
+                tc5::mma(S_t + (uint32_t)(s * 64), moved(dq, (uint32_t)((ks >> 2) * QBOX + (ks & 3) * 32)),
+                         moved(dks, (uint32_t)((ks >> 2) * KBOX + (ks & 3) * 32)), idesc_qk, ks > 0 ? 1u : 0u);
+            }
+            tc5::commit(&s_full[s]);
+            tc5::commit(&k_empty[s]);
+            return true;
+        };
         int pieces = 0;
-        for (Walk w = start((int)blockIdx.x); next(w, r); ++pieces) {
+        for (int u = u_begin; u < u_end; ++pieces) {
+            const Piece r = piece_at(u);
+            u += r.pages;
             if (lane == 0 && ok) {
                 // (a piece's first scores come after the last P V of the piece before: its Q is written when that is read)
                 ok = tma::mbar_wait(q_full, (uint32_t)(pieces & 1), abort_flag, status, 74);
-                for (int i = 0; i < r.pages && ok; i += 2, ++j) {
-                    const int n = min(2, r.pages - i);
-                    const uint32_t ph = (uint32_t)(j & 1);
-                    if (!(ok = tma::mbar_wait(k_full, ph, abort_flag, status, 73))) break;
+                if (ok) ok = issue_scores(j);
+                for (int i = 0; i < r.pages && ok; ++i, ++j) {
+                    // The next page's scores do not wait for this page's softmax: their buffer was last read by the
+                    // softmax of page j - 1, whose p_ready this thread has already seen.
+                    if (i + 1 < r.pages && !(ok = issue_scores(j + 1))) break;
+                    const int s = j & 1;
+                    const uint32_t ph = (uint32_t)((j >> 1) & 1);
+                    if (!(ok = tma::mbar_wait(&v_full[s], ph, abort_flag, status, 76))) break;
+                    if (!(ok = tma::mbar_wait(&p_ready[s], ph, abort_flag, status, 75))) break;
                     tc5::fence_after();
-                    // (over the P of the step before, which the products before these have read: the tensor core works in order)
+                    const uint64_t dvs = moved(dw, (uint32_t)(s * V_STAGE));
 #pragma unroll
-                    for (int ks = 0; ks < DK / 16; ++ks) {
-                        if (!EXACT && ks * 16 >= d) break;
-                        tc5::mma(S_t, moved(dq, (uint32_t)((ks >> 2) * QBOX + (ks & 3) * 32)), moved(dk, (uint32_t)((ks >> 2) * COL + (ks & 3) * 32)),
-                                 idesc_qk[n - 1], ks > 0 ? 1u : 0u);
-                    }
-                    tc5::commit(s_full);
-                    tc5::commit(k_empty);
-                    if (!(ok = tma::mbar_wait(v_full, ph, abort_flag, status, 76))) break;
-                    if (!(ok = tma::mbar_wait(p_ready, ph, abort_flag, status, 75))) break;
-                    tc5::fence_after();
-                    for (int g = 0; g < n; ++g)
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            // P lies in the first columns of the scores: 16 keys are 8 columns
-                            tc5::mma_a_tmem(O_t, S_t + (uint32_t)(g * 32 + kk * 8), moved(dw, (uint32_t)(g * KBOX + kk * 2048)), idesc_pv,
-                                            (i > 0 || g > 0 || kk > 0) ? 1u : 0u);
-                    tc5::commit(v_empty);
+                    for (int kk = 0; kk < 4; ++kk)
+                        // P of page j lies in the first 32 columns of score buffer j & 1: 16 keys are 8 columns
+                        tc5::mma_a_tmem(O_t, S_t + (uint32_t)(s * 64 + kk * 8), moved(dvs, (uint32_t)(kk * 2048)), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+                    tc5::commit(pv_done);
+                    tc5::commit(&v_empty[s]);
                 }
                 if (ok) tc5::commit(o_done);
             }
@@ -311,27 +285,20 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
         const int row = threadIdx.x;                           // row of the tile = tensor-memory lane
         const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
         int pieces = 0;
-        for (Walk w = start((int)blockIdx.x); ok && next(w, r); ++pieces) {
+        for (int u = u_begin; u < u_end && ok; ++pieces) {
+            const Piece r = piece_at(u);
+            u += r.pages;
             const int rows = r.members * G;
             const bool live = row < rows, idle = warp * 32 >= rows;     // (a warp without rows only keeps the pace)
             const int member = live ? row / G : 0;
-            const int from = live ? (plan.rows[r.first + member] * nq + r.head * G + (row - member * G)) : -1;      // row of q
+            const bf16* src = st.q + ((size_t)plan.rows[r.first + member] * nq + (size_t)r.head * G + (row - member * G)) * d;
             if (pieces == 0) { pdl_wait(); pdl_launch(); }     // q, and the scratch is free
             if (!idle) {
-                // Q into its swizzled tile: row r of a box is 128 bytes, 16-byte chunk c at place c ^ (r & 7).  Half a warp reads a
-                // row (a row per lane instead asked the L1 for 32 lines at a time, 3 us of 128 rows)
-                constexpr int LANES = DK / 8, ROWS_AT_ONCE = 32 / LANES;
-                const int c = lane % LANES;
-                uint4 x[32 / ROWS_AT_ONCE];
+                // Q into its swizzled tile: row r of a box is 128 bytes, 16-byte chunk c at place c ^ (r & 7)
 #pragma unroll
-                for (int k = 0; k < 32 / ROWS_AT_ONCE; ++k) {
-                    const int src = __shfl_sync(0xffffffffu, from, k * ROWS_AT_ONCE + lane / LANES);
-                    x[k] = src >= 0 && (EXACT || c * 8 < d) ? *reinterpret_cast<const uint4*>(st.q + (size_t)src * d + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-                }
-#pragma unroll
-                for (int k = 0; k < 32 / ROWS_AT_ONCE; ++k) {
-                    const int to = warp * 32 + k * ROWS_AT_ONCE + lane / LANES;
-                    *reinterpret_cast<uint4*>(Qs + (c >> 3) * QBOX + to * 128 + (((c & 7) ^ (to & 7)) << 4)) = x[k];
+                for (int c = 0; c < DK / 8; ++c) {
+                    const uint4 x = live && (EXACT || c * 8 < d) ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+                    *reinterpret_cast<uint4*>(Qs + (c >> 3) * QBOX + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = x;
                 }
             }
             tc5::fence_proxy_async_smem();
@@ -339,15 +306,14 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
             __syncwarp();
             if (lane == 0) tma::mbar_arrive(q_full);
             float m_used = -INFINITY, l = 0.f;
-            for (int i = 0; i < r.pages; i += 2, ++j) {
-                const int pages = min(2, r.pages - i);
-                if (!(ok = wait(s_full, (uint32_t)(j & 1), 77))) break;
+            for (int i = 0; i < r.pages; ++i, ++j) {
+                const int s = j & 1;
+                if (!(ok = wait(&s_full[s], (uint32_t)((j >> 1) & 1), 77))) break;
                 tc5::fence_after();
-#pragma unroll 1
-                for (int g = 0; g < pages && !idle; ++g) {
+                if (!idle) {
                     uint32_t sr[64], pk[32];
-                    tc5::ld32(S_t + lane_off + (uint32_t)(g * 64), sr);
-                    tc5::ld32(S_t + lane_off + (uint32_t)(g * 64) + 32, sr + 32);
+                    tc5::ld32(S_t + lane_off + (uint32_t)(s * 64), sr);
+                    tc5::ld32(S_t + lane_off + (uint32_t)(s * 64) + 32, sr + 32);
                     tc5::wait_ld();
                     // P = 2^(score scale - maximum in use) as bfloat16 pairs; returns the sum of the page's P
                     auto exponentials = [&]() -> float {
@@ -366,9 +332,8 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
                         unpack2(add2(add2(l4[0], l4[1]), add2(l4[2], l4[3])), la, lb);
                         return la + lb;
                     };
-                    // The maximum in use is that of the pages before (any is exact while nothing overflows): only where a row has none
-                    // yet, or the page's sum says that a score lies more than 2^64 above it, is the page's own found, what was summed
-                    // rescaled where it has grown by more than 2^8, and the page computed again.
+                    // The maximum in use is that of the pages before (any is exact while nothing overflows): only where a row
+                    // has none yet, or the page's sum says that a score lies more than 2^64 above it, is the page's own found, O rescaled where it has grown by more than 2^8, and the page computed again.
                     float lpage = 0.f;
                     bool again = m_used == -INFINITY;
                     if (!__any_sync(0xffffffffu, again)) {
@@ -393,44 +358,37 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
                                 m_used = mx;
                                 l *= corr;
                             }
-                            auto rescale = [&](uint32_t at, bool pairs) {
-                                uint32_t o[32];
-                                tc5::ld32(at + lane_off, o);
-                                tc5::wait_ld();
-#pragma unroll
-                                for (int c = 0; c < 32; ++c) {
-                                    if (pairs) {
-                                        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&o[c]));
-                                        o[c] = pack_bf16(f.x * corr, f.y * corr);
-                                    } else {
-                                        o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
-                                    }
-                                }
-                                tc5::st32(at + lane_off, o);
-                            };
-                            if (__any_sync(0xffffffffu, had)) {
-                                // O is complete: the P V of the step before was issued before these scores.  The P of this step's
-                                // first page is rescaled as the bfloat16 it is (rounded once more, where a maximum grows by 2^8)
-                                if (i > 0)
+                            if (i > 0 && __any_sync(0xffffffffu, had)) {
+                                // P V of the page before must be complete before O is rescaled (that of this page waits for
+                                // this warp's p_ready, that of two pages ago came before these scores: the phase is the one meant)
+                                if (!(ok = wait(pv_done, (uint32_t)((j - 1) & 1), 78))) break;
+                                tc5::fence_after();
 #pragma unroll 1
-                                    for (int c0 = 0; c0 < (EXACT ? DV : dv); c0 += 32) rescale(O_t + (uint32_t)c0, false);
-                                if (g > 0) rescale(S_t, true);
+                                for (int c0 = 0; c0 < (EXACT ? DV : dv); c0 += 32) {
+                                    uint32_t o[32];
+                                    tc5::ld32(O_t + lane_off + c0, o);
+                                    tc5::wait_ld();
+#pragma unroll
+                                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+                                    tc5::st32(O_t + lane_off + c0, o);
+                                }
                                 tc5::wait_st();
                             }
                         }
                         lpage = exponentials();
                     }
                     l += lpage;
-                    // P over this thread's own row of scores it has read: the first page's takes half the columns of the first page's
-                    // scores, the second's the other half
-                    tc5::st32(S_t + lane_off + (uint32_t)(g * 32), pk);
+                    // P over this thread's own row of the scores it has read: nothing else uses this buffer now (the P V of
+                    // two pages ago was issued before these scores, and the tensor core works in order)
+                    tc5::st32(S_t + lane_off + (uint32_t)(s * 64), pk);
                     tc5::wait_st();
                 }
                 tc5::fence_before();
                 __syncwarp();
-                if (lane == 0) tma::mbar_arrive(p_ready);
+                if (lane == 0) tma::mbar_arrive(&p_ready[s]);
             }
-            // the last P V, then the part
+            // The last P V (on a barrier of its own: by pv_done's parity, two phases not yet complete would look like the last one
+            // being so), then the part
             if (!ok || !(ok = wait(o_done, (uint32_t)(pieces & 1), 79))) break;
             tc5::fence_after();
             if (!idle) {
@@ -646,6 +604,7 @@ __global__ void __launch_bounds__(256, 2) shared_own_kernel(const __grid_constan
         *reinterpret_cast<float4*>(args.part_o + to * dv + c) = acc;
         if (c == 0) args.part_ml[to] = make_float2(M, L);
     }
+    pdl_launch();
     pdl_wait();                                     // (its end is the prefix kernel's end, too, for the kernel after it)
 }
 
@@ -688,7 +647,7 @@ __global__ void __launch_bounds__(JOIN_HALVES * 16) shared_join_kernel(bf16* __r
                 ml[k] = make_float2(-INFINITY, 0.f);
                 a[k] = b[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (i < n) {
-                    const size_t own = (size_t)args.own_row + (size_t)row * args.shares + (i - at.y), part = (size_t)at.x + (size_t)i * at.w;
+                    const size_t own = (size_t)args.own_row + (size_t)row * args.shares + (i - at.y), part = (size_t)at.x + (size_t)i * ROWS;
                     ml[k] = args.part_ml[i < at.y ? part + r : own];
                     const float4* src = reinterpret_cast<const float4*>(args.part_o + (i < at.y ? part * dv + ((size_t)lane * at.w + r) * 8 : own * dv + c));
                     if (c < dv) { a[k] = src[0]; b[k] = src[1]; }
@@ -737,7 +696,7 @@ int launch_shared(const CUtensorMap& tk, const CUtensorMap& tv, int ntok, const 
 }  // namespace
 
 // Decode attention (see gg_attn_decode_tma) of a step with shared prefixes: plan as at SharedArgs; runs (1 to 296): CTAs over
-// the prefixes; shares (1 to 64): CTAs that share a row's own pages; part: scratch of (nq ntok (2 + shares) + 128 runs) (dv + 2) + 4 ntok nkv floats, on a 32-byte boundary.
+// the prefixes; shares (1 to 64): CTAs that share a row's own pages; part: scratch of (nq ntok (1 + shares) + 128 runs) (dv + 2) + 4 ntok nkv floats, on a 32-byte boundary.
 // status: codes 71-79 (prefixes), 11 and 12 (own pages) name the wait that ran out.
 GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_pool, void* out, const int* positions,
                              const int* seq_of_token, const int* page_table, int max_pages, int page_size, int n_pages, const int* plan,
@@ -749,7 +708,7 @@ GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_po
         return GG_ERR_ARG;
     if ((((uintptr_t)q) & 15) || (((uintptr_t)k_pool) & 15) || (((uintptr_t)v_pool) & 15) || (((uintptr_t)out) & 15) || (((uintptr_t)part) & 31))
         return GG_ERR_ARG;
-    const long long prefix_rows = 2ll * nq * ntok + (long long)ROWS * runs, rows = prefix_rows + (long long)nq * ntok * shares;
+    const long long prefix_rows = (long long)nq * ntok + (long long)ROWS * runs, rows = prefix_rows + (long long)nq * ntok * shares;
     if (part == nullptr || part_floats < rows * (dv + 2) + 4ll * ntok * nkv || rows > 0x7fffffffll) return GG_ERR_ARG;
     // (units, blocks and the rows of the pools are counted in 32 bits: a row lists at most max_pages pages)
     const unsigned long long pool_rows = (unsigned long long)n_pages * nkv * PAGE;

@@ -73,10 +73,15 @@ def shared_shares(n_tokens: int, nkv: int, own_pages: int) -> int:
     return max(1, min(296 // (n_tokens * nkv), own_pages // 2, SHARED_SHARES))
 
 
-def prefix_pays(groups: Sequence[Tuple[int, int]], nkv: int, d: int, dv: int) -> bool:
-    """Is reading the prefixes of groups of (members, pages) once worth the kernels more that it takes?  Saved is what all members
-    but one of each group would read."""
-    return sum((members - 1) * pages for members, pages in groups) * nkv * (d + dv) >= 1 << 19
+def prefix_pays(groups: Sequence[Tuple[int, int]], n_tokens: int, nkv: int) -> bool:
+    """Is reading the prefixes of groups of (members, pages) once, in a step of n_tokens rows, quicker than every row for itself?  From
+    16 pages of prefixes on that a CTA of the unshared kernel would read (measured, us, unshared / shared, 32 heads of 128 on 8 kv
+    heads: 2 rows, 8 pages a CTA 10 / 13, 16 15 / 15, 32 27 / 21; 8 rows, 8 10.5 / 12.2, 16 15.9 / 14.4; 32 rows, 16 16 / 20, 32 27 /
+    21; 16 heads of 64: 16 rows, 8 8.6 / 9.4, 16 14 / 10)."""
+    pairs, splits = n_tokens * nkv, 1
+    while splits * 2 <= min(8, 296 // pairs):
+        splits *= 2
+    return sum(members * pages for members, pages in groups) * nkv >= 16 * min(296, pairs * splits)
 
 
 def shared_runs(groups: Sequence[Tuple[int, int]], nq: int, nkv: int) -> int:
@@ -131,7 +136,7 @@ class PrefixPlan:
         self.n_tokens = n_tokens
         self.words = host.to(device)
         self.own_pages = own_pages
-        self.groups = [(len(rows), int(pages)) for rows, pages in groups]
+        self.groups: Optional[List[Tuple[int, int]]] = [(len(rows), int(pages)) for rows, pages in groups]
 
     @staticmethod
     def words_for(n_tokens: int) -> int:
@@ -139,13 +144,14 @@ class PrefixPlan:
 
     @classmethod
     def over(cls, words: torch.Tensor, n_tokens: int, own_pages: Optional[int] = None,
-             groups: Sequence[Tuple[int, int]] = ()) -> "PrefixPlan":
+             groups: Optional[Sequence[Tuple[int, int]]] = None) -> "PrefixPlan":
         """A plan whose words are (or will be) on the device already, packed by `pack`; `groups`: (members, pages) of those it will
         hold, which choose the launch (any others are right, too)."""
         plan = cls.__new__(cls)
         if words.dtype != torch.int32 or words.numel() != cls.words_for(n_tokens) or not words.is_contiguous():
             raise KernelError(f"shared attention: a plan of {n_tokens} tokens has {cls.words_for(n_tokens)} int32 words")
-        plan.n_tokens, plan.words, plan.own_pages, plan.groups = n_tokens, words, own_pages, list(groups)
+        plan.n_tokens, plan.words, plan.own_pages, plan.groups = (
+            n_tokens, words, own_pages, None if groups is None else list(groups))
         return plan
 
     @classmethod
@@ -197,11 +203,13 @@ class PrefixPlan:
 
 
 def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, page_size, plan: PrefixPlan, scratch, nq, nkv, d, scale,
-                       sink=None, out_scale: float = 1.0, dv: Optional[int] = None, gate=None, runs: Optional[int] = None, shares: Optional[int] = None) -> None:
+                       sink=None, out_scale: float = 1.0, dv: Optional[int] = None, gate=None, together: Optional[bool] = None, runs: Optional[int] = None,
+                       shares: Optional[int] = None) -> None:
     """Decode attention (`attn_decode_tma`, without windows and chunks) of the plan's token rows: the keys and values of a prefix
-    that several rows share are read once for all of them, in three kernels.  scratch: float32, `shared_scratch` of it; two launches
-    that may run at the same time need scratch of their own.  runs: CTAs over the prefixes (default:
-    `shared_runs`); shares: CTAs that share a row's own pages (default: `shared_shares`)."""
+    that several rows share are read once for all of them, in three kernels, where that pays (`prefix_pays`; `together` True or
+    False decides instead).  scratch: float32, `shared_scratch` of it; two launches that may run at the same time need scratch of
+    their own.  runs: CTAs over the prefixes (default: `shared_runs`); shares: CTAs that share a row's own pages (default:
+    `shared_shares`)."""
     from .tcgen05_gemm import status_word
     dv = d if dv is None else int(dv)
     T = plan.n_tokens
@@ -233,6 +241,17 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
                 or gate.get_device() != here):
             raise KernelError(f"shared attention: a gate is bfloat16 with {T} rows of {nq * dv}, on the current CUDA device")
         p_gate, ldg = gate.data_ptr(), gate.stride(0)
+    if together is None:
+        together = plan.groups is None or prefix_pays(plan.groups, T, nkv)
+    if not together:
+        if page_size != 64:
+            raise KernelError(f"shared attention: pages of 64 positions, not {page_size}")
+        splits = decode_tma_splits(T, nkv, table.shape[1] * page_size, cluster=True)
+        if not (d == dv and d in (64, 128)):
+            splits = min(splits, 8)
+        attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page_size, T, nq, nkv, d, scale, 0, splits, cluster=True,
+                        sink=sink, out_scale=out_scale, dv=dv, gate=gate)
+        return
     if shares is None:
         shares = shared_shares(T, nkv, table.shape[1] if plan.own_pages is None else plan.own_pages)
     elif not 1 <= shares <= SHARED_SHARES:
@@ -241,7 +260,7 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
     if scratch.numel() < room:
         raise KernelError(f"shared attention: scratch must have {room} elements")
     if runs is None:
-        runs = shared_runs(plan.groups, nq, nkv)
+        runs = shared_runs(plan.groups or (), nq, nkv)
     elif not 1 <= runs <= SHARED_RUNS:
         raise KernelError(f"shared attention: 1 to {SHARED_RUNS} runs, not {runs}")
     kernel("attention_shared", "gg_attn_decode_shared")(

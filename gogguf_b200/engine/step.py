@@ -201,7 +201,7 @@ class Stepper:
                 known = self._found[st.index] = (st.sharing, list(slots), shared_groups(rows, [n // st.page_size for n in starts]))
             groups = known[2]
             rq = st.request
-            if groups and prefix_pays([(len(r), pages) for r, pages in groups], rq.num_kv_heads, rq.head_dim, rq.value_dim or rq.head_dim):
+            if groups and prefix_pays([(len(r), pages) for r, pages in groups], len(slots), rq.num_kv_heads):
                 found[st.index] = groups
                 have = [n // st.page_size + 1 for n in starts]
                 for r, pages in groups:

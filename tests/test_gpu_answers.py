@@ -22,7 +22,7 @@ def engine(tmp_path_factory, name, dtype="bfloat16", **kw):
 def always_shares(monkeypatch):
     """Prefixes are read together whatever it saves (the models here are small)."""
     from gogguf_b200.csrc import fast_attention as A
-    monkeypatch.setattr(A, "prefix_pays", lambda groups, nkv, d, dv: True)
+    monkeypatch.setattr(A, "prefix_pays", lambda groups, n_tokens, nkv: True)
 
 
 def counted(monkeypatch):

@@ -83,7 +83,7 @@ class Setup:
             plan = A.PrefixPlan.of_pages(self.lists, self.lengths, PAGE, "cuda")
         if scratch is None:
             scratch = torch.full((A.shared_scratch(self.T, self.nq, self.nkv, self.dv, kw.get("shares")),), math.nan, device="cuda")
-        kw = {"sink": self.sink, "gate": self.gate, "dv": self.dv, **kw}
+        kw = {"sink": self.sink, "gate": self.gate, "dv": self.dv, "together": True, **kw}
         A.attn_decode_shared(self.q, self.k, self.v, self.out, self.positions, self.rows, self.table, PAGE, plan, scratch, self.nq,
                              self.nkv, self.d, self.scale, **kw)
         from gogguf_b200.csrc.tcgen05_gemm import check_status
@@ -139,6 +139,17 @@ def test_rows_that_share_nothing():
     check(s.run(plan=A.PrefixPlan([], 37, "cuda")), *s.want())
 
 
+@pytest.mark.parametrize("kw", [dict(groups=[3, 1], prefix=[2, 4], own=(1, 100), nq=8, nkv=2, d=72, dv=40), dict(groups=[2], prefix=[90], own=(1, 9), nq=4, nkv=2, d=64)])
+def test_apart_where_that_is_quicker(kw):
+    from gogguf_b200.csrc import fast_attention as A
+    s = Setup(**kw)
+    pays = A.prefix_pays([(n, p) for n, p in zip(kw["groups"], kw["prefix"]) if n > 1], s.T, s.nkv)
+    for together in (None, False, True):
+        check(s.run(together=together), *s.want())
+    got = s.run(together=None).clone()
+    assert torch.equal(got, s.run(together=pays))
+
+
 def test_padding_rows_and_two_tokens_of_a_sequence():
     """A padded batch (rows without a sequence), and two tokens of one sequence as two members of a group."""
     from gogguf_b200.csrc import fast_attention as A
@@ -167,7 +178,7 @@ def test_captured_with_plans_that_change():
     s.run(plan=plan, scratch=scratch)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        A.attn_decode_shared(s.q, s.k, s.v, s.out, s.positions, s.rows, s.table, PAGE, plan, scratch, 8, 2, 128, s.scale)
+        A.attn_decode_shared(s.q, s.k, s.v, s.out, s.positions, s.rows, s.table, PAGE, plan, scratch, 8, 2, 128, s.scale, together=True)
     members = [r for r in range(s.T) if s.lists[r][0] == s.lists[0][0]]
     for other in (full, A.PrefixPlan([], s.T, "cuda"), A.PrefixPlan([(members, 3)], s.T, "cuda"), full):
         words.copy_(other.words)

@@ -89,6 +89,13 @@ def test_own_pages_and_their_shares():
     assert A.shared_shares(4000, 8, 100) == 1
 
 
+def test_when_a_prefix_pays_and_in_how_many_runs():
+    assert not A.prefix_pays([], 4, 8) and not A.prefix_pays([(2, 60)], 2, 8) and A.prefix_pays([(2, 130)], 2, 8)
+    assert not A.prefix_pays([(8, 32)], 8, 8) and A.prefix_pays([(8, 64)], 8, 8) and A.prefix_pays([(64, 32)], 64, 8)
+    assert A.prefix_pays([(300, 20)], 300, 8) and not A.prefix_pays([(2, 20)], 300, 8)
+    assert A.shared_runs([(64, 32)], 32, 8) == 148 and A.shared_runs([(64, 512)], 32, 8) == 296 and A.shared_runs([], 32, 8) == 148
+
+
 @pytest.mark.parametrize("groups, n", [([([0, 5], 2)], 5), ([([-1, 2], 2)], 5), ([([1, 1], 2)], 5), ([([0, 1], 2), ([1, 2], 2)], 5),
                                        ([([], 3)], 5), ([([0, 1], 0)], 5), ([], 0)])
 def test_plan_refuses(groups, n):
