@@ -2,6 +2,7 @@
 decode kernel (every sequence brings one token) and the prefill kernel, scratch for the splits."""
 from __future__ import annotations
 
+import functools
 from typing import Callable, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -9,6 +10,7 @@ import torch
 
 from . import kernels as K
 from .build import KernelError, kernel, module, stream_ptr
+from .tcgen05_gemm import status_word
 
 
 def decode_splits(n_tokens: int, nkv: int, max_ctx: int) -> int:
@@ -21,7 +23,6 @@ def _gate(gate):
 
 def attn_decode(q, k_pool, v_pool, out, positions, seq_of_token, table, page_size, n_tokens, nq, nkv, d,
                 scale, window, splits, part_o=None, part_ml=None) -> None:
-    from .tcgen05_gemm import status_word
     kernel("attention_fast", "gg_attn_decode")(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(),
         part_o.data_ptr() if part_o is not None else 0, part_ml.data_ptr() if part_ml is not None else 0,
@@ -30,6 +31,7 @@ def attn_decode(q, k_pool, v_pool, out, positions, seq_of_token, table, page_siz
         status_word(q.device).data_ptr(), stream_ptr())
 
 
+@functools.lru_cache(maxsize=4096)
 def decode_tma_splits(n_tokens: int, nkv: int, max_ctx: int, cluster: bool = False) -> int:
     return int(module("attention_fast").lib.gg_attn_decode_tma_splits(int(n_tokens), int(nkv), int(max_ctx),
                                                                       int(bool(cluster))))
@@ -43,7 +45,6 @@ def attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page
     sink: float32 per query head, joins the softmax's denominator; out_scale: a factor on the result (neither is
     taken by the form that merges its splits with a second kernel).  dv: the values' head size (default d); chunk: a
     position sees its own chunk of that many positions only; gate (rows of nq * dv logits): multiplied in by its sigmoid."""
-    from .tcgen05_gemm import status_word
     kernel("attention_fast", "gg_attn_decode_tma")(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(),
         part_o.data_ptr() if part_o is not None else 0, part_ml.data_ptr() if part_ml is not None else 0,
@@ -138,6 +139,14 @@ class PrefixPlan:
         self.own_pages = own_pages
         self.groups: Optional[List[Tuple[int, int]]] = [(len(rows), int(pages)) for rows, pages in groups]
 
+    def pays(self, nkv: int) -> bool:
+        """`prefix_pays` of this plan's groups (True where they are not known), worked out once."""
+        if self._pays[0] != nkv:
+            self._pays = (nkv, self.groups is None or prefix_pays(self.groups, self.n_tokens, nkv))
+        return self._pays[1]
+
+    _pays = (0, True)             # kv heads, and the answer for them
+
     @staticmethod
     def words_for(n_tokens: int) -> int:
         return 5 + 7 * n_tokens
@@ -210,39 +219,34 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
     False decides instead).  scratch: float32, `shared_scratch` of it; two launches that may run at the same time need scratch of
     their own.  runs: CTAs over the prefixes (default: `shared_runs`); shares: CTAs that share a row's own pages (default:
     `shared_shares`)."""
-    from .tcgen05_gemm import status_word
     dv = d if dv is None else int(dv)
     T = plan.n_tokens
     if not takes(nq, nkv, d, dv):
         raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {d} and {dv} are outside what the kernels take")
+    bf16, i32, words = torch.bfloat16, torch.int32, plan.words
     here = torch._C._cuda_getDevice() if q.is_cuda else -1
-
-    def need(t, dt, what):
-        if t.dtype != dt or not t.is_contiguous():
-            raise KernelError(f"shared attention: {what} must be contiguous {dt}, got {t.dtype}")
-        if here < 0 or t.get_device() != here:
-            raise KernelError(f"shared attention: {what} is on {t.device}, not on the current CUDA device")
-        return t.data_ptr()
-
-    bf16, i32 = torch.bfloat16, torch.int32
-    p_q, p_k, p_v, p_out = need(q, bf16, "q"), need(k_pool, bf16, "k_pool"), need(v_pool, bf16, "v_pool"), need(out, bf16, "out")
-    p_pos, p_seq, p_table = need(positions, i32, "positions"), need(seq_of_token, i32, "seq_of_token"), need(table, i32, "table")
-    p_plan, p_scratch = need(plan.words, i32, "plan"), need(scratch, torch.float32, "scratch")
+    for t, dt in ((q, bf16), (k_pool, bf16), (v_pool, bf16), (out, bf16), (positions, i32), (seq_of_token, i32), (table, i32), (words, i32),
+                  (scratch, torch.float32)) + (() if sink is None else ((sink, torch.float32),)):
+        if t.dtype is not dt or t.get_device() != here or here < 0 or not t.is_contiguous():
+            raise KernelError("shared attention: q, the pools and out are bfloat16, positions, seq_of_token, the table and the plan int32, "
+                              "scratch and a sink float32, all contiguous and on the current CUDA device: got "
+                              f"{t.dtype} of {tuple(t.shape)} with strides {t.stride()} on {t.device}")
+    pools = k_pool.shape[0]
     if (q.numel() < T * nq * d or out.numel() < T * nq * dv or positions.numel() < T or seq_of_token.numel() < T or table.dim() != 2
-            or k_pool.shape != (k_pool.shape[0], nkv, page_size, d) or v_pool.shape != (k_pool.shape[0], nkv, page_size, dv)):
+            or k_pool.shape != (pools, nkv, page_size, d) or v_pool.shape != (pools, nkv, page_size, dv)):
         raise KernelError("shared attention: shapes disagree")
     p_sink = p_gate = ldg = 0
     if sink is not None:
-        p_sink = need(sink, torch.float32, "sink")
         if sink.numel() != nq:
             raise KernelError(f"shared attention: a sink has {nq} elements")
+        p_sink = sink.data_ptr()
     if gate is not None:
         if (gate.dtype != bf16 or gate.dim() != 2 or gate.shape[0] < T or gate.shape[1] < nq * dv or gate.stride(1) != 1
                 or gate.get_device() != here):
             raise KernelError(f"shared attention: a gate is bfloat16 with {T} rows of {nq * dv}, on the current CUDA device")
         p_gate, ldg = gate.data_ptr(), gate.stride(0)
     if together is None:
-        together = plan.groups is None or prefix_pays(plan.groups, T, nkv)
+        together = plan.pays(nkv)
     if not together:
         if page_size != 64:
             raise KernelError(f"shared attention: pages of 64 positions, not {page_size}")
@@ -264,14 +268,14 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
     elif not 1 <= runs <= SHARED_RUNS:
         raise KernelError(f"shared attention: 1 to {SHARED_RUNS} runs, not {runs}")
     kernel("attention_shared", "gg_attn_decode_shared")(
-        p_q, p_k, p_v, p_out, p_pos, p_seq, p_table, table.shape[1], page_size, k_pool.shape[0], p_plan, T, nq, nkv, d, dv, float(scale),
-        int(runs), int(shares), p_sink, float(out_scale), p_gate, ldg, p_scratch, scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
+        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), table.data_ptr(),
+        table.shape[1], page_size, pools, words.data_ptr(), T, nq, nkv, d, dv, float(scale), int(runs), int(shares), p_sink, float(out_scale),
+        p_gate, ldg, scratch.data_ptr(), scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
 
 
 def attn_prefill(q, k_pool, v_pool, out, cu_seqlens, ctx_lens, seq_of_token, table, page_size, n_seqs,
                  max_tiles, nq, nkv, d, scale, window, sink=None, out_scale: float = 1.0, dv: Optional[int] = None,
                  chunk: int = 0, gate=None) -> None:
-    from .tcgen05_gemm import status_word
     kernel("attention_fast", "gg_attn_prefill")(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(),
         ctx_lens.data_ptr(), seq_of_token.data_ptr(), table.data_ptr(), table.shape[-1], page_size,
@@ -284,7 +288,6 @@ def attn_prefill_tc(q, k_pool, v_pool, out, cu_seqlens, ctx_lens, seq_of_token, 
                     n_seqs, max_tiles, nq, nkv, d, scale, window, sink=None, out_scale: float = 1.0,
                     dv: Optional[int] = None, chunk: int = 0, gate=None, splits: int = 1) -> None:
     """Prefill attention on tcgen05: 128-query tiles, S and O in tensor memory; the pages of a tile shared by `splits` CTAs."""
-    from .tcgen05_gemm import status_word
     kernel("attention_fast", "gg_attn_prefill_tc")(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(),
         ctx_lens.data_ptr(), seq_of_token.data_ptr(), table.data_ptr(), table.shape[-1], page_size,
@@ -324,6 +327,7 @@ def prefill_splits(n_tokens: int, n_seqs: int, nq: int, reach: int, max_new: Opt
     return best
 
 
+@functools.lru_cache(maxsize=4096)
 def takes(nq: int, nkv: int, d: int, dv: int) -> bool:
     """Do the tensor-core kernels take these sizes?  Head sizes in multiples of 8 up to 128, at most 16 query heads per kv
     head."""

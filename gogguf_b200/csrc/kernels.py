@@ -1440,7 +1440,7 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, hi
     here = torch._C._cuda_getDevice() if logits.is_cuda else -1
 
     def need(t, dt, what):
-        if t.dtype != dt or not t.is_contiguous() or t.get_device() != here:
+        if t.dtype is not dt or t.get_device() != here or not t.is_contiguous():
             raise KernelError(f"shape_logits: {what} must be contiguous {dt} on the logits' device, got {t.dtype} on {t.device}")
         return t.data_ptr()
 
