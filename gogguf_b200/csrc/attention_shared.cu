@@ -16,6 +16,16 @@
 // step without prefixes does it (attention_fast.cu).  (As rows of the prefix's product, a page of a member's own took the tensor
 // core as long as one of the prefix: 64 rows with up to 500 positions of their own on 2,048 were 44 us.  As CTAs of the prefix's
 // kernel they ran one an SM: a CTA of a kernel that allocates tensor memory keeps others of it off its SM until it has done so.)
+//
+// What bounds it.  64 rows of 32 heads (8 kv heads of 128) on 512 pages, with up to 200 positions of their own: 64 us (each row by
+// itself 700), of which the prefix kernel takes 45 (a page and tile 1.4 us of a CTA, two CTAs an SM, 268 MB through L2 at 6.7 TB/s, in which
+// its products alone would take half), the rows' own pages behind it 6 more, the parts 5.  On 32 pages, with up to 500 positions of their
+// own, 31 us (61): the own pages' 74 MB in 20 us, for most rows have four pages or five and a CTA's beginning and end are worth three; 12 of
+// the 20 share the SMs with the prefix kernel.
+// Tried and slower (us, of 64 rows on 32 and 512 pages, before the rows' CTAs left early: 33 and 67): runs in clusters of eight that add
+// up their parts in shared memory 40 and 62 (but 17 of 8 rows where this is 13), rows' own pages as rows of the product 74 and 168 or
+// in the line of pages 44 and 73, own pages as CTAs of the prefix kernel 36 and 64 (24 and 30 of ragged prompts where this was 19 and
+// 20), 128 keys a step 34 and 70, 256 rows a tile 44 and 73, eight warps for the softmax 37 and 69.
 #include "attention_common.cuh"
 
 namespace {
@@ -40,14 +50,15 @@ struct SharedArgs {
     int4* where;                      // [token row][kv head]: first row of its prefix's first part, how many parts there are, the
                                       // place of its rows in them, and a part's rows
     int own_row;                      // the first row behind the prefixes' parts
+    int max_pages;                    // of a row of the page table: a plan of more is read as one of so many
 };
 
 struct SharedPlan {
     const int *count, *first, *pages, *lead, *rows, *pages_of, *group_of, *member_of;
-    int cap;
+    int cap, max_pages;
     __device__ __forceinline__ SharedPlan(const SharedArgs& a)
         : count(a.plan), first(a.plan + 4), pages(first + a.cap + 1), lead(pages + a.cap), rows(lead + a.cap), pages_of(rows + a.cap),
-          group_of(pages_of + a.cap), member_of(group_of + a.cap), cap(a.cap) {}
+          group_of(pages_of + a.cap), member_of(group_of + a.cap), cap(a.cap), max_pages(a.max_pages) {}
     static __device__ __forceinline__ int tiles(int members, int G) {
         const int most = ROWS / G;
         return (members + most - 1) / most;
@@ -62,6 +73,12 @@ struct SharedPlan {
 
     // All units, and the group that unit u is of (u < 0: group `which`), by a whole warp: a lane a group.
     struct Group { int before, pages, first, members, lead; };
+    // the first of a group's sequences (rows that only fill up a step have none; the others of the group do not need them)
+    __device__ __forceinline__ int sequence(const int* seq_of_token, int lead_row, int at, int members) const {
+        int b = seq_of_token[lead_row];
+        for (int k = 1; b < 0 && k < members; ++k) b = seq_of_token[rows[at + k]];
+        return max(b, 0);
+    }
     __device__ __forceinline__ Group find(int u, int which, int nkv, int G, int lane, int& total) const {
         Group found = {};
         int groups = 1;
@@ -69,7 +86,7 @@ struct SharedPlan {
         for (int g0 = 0; g0 < groups; g0 += 32) {
             const int g = min(g0 + lane, cap - 1);
             // (asked for before the number of groups is known: beyond the last one stands something that is not used)
-            const int pg = pages[g], f = first[g], m = first[g + 1] - f, head = lead[g];
+            const int pg = min(pages[g], max_pages), f = first[g], m = first[g + 1] - f, head = lead[g];
             if (g0 == 0) groups = *count;
             const int units = g0 + lane < groups ? pg * tiles(m, G) * nkv : 0;
             int upto = units;
@@ -183,7 +200,7 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     if (!ok && threadIdx.x == 0) atomicCAS(status, 0, 29);
 
     // The run is cut where the (tile, kv head) changes.  Every role walks the same cuts.
-    struct Piece { int first, members, head, page0, pages, lead; size_t row0; };
+    struct Piece { int first, members, head, page0, pages, lead, all_first, all_members; size_t row0; };
     auto piece_at = [&](int u) -> Piece {
         int all;
         const SharedPlan::Group g = plan.find(u, -1, nkv, G, lane, all);
@@ -196,6 +213,8 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
         r.first = g.first + tile * tm;
         r.members = min(tm, g.members - tile * tm);
         r.lead = g.lead;
+        r.all_first = g.first;
+        r.all_members = g.members;
         r.row0 = (size_t)nkv * G * r.first + (size_t)r.head * G * r.members + (size_t)run * ROWS;
         return r;
     };
@@ -213,7 +232,7 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
             const Piece r = piece_at(u);
             u += r.pages;
             if (lane == 0 && ok) {
-                const int* pt = st.page_table + (size_t)st.seq_of_token[r.lead] * st.max_pages;
+                const int* pt = st.page_table + (size_t)plan.sequence(st.seq_of_token, r.lead, r.all_first, r.all_members) * st.max_pages;
                 for (int i = 0; i < r.pages; ++i, ++j) {
                     const int s = j & 1;
                     const uint32_t ph = (uint32_t)((j >> 1) & 1) ^ 1u;
@@ -426,8 +445,8 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
 
 // One share of the pages that only row `tok` reads, for the query heads of one kv head: four warps take 16 keys of every page
 // (fragments as in attention_fast.cu), their results are merged in shared memory.
-// This kernel starts when the prefix kernel's CTAs have all seen the kernel before them complete, and waits for the prefix kernel
-// only at its end: what it reads, q and the newest position among it, was there when it started.
+// This kernel starts when the prefix kernel's CTAs have all seen the kernel before them complete, and its last CTA alone waits for the
+// prefix kernel, at its end: what it reads, q and the newest position among it, was there when it started.
 template <int DK, int DV, bool EXACT>
 __global__ void __launch_bounds__(256, 2) shared_own_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                                 const SharedStep st, const SharedArgs args) {
@@ -605,7 +624,9 @@ __global__ void __launch_bounds__(256, 2) shared_own_kernel(const __grid_constan
         if (c == 0) args.part_ml[to] = make_float2(M, L);
     }
     pdl_launch();
-    pdl_wait();                                     // (its end is the prefix kernel's end, too, for the kernel after it)
+    // The end of this kernel is the prefix kernel's end, too, for the kernel after it: one CTA that waits for it is enough, and the
+    // others leave their place to those that have not begun.
+    if (blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 // Half a warp a row, eight columns a lane, or several (`team`, a power of two): its prefix's parts in the order of their runs, then its
@@ -722,7 +743,7 @@ GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_po
                            status};
     float* where = part + rows * dv;
     const SharedArgs args = {plan, ntok, runs, shares, part, reinterpret_cast<float2*>(where + 4ll * ntok * nkv), reinterpret_cast<int4*>(where),
-                             (int)prefix_rows};
+                             (int)prefix_rows, max_pages};
 #define GG_SHARED(DK_, DV_, EX_) launch_shared<DK_, DV_, EX_>(tk, tv, ntok, st, args, stream)
     if (d == 128 && dv == 128) rc = GG_SHARED(128, 128, true);
     else if (d == 64 && dv == 64) rc = GG_SHARED(64, 64, true);

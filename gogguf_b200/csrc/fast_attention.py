@@ -69,26 +69,28 @@ def shared_scratch(n_tokens: int, nq: int, nkv: int, dv: int, shares: Optional[i
 
 
 def shared_shares(n_tokens: int, nkv: int, own_pages: int) -> int:
-    """CTAs that share a row's own pages, of which the longest row has `own_pages`: what one wave of the device holds, and two pages
-    each at least."""
-    return max(1, min(296 // (n_tokens * nkv), own_pages // 2, SHARED_SHARES))
+    """CTAs that share a row's own pages, of which the longest row has `own_pages`: up to one and a half for each place on the device, and
+    two pages each at least (25 rows of 4 kv heads of 80, some of which have 37 pages of their own, 1 / 2 / 4 / 8 shares: 26 / 19.4 /
+    17.7 / 18.0 us; 64 rows of 8 kv heads, with up to 8 pages, 1 / 2 / 4: 31 / 33 / 39)."""
+    return max(1, min(444 // (n_tokens * nkv), own_pages // 2, SHARED_SHARES))
 
 
 def prefix_pays(groups: Sequence[Tuple[int, int]], n_tokens: int, nkv: int) -> bool:
     """Is reading the prefixes of groups of (members, pages) once, in a step of n_tokens rows, quicker than every row for itself?  From
-    16 pages of prefixes on that a CTA of the unshared kernel would read (measured, us, unshared / shared, 32 heads of 128 on 8 kv
-    heads: 2 rows, 8 pages a CTA 10 / 13, 16 15 / 15, 32 27 / 21; 8 rows, 8 10.5 / 12.2, 16 15.9 / 14.4; 32 rows, 16 16 / 20, 32 27 /
-    21; 16 heads of 64: 16 rows, 8 8.6 / 9.4, 16 14 / 10)."""
+    12 pages of prefixes on that a CTA of the unshared kernel would read (measured, us, unshared / shared with two pages of a row's own,
+    32 heads of 128 on 8 kv heads: 2 rows, 8 pages a CTA 10 / 13, 16 15.4 / 15.4, 32 26 / 21; 8 rows, 8 10.6 / 12.1, 16 15.9 / 14.8;
+    32 rows, 16 16 / 19, 32 27 / 20; 64 rows, 14 21 / 22, 27 31 / 23; 16 heads of 64: 8 rows, 8 8.6 / 9.9, 16 14.1 / 11.4; 24 heads of
+    80 on 4 kv heads: 16 rows, 8 11.1 / 12.0, 16 16.2 / 13.3)."""
     pairs, splits = n_tokens * nkv, 1
     while splits * 2 <= min(8, 296 // pairs):
         splits *= 2
-    return sum(members * pages for members, pages in groups) * nkv >= 16 * min(296, pairs * splits)
+    return sum(members * pages for members, pages in groups) * nkv >= 12 * min(296, pairs * splits)
 
 
 def shared_runs(groups: Sequence[Tuple[int, int]], nq: int, nkv: int) -> int:
     """CTAs over the prefixes of groups of (members, pages): one an SM, which leaves room for the CTAs of the rows' own pages beside
-    it, until a CTA has more than six pages (measured, us, one against two an SM: 64 rows of 32 heads on 32 pages 34 / 39; 12 rows of
-    32 heads on 2 kv heads, 256 pages 23 / 21; 64 rows on 512 pages 85 / 68)."""
+    it, until a CTA has more than six pages (measured, us, one against two an SM: 64 rows of 32 heads on 32 pages 31 / 38; 12 rows of
+    32 heads on 2 kv heads, 256 pages 23 / 21; 64 rows on 512 pages 74 / 64)."""
     most = SHARED_ROWS // (nq // nkv)
     units = sum(pages * -(-members // most) for members, pages in groups) * nkv
     return SHARED_RUNS // 2 if units <= 6 * (SHARED_RUNS // 2) else SHARED_RUNS
@@ -232,6 +234,8 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
                               "scratch and a sink float32, all contiguous and on the current CUDA device: got "
                               f"{t.dtype} of {tuple(t.shape)} with strides {t.stride()} on {t.device}")
     pools = k_pool.shape[0]
+    if plan.groups and max(pages for _, pages in plan.groups) > table.shape[-1]:
+        raise KernelError(f"shared attention: the plan's prefixes are longer than the table's {table.shape[-1]} pages")
     if (q.numel() < T * nq * d or out.numel() < T * nq * dv or positions.numel() < T or seq_of_token.numel() < T or table.dim() != 2
             or k_pool.shape != (pools, nkv, page_size, d) or v_pool.shape != (pools, nkv, page_size, dv)):
         raise KernelError("shared attention: shapes disagree")

@@ -185,7 +185,8 @@ __global__ void shape_advance_kernel(int* tokens, const int* __restrict__ ring_r
     int id = tokens[r];
     if (states != nullptr && states[ring] >= 0) {
         const int s = states[ring];
-        const int to = s < n_states && id >= 0 && id < V ? next[(size_t)s * n_classes + classes[id]] : -1;
+        const int c = id >= 0 && id < V ? classes[id] : -1;
+        const int to = s < n_states && c >= 0 && c < n_classes ? next[(size_t)s * n_classes + c] : -1;
         if (to < 0) tokens[r] = id = -1;
         else states[ring] = to;
     }

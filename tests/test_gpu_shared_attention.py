@@ -163,6 +163,53 @@ def test_padding_rows_and_two_tokens_of_a_sequence():
     got = s.run(plan=A.PrefixPlan([([2, 0], 4)], 3, "cuda"))
     check(got[[0, 2]], want[0][[0, 2]], want[1][[0, 2]])
     assert (got[1] == 0).all()                          # as the unshared kernel leaves padding
+    got = s.run(plan=A.PrefixPlan([([1, 2, 0], 4)], 3, "cuda"))
+    check(got[[0, 2]], want[0][[0, 2]], want[1][[0, 2]])      # a group whose first row is padding
+    assert (got[1] == 0).all()
+
+
+def test_a_plan_longer_than_the_table():
+    """Refused where the plan's pages are known; packed words that say so read no further than the table, and other rows are right."""
+    from gogguf_b200.csrc import fast_attention as A
+    from gogguf_b200.csrc.build import KernelError
+    s = Setup(groups=[2, 3], prefix=[4, 6], own=(5, 50), nq=8, nkv=2, d=64)
+    groups = [([0, 1], 9000), ([2, 3, 4], s.table.shape[1] + 1)]
+    with pytest.raises(KernelError, match="longer than the table"):
+        s.run(plan=A.PrefixPlan(groups, s.T, "cuda"))
+    words = A.PrefixPlan([([r for r in range(s.T) if s.lists[r][0] == s.lists[0][0]], 9000)], s.T, "cuda").words
+    other = [r for r in range(s.T) if s.lists[r][0] != s.lists[0][0]]
+    got = s.run(plan=A.PrefixPlan.over(words, s.T))
+    check(got[other], *(w[other] for w in s.want()))
+
+
+def test_calls_one_after_the_other_in_one_scratch():
+    """Six calls behind each other, of two steps in turn, in the same scratch, launched one by one and captured."""
+    from gogguf_b200.csrc import fast_attention as A
+    steps = [Setup(groups=[5, 3], prefix=[8, 40], own=(1, 100), nq=8, nkv=2, d=128, seed=1), Setup(groups=[7, 1], prefix=[19, 2], own=(1, 300), nq=8, nkv=2, d=128, seed=2)]
+    plans = [A.PrefixPlan.of_pages(s.lists, s.lengths, PAGE, "cuda") for s in steps]
+    scratch = torch.empty(A.shared_scratch(8, 8, 2, 128), device="cuda")
+    outs = [torch.full_like(steps[0].out, 7.0) for _ in range(6)]
+
+    def calls():
+        for i, out in enumerate(outs):
+            s = steps[i % 2]
+            A.attn_decode_shared(s.q, s.k, s.v, out, s.positions, s.rows, s.table, PAGE, plans[i % 2], scratch, 8, 2, 128, s.scale, together=True)
+
+    calls()
+    torch.cuda.synchronize()
+    first = [o.clone() for o in outs]
+    for i, out in enumerate(first):
+        check(out[:8], *steps[i % 2].want())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls()
+    for out in outs:
+        out.fill_(5.0)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for out, was in zip(outs, first):
+        assert torch.equal(out[:8], was[:8])
 
 
 def test_captured_with_plans_that_change():
