@@ -33,12 +33,12 @@ class GenerateParams:
     repeat_last_n: int = 64
     stop_token_ids: Optional[Sequence[int]] = None     # None: the model's own (eos_token_id)
     on_token: Optional[Callable[[int, int], bool]] = None   # (request index, token) -> go on?
+    keep_logits: bool = False      # results carry the float32 logits every sampled token was drawn from (host copies, as the model gave them)
     answers: int = 1               # results per prompt: answer a of prompt i is result i * answers + a, drawn as that request
     frequency_penalty: float = 0.0 # subtracted from a logit for every time its id stands among the last repeat_last_n
     presence_penalty: float = 0.0  # subtracted once from the logits of the ids that stand there
     logit_bias: Optional[Mapping[int, float]] = None   # id -> number added to its logit (-inf: never)
     grammar: Optional[TokenGrammar] = None             # the ids that an answer may go on with, from one id to the next
-    keep_logits: bool = False      # results carry the float32 logits every sampled token was drawn from (host copies)
 
 
 @dataclass
@@ -93,10 +93,10 @@ def plan_shared_batches(prompt_lens: Sequence[int], sources: Sequence[int], max_
         if n > context:
             raise ValueError(f"request {i}: prompt of {n} tokens exceeds the context of {context}")
         pages = -(-min(n + max(max_new, 0), context) // page_size)
-        alone = pages - min(prefix_tokens, n) // page_size
+        alone = max(1, pages - min(prefix_tokens, n) // page_size)          # (a slot for itself is counted as a page, too)
         if alone * page_size > capacity_tokens:
             raise ValueError(f"request {i}: needs room for {alone * page_size} tokens but the cache holds {capacity_tokens}")
-        need = pages - n // page_size if sources[i] in cur else alone
+        need = max(1, pages - n // page_size) if sources[i] in cur else alone
         if cur and (len(cur) >= max_batch or (used + need) * page_size > capacity_tokens):
             batches.append(cur)
             cur, used, need = [], 0, alone
@@ -420,7 +420,7 @@ class GenerationSession:
         if params.answers != 1:
             raise ValueError("a session gives one answer to each of its prompts")
         shaping = LogitShaping.of(params, self._gen.vocab_size)
-        key = (params.sampler, params.repeat_penalty, params.repeat_last_n, shaping.key() if shaping is not None else None)
+        key = (params.sampler, params.repeat_penalty, params.repeat_last_n, shaping)
         sampler = self._samplers.get(key)
         if sampler is None:
             sampler = self._samplers[key] = make_sampler(params.sampler, params.repeat_penalty, params.repeat_last_n,

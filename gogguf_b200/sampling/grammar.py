@@ -17,8 +17,9 @@ class TokenGrammar:
     class is not allowed; `start`: the state of a sequence that has made no id yet."""
 
     def __init__(self, classes: Sequence[int], next: Sequence[Sequence[int]], start: int = 0):
-        self.classes = np.ascontiguousarray(classes, dtype=np.int32)
-        self.next = np.ascontiguousarray(next, dtype=np.int32)
+        self.classes = np.array(classes, dtype=np.int32, order="C")          # (copies that nobody writes to: `on` keeps others)
+        self.next = np.array(next, dtype=np.int32, order="C")
+        self.classes.flags.writeable = self.next.flags.writeable = False
         self.start = int(start)
         if self.classes.ndim != 1 or self.classes.size == 0 or self.next.ndim != 2 or self.next.size == 0:
             raise ValueError("a grammar has a class per id and a row of classes per state")
@@ -107,5 +108,5 @@ class TokenGrammar:
         """(masks, classes, next) on a device, made at the first call."""
         device = torch.device(device)
         if device not in self._on:
-            self._on[device] = tuple(torch.from_numpy(np.ascontiguousarray(a)).to(device) for a in (self.masks(), self.classes, self.next))
+            self._on[device] = tuple(torch.from_numpy(np.array(a)).to(device) for a in (self.masks(), self.classes, self.next))
         return self._on[device]

@@ -203,6 +203,8 @@ class Sampler:
             return
         n, rows = self.repeat_last_n, len(streams)
         if self.shaped:
+            if not ShapingState.advances(self.shaping):
+                return
             self._state = ShapingState(self.shaping, prompts, [()] * rows, device)
             self._rings = ()
             self._ring_rows = self._ring_pairs(rows, device)

@@ -49,11 +49,10 @@ class LogitShaping:
         if frequency == 0 and presence == 0 and not bias and grammar is None:
             return None
         repeat = float(params.repeat_penalty)
+        if repeat == math.inf:
+            raise ValueError("repeat_penalty must be finite")
         return cls(repeat if repeat > 0 else 1.0, int(params.repeat_last_n) if params.repeat_last_n else 64, frequency, presence,
                    tuple(sorted(bias)), grammar)
-
-    def key(self):
-        return (self.repeat, self.last_n, self.frequency, self.presence, self.bias, id(self.grammar) if self.grammar is not None else None)
 
     @property
     def counts(self) -> bool:
@@ -86,9 +85,15 @@ def shape_host(row: np.ndarray, shaping: LogitShaping, history: Sequence[int], g
 class ShapingState:
     """The requests' last ids, biases and grammar states on the device."""
 
+    @staticmethod
+    def advances(shaping: LogitShaping) -> bool:
+        """Can a state follow the drawn ids on the device?  Not where the window has no end."""
+        return shaping.last_n > 0 or not shaping.counts
+
     def __init__(self, shaping: LogitShaping, histories: Sequence[Sequence[int]], generated: Sequence[Sequence[int]], device):
         self.shaping = shaping
-        rows, n = len(histories), shaping.last_n
+        # (a window below one is the whole history: as it is now, for states that are made for a step)
+        rows, n = len(histories), shaping.last_n if shaping.last_n > 0 else max([1] + [len(h) for h in histories])
         self.hist = self.hist_len = self.hist_pos = None
         if shaping.counts:
             hist = np.full((rows, n), -1, dtype=np.int32)

@@ -175,6 +175,22 @@ def test_a_step_ahead_of_the_host_draws_what_the_host_draws(tmp_path_factory, sa
             assert t == sample_host(row, cfg, uniform01(cfg.seed, i, k)), (i, k)
 
 
+def test_a_window_without_an_end(tmp_path_factory):
+    """repeat_last_n below zero: all of prompt and answer count, step by step."""
+    import gogguf_b200 as gg
+    from gogguf_b200.sampling import LogitShaping
+    eng = engine(tmp_path_factory, "L", "float32")
+    ctx = eng.new_context()
+    prompts = [random_tokens(eng.model.spec.vocab_size, n, n) for n in (80, 2)]
+    kw = dict(max_tokens=9, stop_token_ids=[], repeat_penalty=1.2, repeat_last_n=-1, frequency_penalty=2.0, logit_bias={4: 1.0})
+    shaping = LogitShaping.of(gg.GenerateParams(**kw), eng.model.spec.vocab_size)
+    out = ctx.generate(prompts, gg.GenerateParams(keep_logits=True, **kw))
+    for p, r in zip(prompts, out):
+        for k, t in enumerate(r.tokens):
+            assert t == int(follow(r.logits[k], shaping, list(p) + r.tokens[:k], r.tokens[:k]).argmax())
+    assert [r.tokens for r in ctx.generate(prompts, gg.GenerateParams(**kw))] == [r.tokens for r in out]
+
+
 def test_an_answer_that_the_grammar_ends(tmp_path_factory):
     """A state in which nothing is allowed ends that answer, in the loop that is a step ahead and in the one that is not; the others go on."""
     import gogguf_b200 as gg

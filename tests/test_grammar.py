@@ -49,6 +49,15 @@ def test_refusals(bad):
         TokenGrammar(**bad)
 
 
+def test_a_grammar_does_not_change_with_what_it_was_made_from():
+    classes, rows = np.zeros(4, dtype=np.int32), np.zeros((1, 1), dtype=np.int32)
+    g = TokenGrammar(classes, rows)
+    classes[:], rows[:] = 1, -1
+    assert g.step(0, 3) == 0 and g.on("cpu")[1].tolist() == [0] * 4
+    with pytest.raises(ValueError):
+        g.next[0, 0] = -1
+
+
 def test_ids_outside_the_vocabulary_are_refused():
     with pytest.raises(ValueError):
         TokenGrammar.from_rows(10, [{10: 0}])

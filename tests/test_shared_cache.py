@@ -260,6 +260,23 @@ def test_answers_refusals():
         g.generate([[1]], GenerateParams(answers=2), held={0: slot})
 
 
+def test_answers_to_a_prompt_as_long_as_the_context():
+    """They add no page to the prompt's, and are planned in batches that the slots hold all the same."""
+    g = Generator(ScriptedStepper(max_tokens=64 * 4), V, 64)
+    res = g.generate([[1] * 64], GenerateParams(max_tokens=5, answers=11, stop_token_ids=[]))
+    assert [r.tokens for r in res] == [[2]] * 11 and g.cache.live_slots == 0
+    g.cache.check()
+
+
+def test_windows_without_an_end():
+    """repeat_last_n below zero is the whole history; a repeat penalty joins the others."""
+    run = lambda **kw: [r.tokens for r in Generator(ScriptedStepper(), V, 1000).generate([[7, 5, 1]], GenerateParams(max_tokens=4, stop_token_ids=[0], **kw))]
+    assert run(presence_penalty=9.0, logit_bias={9: 4.0}, repeat_last_n=-1) == [[2, 3, 4, 9]]
+    assert run(presence_penalty=9.0, logit_bias={9: 4.0}, repeat_last_n=2) == [[2, 3, 4, 5]]
+    with pytest.raises(ValueError):
+        run(presence_penalty=9.0, repeat_penalty=float("inf"))
+
+
 def test_penalties_biases_and_a_grammar_in_the_loop():
     run = lambda **kw: [r.tokens for r in Generator(ScriptedStepper(), V, 1000).generate([[1]], GenerateParams(max_tokens=4, stop_token_ids=[0], **kw))]
     assert run() == [[2, 3, 4, 5]]
