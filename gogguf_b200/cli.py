@@ -2,6 +2,7 @@
 
     gogguf_b200 run (-m DIR | --random CONFIG.json [--weights-seed 0]) -p "1 2 3" [-p "4 5"] [-n 128] [--temp 0]
                     [--top-k 0] [--top-p 1] [--min-p 0] [--repeat-penalty 1] [--repeat-last-n 64] [--seed 0]
+                    [--frequency-penalty 0] [--presence-penalty 0] [--logit-bias ID=VALUE ...] [--answers 1]
                     [--dtype bfloat16] [-i]
     gogguf_b200 info -m DIR
     gogguf_b200 inspect DIR
@@ -14,7 +15,8 @@
 `run` keeps the reference's option names and defaults (cmd/gogguf/run.go:17-34).  A prompt is a list
 of token ids (the tokenizer is outside this library); several -p make a batch.  Dropped: -hf
 (network), --chat/--thinking (text templates), -ngl (the whole model is always on the GPU).  -i is the
-reference's REPL on token ids: one conversation, a line of new ids per turn.
+reference's REPL on token ids: one conversation, a line of new ids per turn.  Beyond the reference:
+frequency and presence penalties, biases, and several answers to a prompt, which is run once for them.
 `info` prints what the reference's info prints (cmd/gogguf/info.go:27-44), `inspect` every
 configuration key and tensor (cmd/gogguf/inspect.go:13-41).  `random` is the random-weights mode.
 `dumplayers`, `comparelayers` and `layerlogits` are the reference's layer tools (cmd/tools/dumplayers.go,

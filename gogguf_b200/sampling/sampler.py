@@ -9,7 +9,9 @@ also has a kernel, which answers from each row's 1,024 largest logits and flags 
 that may not be the whole answer; the host reads the flags every step (so this configuration does not
 run a step ahead) and takes flagged rows, like everything with a penalty but no kernel path, through
 this module's host chain.  The order is
-the reference's: penalty, temperature, top-k, min-p, mask to -1e10, softmax, top-p, draw.
+the reference's: penalty, temperature, top-k, min-p, mask to -1e10, softmax, top-p, draw.  What the
+reference has not, frequency and presence penalties, biases and grammars (`shaping.py`), comes where the
+penalty does, with the repeat penalty in the same pass.
 
 Random draws are counter based: u = uniform01(seed, stream, step) with `stream` the request's index
 and `step` the number of tokens it has generated, so a sequence's draws do not depend on what else
