@@ -17,27 +17,37 @@
 // core as long as one of the prefix: 64 rows with up to 500 positions of their own on 2,048 were 44 us.  As CTAs of the prefix's
 // kernel they ran one an SM: a CTA of a kernel that allocates tensor memory keeps others of it off its SM until it has done so.)
 //
-// What bounds it.  64 rows of 32 heads (8 kv heads of 128) on 512 pages, with up to 200 positions of their own: 64 us (each row by
+// What bounds it.  64 rows of 32 heads (8 kv heads of 128) on 512 pages, with up to 200 positions of their own: 62 us (each row by
 // itself 700), of which the prefix kernel takes 45 (a page and tile 1.4 us of a CTA, two CTAs an SM, 268 MB through L2 at 6.7 TB/s, in which
 // its products alone would take half), the rows' own pages behind it 6 more, the parts 5.  On 32 pages, with up to 500 positions of their
-// own, 31 us (61): the own pages' 74 MB in 20 us, for most rows have four pages or five and a CTA's beginning and end are worth three; 12 of
-// the 20 share the SMs with the prefix kernel.
-// Tried and slower (us, of 64 rows on 32 and 512 pages, before the rows' CTAs left early: 33 and 67): runs in clusters of eight that add
-// up their parts in shared memory 40 and 62 (but 17 of 8 rows where this is 13), rows' own pages as rows of the product 74 and 168 or
-// in the line of pages 44 and 73, own pages as CTAs of the prefix kernel 36 and 64 (24 and 30 of ragged prompts where this was 19 and
-// 20), 128 keys a step 34 and 70, 256 rows a tile 44 and 73, eight warps for the softmax 37 and 69.
+// own, 28 us (61): the own pages' 74 MB in 17 us (a CTA's beginning and end are worth three of its pages, of which it has one to eight),
+// the prefix kernel beside them for the first 10, the parts 3.
+// Tried and slower (us, of 64 rows on 32 and 512 pages, when this was 33 and 67): runs in clusters of eight that add up their parts in
+// shared memory 40 and 62 (but 17 of 8 rows where this is 12), rows' own pages as rows of the product 74 and 168 or in the line of pages 44
+// and 73, own pages as CTAs of the prefix kernel 36 and 64 (24 and 30 of ragged prompts where this was 19 and 20), 128 keys a step 34
+// and 70, 256 rows a tile 44 and 73, eight warps for the softmax 37 and 69.
+#include <type_traits>
+
 #include "attention_common.cuh"
 
 namespace {
 
 constexpr int ROWS = 128;             // of a tile
-constexpr int THREADS = 192;
+constexpr int THREADS = 192;          // of the prefix kernel
+constexpr int OWN_THREADS = 128;      // of the kernel over rows' own pages
 constexpr int MAX_RUNS = 296;         // of the prefix kernel: two per SM
-constexpr int OWN_STAGES_BYTES = 96 * 1024;
+
+// Stages of the ring of a row's own pages: 64 KB of them in the form for eight query heads (three CTAs an SM; 96 KB and two: 29.7 us
+// where this is 27.9), 96 KB in that for sixteen, whose registers leave room for two.
+__host__ __device__ constexpr int own_stages(int stage_bytes, bool eight) {
+    const int n = (eight ? 64 : 96) * 1024 / stage_bytes;
+    return n < 4 ? n : 4;
+}
 
 // The plan, integers of a step, with room for `cap` token rows: how many groups; from word 4 on, per group the place of its first
 // member in `rows` (and one place beyond the last group's), its pages and its first member; `rows`, the members' token rows group
-// by group; per token row the pages that are its prefix (0: none), its group (-1: none) and its place among the group's members.
+// by group; per token row the pages that are its prefix (0: none), its group (-1: none) and its place among the group's members; the token rows in
+// the order in which their own pages are read, most pages first.
 // A group's members are cut into tiles of equal size; the units of work are the pages of (group, tile, kv head) in that order, and
 // run c takes `per` of them from c per on.  The part that run c leaves of a (tile, kv head) begins at row row0 + 128 c, with row0
 // the rows of all (tile, kv head)s before: later parts are later in c or in row0, and 128 is the most a part has, so no two
@@ -54,11 +64,11 @@ struct SharedArgs {
 };
 
 struct SharedPlan {
-    const int *count, *first, *pages, *lead, *rows, *pages_of, *group_of, *member_of;
+    const int *count, *first, *pages, *lead, *rows, *pages_of, *group_of, *member_of, *order;
     int cap, max_pages;
     __device__ __forceinline__ SharedPlan(const SharedArgs& a)
         : count(a.plan), first(a.plan + 4), pages(first + a.cap + 1), lead(pages + a.cap), rows(lead + a.cap), pages_of(rows + a.cap),
-          group_of(pages_of + a.cap), member_of(group_of + a.cap), cap(a.cap), max_pages(a.max_pages) {}
+          group_of(pages_of + a.cap), member_of(group_of + a.cap), order(member_of + a.cap), cap(a.cap), max_pages(a.max_pages) {}
     static __device__ __forceinline__ int tiles(int members, int G) {
         const int most = ROWS / G;
         return (members + most - 1) / most;
@@ -443,28 +453,189 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     }
 }
 
-// One share of the pages that only row `tok` reads, for the query heads of one kv head: four warps take 16 keys of every page
-// (fragments as in attention_fast.cu), their results are merged in shared memory.
+// What a warp holds of a row's own pages: the query heads, the sums so far, and what it does with its 16 keys of a page.  The maximum m is
+// in log2 units, l a lane's share of the sum until `finish`.
+//
+// Up to sixteen query heads are the rows of the products (fragments as in attention_fast.cu).
+template <int DK, int DV, bool EXACT>
+struct SixteenHeads {
+    static constexpr int KS = DK / 16, NT = DV / 8, BOX_BYTES = 64 * 64 * 2;
+    uint32_t qa[KS][4];
+    float o[NT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+    __device__ __forceinline__ void load(const bf16* q0, int G, int d, int g, int t) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = g + 8 * (e & 1), c = ks * 16 + 2 * t + 8 * (e >> 1);
+                qa[ks][e] = row < G && (EXACT || c < d) ? __ldcg(reinterpret_cast<const unsigned int*>(q0 + (size_t)row * d + c)) : 0u;
+            }
+    }
+    __device__ __forceinline__ void page(const uint8_t* k, const uint8_t* v, int krow, int key0, int pos, float scale_log2, int lane) {
+        const int t = lane & 3;
+        float sc[2][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const bf16* box = reinterpret_cast<const bf16*>(k + (ks >> 2) * BOX_BYTES);
+            uint32_t kb[4];
+            ldsm_x4(kb, sw<64>(const_cast<bf16*>(box), krow + (lane & 7) + ((lane >> 4) << 3), (ks & 3) * 2 + ((lane >> 3) & 1)));
+            mma16816(sc[0], qa[ks], kb[0], kb[1]);
+            mma16816(sc[1], qa[ks], kb[2], kb[3]);
+        }
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = key0 + j * 8 + 2 * t + (e & 1) <= pos ? sc[j][e] * scale_log2 : -INFINITY;
+                sc[j][e] = x;
+                mx[e >> 1] = fmaxf(mx[e >> 1], x);
+            }
+        uint32_t pa[4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+            const float mn = fmaxf(m[r], mx[r]);
+            const float mu = mn == -INFINITY ? 0.f : mn;
+            const float corr = fast_exp2(m[r] - mu);
+            m[r] = mn;
+            const float p00 = fast_exp2(sc[0][2 * r] - mu), p01 = fast_exp2(sc[0][2 * r + 1] - mu);
+            const float p10 = fast_exp2(sc[1][2 * r] - mu), p11 = fast_exp2(sc[1][2 * r + 1] - mu);
+            l[r] = l[r] * corr + (p00 + p01 + p10 + p11);
+            pa[r] = pack_bf16(p00, p01);
+            pa[2 + r] = pack_bf16(p10, p11);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) { o[n][2 * r] *= corr; o[n][2 * r + 1] *= corr; }
+        }
+#pragma unroll
+        for (int np = 0; np < NT / 2; ++np) {
+            const bf16* box = reinterpret_cast<const bf16*>(v + (np >> 2) * BOX_BYTES);
+            uint32_t vb[4];
+            ldsm_x4_trans(vb, sw<64>(const_cast<bf16*>(box), krow + (lane & 7) + (((lane >> 3) & 1) << 3), (np & 3) * 2 + (lane >> 4)));
+            mma16816(o[2 * np], pa, vb[0], vb[1]);
+            mma16816(o[2 * np + 1], pa, vb[2], vb[3]);
+        }
+    }
+    // a head's values into `row_of(head)`, its maximum and sum into `ml_of(head)`
+    template <typename Row, typename Ml>
+    __device__ __forceinline__ void finish(int G, int g, int t, Row row_of, Ml ml_of) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        }
+        // only the G rows that are query heads go on (the MMA tile has 16)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if (g + 8 * r >= G) continue;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(row_of(g + 8 * r) + n * 8 + 2 * t) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+            if (t == 0) *ml_of(g + 8 * r) = make_float2(m[r], l[r]);
+        }
+    }
+};
+
+// Up to eight are the columns instead, S^T = K Q^T and O^T = V^T P^T: half the products and half the registers for O, for P^T's way from
+// the rows of one product to those of the other (a transposition of 8 x 8 in registers).
+template <int DK, int DV, bool EXACT>
+struct EightHeads {
+    static constexpr int KS = DK / 16, NT = DV / 16, BOX_BYTES = 64 * 64 * 2;
+    uint32_t qb[KS][2];
+    float o[NT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};      // of heads 2 t and 2 t + 1
+    __device__ __forceinline__ void load(const bf16* q0, int G, int d, int g, int t) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = ks * 16 + 2 * t + 8 * e;
+                qb[ks][e] = g < G && (EXACT || c < d) ? __ldcg(reinterpret_cast<const unsigned int*>(q0 + (size_t)g * d + c)) : 0u;
+            }
+    }
+    static __device__ __forceinline__ uint32_t transposed(uint32_t x) {
+        uint32_t y;
+        asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+        return y;
+    }
+    __device__ __forceinline__ void page(const uint8_t* k, const uint8_t* v, int krow, int key0, int pos, float scale_log2, int lane) {
+        const int g = lane >> 2;
+        float sc[4] = {};                                  // keys g, g, g + 8, g + 8; heads 2 t, 2 t + 1, 2 t, 2 t + 1
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const bf16* box = reinterpret_cast<const bf16*>(k + (ks >> 2) * BOX_BYTES);
+            uint32_t ka[4];
+            ldsm_x4(ka, sw<64>(const_cast<bf16*>(box), krow + (lane & 7) + (((lane >> 3) & 1) << 3), (ks & 3) * 2 + (lane >> 4)));
+            mma16816(sc, ka, qb[ks][0], qb[ks][1]);
+        }
+        float p[4], corr[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float x0 = key0 + g <= pos ? sc[h] * scale_log2 : -INFINITY, x1 = key0 + g + 8 <= pos ? sc[2 + h] * scale_log2 : -INFINITY;
+            float mx = fmaxf(x0, x1);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float mn = fmaxf(m[h], mx), mu = mn == -INFINITY ? 0.f : mn;
+            corr[h] = fast_exp2(m[h] - mu);
+            m[h] = mn;
+            p[h] = fast_exp2(x0 - mu);
+            p[2 + h] = fast_exp2(x1 - mu);
+            l[h] = l[h] * corr[h] + (p[h] + p[2 + h]);
+        }
+        const uint32_t p0 = transposed(pack_bf16(p[0], p[1])), p1 = transposed(pack_bf16(p[2], p[3]));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const bf16* box = reinterpret_cast<const bf16*>(v + (n >> 2) * BOX_BYTES);
+            uint32_t va[4];
+            ldsm_x4_trans(va, sw<64>(const_cast<bf16*>(box), krow + (lane & 7) + ((lane >> 4) << 3), (n & 3) * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] *= corr[e & 1];
+            mma16816(o[n], va, p0, p1);
+        }
+    }
+    template <typename Row, typename Ml>
+    __device__ __forceinline__ void finish(int G, int g, int t, Row row_of, Ml ml_of) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (2 * t + h >= G) continue;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                row_of(2 * t + h)[n * 16 + g] = o[n][h];
+                row_of(2 * t + h)[n * 16 + g + 8] = o[n][2 + h];
+            }
+            if (g == 0) *ml_of(2 * t + h) = make_float2(m[h], l[h]);
+        }
+    }
+};
+
+// One share of the pages that only row `tok` reads, for the query heads of one kv head: four warps take 16 keys of every page, their
+// results are merged in shared memory; the first thread asks for the pages.  (A warp more for that leaves an SM two CTAs instead of three:
+// 64 rows on 32 pages 31 us, this 29.4.)  Rows with many pages come first, so that the last CTAs to begin are short: 27.9 us.
 // This kernel starts when the prefix kernel's CTAs have all seen the kernel before them complete, and its last CTA alone waits for the
 // prefix kernel, at its end: what it reads, q and the newest position among it, was there when it started.
-template <int DK, int DV, bool EXACT>
-__global__ void __launch_bounds__(256, 2) shared_own_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                                                                const SharedStep st, const SharedArgs args) {
+template <int DK, int DV, bool EXACT, bool EIGHT>
+__global__ void __maxnreg__(EIGHT ? 128 : 144) shared_own_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                                                                 const SharedStep st, const SharedArgs args) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    const int pair = (int)blockIdx.x / args.shares, tok = pair / st.nkv, kvh = pair % st.nkv, share = (int)blockIdx.x % args.shares;
+    const SharedPlan plan(args);
+    const int pair = (int)blockIdx.x / args.shares, kvh = pair % st.nkv, share = (int)blockIdx.x % args.shares, tok = plan.order[pair / st.nkv];
     constexpr int HK = DK / 64, HV = DV / 64;
     constexpr int BOX_BYTES = 64 * 64 * 2;                 // 8 KB
     constexpr int STAGE_BYTES = (HK + HV) * BOX_BYTES;     // K halves then V halves
-    constexpr int STAGES = OWN_STAGES_BYTES / STAGE_BYTES > 4 ? 4 : OWN_STAGES_BYTES / STAGE_BYTES;
-    constexpr int KS = DK / 16, NT = DV / 8;
+    constexpr int STAGES = own_stages(STAGE_BYTES, EIGHT);
+    constexpr int LD = DV + 4;                             // of a merged row: lanes of a warp write to banks of their own
     const int d = EXACT ? DK : st.d, dv = EXACT ? DV : st.dv, nkv = st.nkv, nq = st.nq, G = nq / nkv;
-    const float scale_log2 = st.scale_log2;
     int* status = st.status;
     uint64_t* full = (uint64_t*)(smem + STAGES * STAGE_BYTES);
     uint64_t* empty = full + STAGES;
     volatile int* abort_flag = (volatile int*)(empty + STAGES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const SharedPlan plan(args);
     const int b = st.seq_of_token[tok], at = st.positions[tok], first = plan.pages_of[tok];
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { tma::mbar_init(&full[s], 1); tma::mbar_init(&empty[s], 4); }
@@ -481,102 +652,42 @@ __global__ void __launch_bounds__(256, 2) shared_own_kernel(const __grid_constan
         p_begin = first + share * each;
         npg = max(0, min(each, n - share * each));
     }
-    float o[NT][4];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f; }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    using Heads = std::conditional_t<EIGHT, EightHeads<DK, DV, EXACT>, SixteenHeads<DK, DV, EXACT>>;
+    Heads heads;
     int4 where = make_int4(0, 0, 0, 0);
-    if (warp == 4) {
-        if (lane == 0) {
-            const int* pt = st.page_table + (size_t)b * st.max_pages;
-            for (int i = 0; i < npg; ++i) {
-                const int s = i % STAGES;
-                const uint32_t ph = (uint32_t)(i / STAGES) & 1u;
-                if (!tma::mbar_wait(&empty[s], ph ^ 1u, abort_flag, status, 11)) break;
-                tma::mbar_expect_tx(&full[s], STAGE_BYTES);
-                const int row = (gg_page(pt, p_begin + i, st.max_pages, PageBounds{st.n_pages, status}, 54) * nkv + kvh) * PAGE;
-                uint8_t* dst = smem + s * STAGE_BYTES;
+    if (npg > 0) {
+        const int* pt = st.page_table + (size_t)b * st.max_pages;
+        auto ask = [&](int i) {             // for page i, by one thread
+            const int s = i % STAGES;
+            tma::mbar_expect_tx(&full[s], STAGE_BYTES);
+            const int row = (gg_page(pt, p_begin + i, st.max_pages, PageBounds{st.n_pages, status}, 54) * nkv + kvh) * PAGE;
+            uint8_t* dst = smem + s * STAGE_BYTES;
 #pragma unroll
-                for (int hf = 0; hf < HK; ++hf) tma::load_2d(dst + hf * BOX_BYTES, &tmK, &full[s], hf * 64, row);
+            for (int hf = 0; hf < HK; ++hf) tma::load_2d(dst + hf * BOX_BYTES, &tmK, &full[s], hf * 64, row);
 #pragma unroll
-                for (int hf = 0; hf < HV; ++hf) tma::load_2d(dst + (HK + hf) * BOX_BYTES, &tmV, &full[s], hf * 64, row);
-            }
-        }
-    } else if (warp == 5) {
-        if (share == 0) where = plan.where(tok, kvh, nkv, G, args.runs, lane);
-    } else if (npg > 0) {
-        // Q fragments in the standard A layout: row = head of the group, k = head dimension
-        uint32_t qa[KS][4];
-        {
-            const bf16* q0 = st.q + ((size_t)tok * nq + (size_t)kvh * G) * d;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const int c = ks * 16 + 2 * t;
-                const bool in0 = EXACT || c < d, in1 = EXACT || c + 8 < d;
-                qa[ks][0] = g < G && in0 ? __ldcg(reinterpret_cast<const unsigned int*>(q0 + (size_t)g * d + c)) : 0u;
-                qa[ks][1] = g + 8 < G && in0 ? __ldcg(reinterpret_cast<const unsigned int*>(q0 + (size_t)(g + 8) * d + c)) : 0u;
-                qa[ks][2] = g < G && in1 ? __ldcg(reinterpret_cast<const unsigned int*>(q0 + (size_t)g * d + c + 8)) : 0u;
-                qa[ks][3] = g + 8 < G && in1 ? __ldcg(reinterpret_cast<const unsigned int*>(q0 + (size_t)(g + 8) * d + c + 8)) : 0u;
-            }
-        }
+            for (int hf = 0; hf < HV; ++hf) tma::load_2d(dst + (HK + hf) * BOX_BYTES, &tmV, &full[s], hf * 64, row);
+        };
+        if (threadIdx.x == 0)
+            for (int i = 0; i < min(npg, STAGES); ++i) ask(i);
+        __syncwarp();
+        heads.load(st.q + ((size_t)tok * nq + (size_t)kvh * G) * d, G, d, g, t);
+        if (warp == 3 && share == 0) where = plan.where(tok, kvh, nkv, G, args.runs, lane);
         const int krow = warp * 16;     // this warp's 16 keys of every page
         for (int i = 0; i < npg; ++i) {
             const int s = i % STAGES;
             const uint32_t ph = (uint32_t)(i / STAGES) & 1u;
-            if (!tma::mbar_wait(&full[s], ph, abort_flag, status, 12)) break;
-            const uint8_t* st = smem + s * STAGE_BYTES;
+            if (!__all_sync(0xffffffffu, tma::mbar_wait(&full[s], ph, abort_flag, status, 12))) break;
+            const uint8_t* stage = smem + s * STAGE_BYTES;
             const int key0 = (p_begin + i) * PAGE + krow;
-            float sc[2][4];
-            sc[0][0] = sc[0][1] = sc[0][2] = sc[0][3] = 0.f;
-            sc[1][0] = sc[1][1] = sc[1][2] = sc[1][3] = 0.f;
-            if (key0 <= pos) {      // whole-warp decision: any visible key among these 16?
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const bf16* box = reinterpret_cast<const bf16*>(st + (ks >> 2) * BOX_BYTES);
-                    uint32_t kb[4];
-                    ldsm_x4(kb, sw<64>(const_cast<bf16*>(box), krow + (lane & 7) + ((lane >> 4) << 3), (ks & 3) * 2 + ((lane >> 3) & 1)));
-                    mma16816(sc[0], qa[ks], kb[0], kb[1]);
-                    mma16816(sc[1], qa[ks], kb[2], kb[3]);
-                }
-                float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int kidx = key0 + j * 8 + 2 * t + (e & 1);
-                        const float v = kidx <= pos ? sc[j][e] * scale_log2 : -INFINITY;
-                        sc[j][e] = v;
-                        mx[e >> 1] = fmaxf(mx[e >> 1], v);
-                    }
-                uint32_t pa[4];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                    const float mn = fmaxf(m[r], mx[r]);
-                    const float mu = mn == -INFINITY ? 0.f : mn;
-                    const float corr = fast_exp2(m[r] - mu);
-                    m[r] = mn;
-                    const float p00 = fast_exp2(sc[0][2 * r] - mu), p01 = fast_exp2(sc[0][2 * r + 1] - mu);
-                    const float p10 = fast_exp2(sc[1][2 * r] - mu), p11 = fast_exp2(sc[1][2 * r + 1] - mu);
-                    l[r] = l[r] * corr + (p00 + p01 + p10 + p11);
-                    pa[r] = pack_bf16(p00, p01);
-                    pa[2 + r] = pack_bf16(p10, p11);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) { o[n][2 * r] *= corr; o[n][2 * r + 1] *= corr; }
-                }
-#pragma unroll
-                for (int np = 0; np < NT / 2; ++np) {
-                    const bf16* box = reinterpret_cast<const bf16*>(st + (HK + (np >> 2)) * BOX_BYTES);
-                    uint32_t vb[4];
-                    ldsm_x4_trans(vb, sw<64>(const_cast<bf16*>(box), krow + (lane & 7) + (((lane >> 3) & 1) << 3), (np & 3) * 2 + (lane >> 4)));
-                    mma16816(o[2 * np], pa, vb[0], vb[1]);
-                    mma16816(o[2 * np + 1], pa, vb[2], vb[3]);
-                }
-            }
+            // (a decision of the whole warp: any visible key among these 16?)
+            if (key0 <= pos) heads.page(stage, stage + HK * BOX_BYTES, krow, key0, pos, st.scale_log2, lane);
             __syncwarp();
             if (lane == 0) tma::mbar_arrive(&empty[s]);
+            if (threadIdx.x == 0 && i + STAGES < npg && tma::mbar_wait(&empty[s], ph, abort_flag, status, 11)) ask(i + STAGES);
+            __syncwarp();
         }
+    } else if (warp == 3 && share == 0) {
+        where = plan.where(tok, kvh, nkv, G, args.runs, lane);
     }
     __syncthreads();          // all pages consumed (or the CTA gave up): the ring can be reused for the merge
     if (*abort_flag) {
@@ -584,38 +695,24 @@ __global__ void __launch_bounds__(256, 2) shared_own_kernel(const __grid_constan
         while (clock64() - t0 < 2000000LL) { }       // let copies in flight land before the CTA goes away
         __syncthreads();
     }
-    if (warp == 5 && share == 0 && lane == 0) args.where[tok * nkv + kvh] = where;
-    float* sm_o = reinterpret_cast<float*>(smem);                 // [4][16][DV]
-    float* sm_ml = sm_o + 4 * 16 * DV;                            // [4][16][2]
-    if (warp < 4) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        }
-        // only the G rows that are query heads go on (the MMA tile has 16)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            if (g + 8 * r >= G) continue;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-                *reinterpret_cast<float2*>(&sm_o[(warp * 16 + g + 8 * r) * DV + n * 8 + 2 * t]) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
-            if (t == 0) { sm_ml[(warp * 16 + g + 8 * r) * 2] = m[r]; sm_ml[(warp * 16 + g + 8 * r) * 2 + 1] = l[r]; }
-        }
-    }
+    if (warp == 3 && share == 0 && lane == 0) args.where[tok * nkv + kvh] = where;
+    float* sm_o = reinterpret_cast<float*>(smem);                 // [4][16][LD]
+    float2* sm_ml = reinterpret_cast<float2*>(sm_o + 4 * 16 * LD);     // [4][16]
+    heads.finish(G, g, t, [&](int head) { return sm_o + (warp * 16 + head) * LD; }, [&](int head) { return sm_ml + warp * 16 + head; });
     __syncthreads();
-    for (int idx = threadIdx.x; idx < G * dv / 4; idx += THREADS) {
+    for (int idx = threadIdx.x; idx < G * dv / 4; idx += OWN_THREADS) {
         const int r = idx / (dv / 4), c = (idx - r * (dv / 4)) * 4;
-        float m4[4], M = -INFINITY, L = 0.f;
+        float2 ml[4];
+        float M = -INFINITY, L = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) { m4[w] = sm_ml[(w * 16 + r) * 2]; M = fmaxf(M, m4[w]); }
+        for (int w = 0; w < 4; ++w) { ml[w] = sm_ml[w * 16 + r]; M = fmaxf(M, ml[w].x); }
         if (M != -INFINITY) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float f = fast_exp2(m4[w] - M);
-                const float4 v = *reinterpret_cast<const float4*>(&sm_o[(w * 16 + r) * DV + c]);
-                L = fmaf(sm_ml[(w * 16 + r) * 2 + 1], f, L);
+                const float f = fast_exp2(ml[w].x - M);
+                const float4 v = *reinterpret_cast<const float4*>(&sm_o[(w * 16 + r) * LD + c]);
+                L = fmaf(ml[w].y, f, L);
                 acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
             }
         }
@@ -699,19 +796,19 @@ __global__ void __launch_bounds__(JOIN_HALVES * 16) shared_join_kernel(bf16* __r
     *reinterpret_cast<uint4*>(out + ((size_t)tok * nq + h) * dv + c) = make_uint4(y[0], y[1], y[2], y[3]);
 }
 
-template <int DK, int DV, bool EXACT>
+template <int DK, int DV, bool EXACT, bool EIGHT>
 int launch_shared(const CUtensorMap& tk, const CUtensorMap& tv, int ntok, const SharedStep& st, const SharedArgs& args, cudaStream_t stream) {
     // Q, K x 2, V x 2 (boxes of 64 columns: 16 KB of Q, 8 KB of K or V), barriers
     constexpr int smem = (DK / 64) * (16384 + 2 * 8192) + (DV / 64) * 2 * 8192 + 256;
     // the ring of a row's own pages, over which its warps' results are merged; barriers
-    constexpr int stage = (DK + DV) / 64 * 8192, ring = (OWN_STAGES_BYTES / stage > 4 ? 4 : OWN_STAGES_BYTES / stage) * stage, own = ring + 256;
-    static_assert(own >= 4 * 16 * (DV + 2) * 4, "the merge lies where the ring was");
+    constexpr int stage = (DK + DV) / 64 * 8192, ring = own_stages(stage, EIGHT) * stage, own = ring + 256;
+    static_assert(own >= 4 * 16 * (DV + 4 + 2) * 4, "the merge lies where the ring was");
     static int known[2][GG_MAX_DEVICES];
     int resident = 0, rc;
     if ((rc = gg_resident(shared_prefix_kernel<DK, DV, EXACT>, THREADS, smem, known[0], resident)) != 0) return rc;
-    if ((rc = gg_resident(shared_own_kernel<DK, DV, EXACT>, THREADS, own, known[1], resident)) != 0) return rc;
+    if ((rc = gg_resident(shared_own_kernel<DK, DV, EXACT, EIGHT>, OWN_THREADS, own, known[1], resident)) != 0) return rc;
     if ((rc = gg_launch(shared_prefix_kernel<DK, DV, EXACT>, dim3(args.runs), dim3(THREADS), smem, stream, 1, tk, tv, st, args)) != 0) return rc;
-    return gg_launch(shared_own_kernel<DK, DV, EXACT>, dim3(ntok * st.nkv * args.shares), dim3(THREADS), own, stream, 1, tk, tv, st, args);
+    return gg_launch(shared_own_kernel<DK, DV, EXACT, EIGHT>, dim3(ntok * st.nkv * args.shares), dim3(OWN_THREADS), own, stream, 1, tk, tv, st, args);
 }
 
 }  // namespace
@@ -744,7 +841,8 @@ GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_po
     float* where = part + rows * dv;
     const SharedArgs args = {plan, ntok, runs, shares, part, reinterpret_cast<float2*>(where + 4ll * ntok * nkv), reinterpret_cast<int4*>(where),
                              (int)prefix_rows, max_pages};
-#define GG_SHARED(DK_, DV_, EX_) launch_shared<DK_, DV_, EX_>(tk, tv, ntok, st, args, stream)
+#define GG_SHARED(DK_, DV_, EX_) (nq / nkv <= 8 ? launch_shared<DK_, DV_, EX_, true>(tk, tv, ntok, st, args, stream) \
+                                                : launch_shared<DK_, DV_, EX_, false>(tk, tv, ntok, st, args, stream))
     if (d == 128 && dv == 128) rc = GG_SHARED(128, 128, true);
     else if (d == 64 && dv == 64) rc = GG_SHARED(64, 64, true);
     else if (d <= 64 && dv <= 64) rc = GG_SHARED(64, 64, false);

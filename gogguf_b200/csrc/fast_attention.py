@@ -70,8 +70,8 @@ def shared_scratch(n_tokens: int, nq: int, nkv: int, dv: int, shares: Optional[i
 
 def shared_shares(n_tokens: int, nkv: int, own_pages: int) -> int:
     """CTAs that share a row's own pages, of which the longest row has `own_pages`: up to one and a half for each place on the device, and
-    two pages each at least (25 rows of 4 kv heads of 80, some of which have 37 pages of their own, 1 / 2 / 4 / 8 shares: 26 / 19.4 /
-    17.7 / 18.0 us; 64 rows of 8 kv heads, with up to 8 pages, 1 / 2 / 4: 31 / 33 / 39)."""
+    two pages each at least (25 rows of 4 kv heads of 80, some of which have 37 pages of their own, 1 / 2 / 4 shares: 25.6 / 18.1 /
+    16.4 us; 64 rows of 8 kv heads, with up to 8 pages, 28 / 30 / 34)."""
     return max(1, min(444 // (n_tokens * nkv), own_pages // 2, SHARED_SHARES))
 
 
@@ -88,12 +88,16 @@ def prefix_pays(groups: Sequence[Tuple[int, int]], n_tokens: int, nkv: int) -> b
 
 
 def shared_runs(groups: Sequence[Tuple[int, int]], nq: int, nkv: int) -> int:
-    """CTAs over the prefixes of groups of (members, pages): one an SM, which leaves room for the CTAs of the rows' own pages beside
-    it, until a CTA has more than six pages (measured, us, one against two an SM: 64 rows of 32 heads on 32 pages 31 / 38; 12 rows of
-    32 heads on 2 kv heads, 256 pages 23 / 21; 64 rows on 512 pages 74 / 64)."""
+    """CTAs over the prefixes of groups of (members, pages): one an SM at most, which leaves room for the CTAs of the rows' own pages beside
+    it, until those would have more than six pages each (measured, us, one against two an SM: 64 rows of 32 heads on 32 pages 28 / 36;
+    12 rows of 32 heads on 2 kv heads, 256 pages 23 / 20; 64 rows on 512 pages 74 / 62), and with four pages each at least: a CTA's beginning
+    and end cost as much as three (64 rows on 16 pages, 2 / 3 / 4 / 8 pages a CTA: 27.0 / 26.0 / 25.7 / 26.2; 32 rows on 32 pages 22.1 /
+    23.3 / 20.8 / 22.9; 48 and 16 rows of 40 heads on 20 pages 29.2 / 26.7 / 25.6 / 31.5)."""
     most = SHARED_ROWS // (nq // nkv)
     units = sum(pages * -(-members // most) for members, pages in groups) * nkv
-    return SHARED_RUNS // 2 if units <= 6 * (SHARED_RUNS // 2) else SHARED_RUNS
+    if units > 6 * (SHARED_RUNS // 2):
+        return SHARED_RUNS
+    return min(SHARED_RUNS // 2, -(-units // 4)) or SHARED_RUNS // 2
 
 
 def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[int], int]]:
@@ -130,15 +134,15 @@ def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[i
 class PrefixPlan:
     """Which token rows of a decode step read which prefix together, as `attn_decode_shared` takes it: `groups` is a list of
     (token rows, leading pages that are the same in all their sequences).  Every shared page must lie wholly before its rows'
-    own positions.  A plan serves all layers of a step that read through the same page table.  `own_pages`: the most pages that a
-    row reads beside the shared ones, where that is known."""
+    own positions.  A plan serves all layers of a step that read through the same page table.  `own_pages`: the pages that each
+    row reads beside the shared ones, where that is known (it only chooses the launch and its order)."""
 
-    def __init__(self, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, device, own_pages: Optional[int] = None):
+    def __init__(self, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, device, own_pages: Optional[Sequence[int]] = None):
         host = torch.empty(self.words_for(n_tokens), dtype=torch.int32)
-        self.pack(groups, n_tokens, host.numpy())
+        self.pack(groups, n_tokens, host.numpy(), own_pages)
         self.n_tokens = n_tokens
         self.words = host.to(device)
-        self.own_pages = own_pages
+        self.own_pages = None if own_pages is None else max(own_pages)
         self.groups: Optional[List[Tuple[int, int]]] = [(len(rows), int(pages)) for rows, pages in groups]
 
     def pays(self, nkv: int) -> bool:
@@ -151,13 +155,13 @@ class PrefixPlan:
 
     @staticmethod
     def words_for(n_tokens: int) -> int:
-        return 5 + 7 * n_tokens
+        return 5 + 8 * n_tokens
 
     @classmethod
     def over(cls, words: torch.Tensor, n_tokens: int, own_pages: Optional[int] = None,
              groups: Optional[Sequence[Tuple[int, int]]] = None) -> "PrefixPlan":
         """A plan whose words are (or will be) on the device already, packed by `pack`; `groups`: (members, pages) of those it will
-        hold, which choose the launch (any others are right, too)."""
+        hold, and `own_pages`, the most that a row reads beside them, choose the launch (any others are right, too)."""
         plan = cls.__new__(cls)
         if words.dtype != torch.int32 or words.numel() != cls.words_for(n_tokens) or not words.is_contiguous():
             raise KernelError(f"shared attention: a plan of {n_tokens} tokens has {cls.words_for(n_tokens)} int32 words")
@@ -166,15 +170,21 @@ class PrefixPlan:
         return plan
 
     @classmethod
-    def pack(cls, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, out: np.ndarray) -> None:
-        """Write the plan's words (csrc/attention_shared.cu: SharedArgs) to `out`; refuses rows that are not the step's, that
+    def pack(cls, groups: Sequence[Tuple[Sequence[int], int]], n_tokens: int, out: np.ndarray, own_pages: Optional[Sequence[int]] = None) -> None:
+        """Write the plan's words (csrc/attention_shared.cu: SharedArgs) to `out`, with the rows of most `own_pages` first in the order in
+        which those are read; refuses rows that are not the step's, that
         appear twice, and groups without a row or page."""
         if n_tokens <= 0:
             raise KernelError("shared attention: a plan needs at least one token row")
         first = out[4:5 + n_tokens]
-        pages, lead, rows, pages_of, group_of, member_of = (out[5 + k * n_tokens:5 + (k + 1) * n_tokens] for k in range(1, 7))
+        pages, lead, rows, pages_of, group_of, member_of, order = (out[5 + k * n_tokens:5 + (k + 1) * n_tokens] for k in range(1, 8))
         out[:cls.words_for(n_tokens)] = 0
         group_of[:] = -1
+        if own_pages is not None and len(own_pages) > n_tokens:
+            raise KernelError(f"shared attention: own pages of {len(own_pages)} rows, the step has {n_tokens}")
+        most = np.zeros(n_tokens, dtype=np.int64)
+        most[:len(own_pages or ())] = own_pages or ()
+        order[:] = np.argsort(-most, kind="stable")
         at = 0
         for g, (members, shared) in enumerate(groups):
             members = list(members)
@@ -210,7 +220,7 @@ class PrefixPlan:
         for rows, shared in groups:
             for r in rows:
                 own[r] -= shared
-        return cls(groups, len(pages), device, own_pages=max(own))
+        return cls(groups, len(pages), device, own_pages=own)
 
 
 def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, page_size, plan: PrefixPlan, scratch, nq, nkv, d, scale,

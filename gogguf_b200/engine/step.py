@@ -89,10 +89,14 @@ def plan_words(n_tokens: int) -> int:
 
 @dataclass
 class SharedPrefixes:
-    """The prefixes that a decode step's sequences share, by KV group: groups of (rows of the step, pages), and the most pages that a
+    """The prefixes that a decode step's sequences share, by KV group: groups of (rows of the step, pages), and the pages that each
     sequence reads beside them."""
     groups: Dict[int, List[Tuple[List[int], int]]]
-    own_pages: int
+    own: Dict[int, List[int]]
+
+    @property
+    def own_pages(self) -> int:
+        return max(max(have) for have in self.own.values())
 
     def key(self) -> Tuple:
         """What a captured step's launches depend on: the groups' weight and the own pages, each up to a power of two."""
@@ -192,7 +196,7 @@ class Stepper:
             return None
         from ..csrc.fast_attention import prefix_pays, shared_groups
         starts = [self.cache.lengths[s] for s in slots]
-        found, own = {}, 0
+        found, own = {}, {}
         for st in stores:
             # (what sequences share does not change while they grow)
             known = self._found.get(st.index)
@@ -207,7 +211,7 @@ class Stepper:
                 for r, pages in groups:
                     for i in r:
                         have[i] -= pages
-                own = max(own, max(have))
+                own[st.index] = have
         return SharedPrefixes(found, own) if found else None
 
     def prefix_plans(self, lay: StepLayout, dev: torch.Tensor, prefixes: Optional[SharedPrefixes]) -> Dict[int, object]:
@@ -284,7 +288,7 @@ class Stepper:
                 pt[:len(entries)] = np.asarray(cache.page_table(g, slots, width), dtype=np.int32)
         for g, gs in (prefixes.groups.items() if prefixes else ()):
             from ..csrc.fast_attention import PrefixPlan
-            PrefixPlan.pack(gs, B, lay.view(h, f"prefix{g}"))
+            PrefixPlan.pack(gs, B, lay.view(h, f"prefix{g}"), prefixes.own[g])
         dev[:lay.total].copy_(host[:lay.total], non_blocking=True)
         if dev.is_cuda:
             if self._copied is None:

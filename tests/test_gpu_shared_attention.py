@@ -106,6 +106,13 @@ CASES = {
     "values wider than keys": dict(groups=[5], prefix=[11], own=(1, 70), nq=6, nkv=2, d=40, dv=120),
     "keys wider than values": dict(groups=[5], prefix=[11], own=(1, 70), nq=6, nkv=2, d=128, dv=64, gate=True),
     "sinks and gates": dict(groups=[8, 2], prefix=[12, 20], own=(30, 300), nq=16, nkv=4, d=128, sink=True, gate=True),
+    "twelve heads, values wider": dict(groups=[5, 1], prefix=[11, 3], own=(1, 200), nq=24, nkv=2, d=40, dv=120, sink=True),
+    "eleven heads, keys wider": dict(groups=[4], prefix=[3], own=(1, 200), nq=11, nkv=1, d=128, dv=64),
+    "ten heads of 64": dict(groups=[7], prefix=[5], own=(1, 300), nq=20, nkv=2, d=64, gate=True),
+    "sixteen small heads": dict(groups=[9, 2], prefix=[4, 20], own=(1, 90), nq=16, nkv=1, d=32, dv=24),
+    "nine heads of 80 and 72": dict(groups=[3, 1], prefix=[9, 9], own=(60, 140), nq=36, nkv=4, d=80, dv=72, sink=True),
+    "eight small heads": dict(groups=[9, 2], prefix=[4, 20], own=(1, 90), nq=16, nkv=2, d=24, dv=56),
+    "eight heads of 128, sixteen wide scores": dict(groups=[3], prefix=[8], own=(1, 200), nq=8, nkv=1, d=128, size=60.0),
     "scores far apart": dict(groups=[6], prefix=[10], own=(1, 90), nq=8, nkv=4, d=64, size=60.0),
 }
 

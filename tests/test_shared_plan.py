@@ -70,7 +70,7 @@ def test_groups_of_random_trees_share_what_they_say(seed):
 def test_plan_words():
     plan = A.PrefixPlan([([3, 0], 7), ([2], 1)], 5, "cpu")
     w = plan.words.tolist()
-    assert len(w) == A.PrefixPlan.words_for(5) == 40 and w[0] == 2
+    assert len(w) == A.PrefixPlan.words_for(5) == 45 and w[0] == 2
     assert w[4:7] == [0, 2, 3]                      # first members
     assert w[10:12] == [7, 1]                       # pages
     assert w[15:17] == [3, 2]                       # first rows
@@ -79,7 +79,17 @@ def test_plan_words():
     assert w[30:35] == [0, -1, 1, 0, -1]            # group of each row
     assert [w[35], w[37], w[38]] == [1, 0, 0]       # place among the members
     empty = A.PrefixPlan([], 3, "cpu").words.tolist()
-    assert empty == [0] * 20 + [-1] * 3 + [0] * 3
+    assert empty == [0] * 20 + [-1] * 3 + [0] * 3 + [0, 1, 2]
+
+
+def test_rows_with_many_pages_of_their_own_come_first():
+    words = np.full(A.PrefixPlan.words_for(4), 9, dtype=np.int32)
+    A.PrefixPlan.pack([([0, 2], 1)], 4, words, [2, 7, 3])                 # the last row is padding
+    assert words[-4:].tolist() == [1, 2, 0, 3]
+    A.PrefixPlan.pack([], 4, words)
+    assert words[-4:].tolist() == [0, 1, 2, 3]
+    with pytest.raises(KernelError):
+        A.PrefixPlan.pack([], 4, words, [1] * 5)
 
 
 def test_own_pages_and_their_shares():
@@ -93,7 +103,7 @@ def test_when_a_prefix_pays_and_in_how_many_runs():
     assert not A.prefix_pays([], 4, 8) and not A.prefix_pays([(2, 60)], 2, 8) and A.prefix_pays([(2, 130)], 2, 8)
     assert not A.prefix_pays([(8, 32)], 8, 8) and A.prefix_pays([(8, 64)], 8, 8) and A.prefix_pays([(64, 32)], 64, 8)
     assert A.prefix_pays([(300, 20)], 300, 8) and not A.prefix_pays([(2, 20)], 300, 8)
-    assert A.shared_runs([(64, 32)], 32, 8) == 148 and A.shared_runs([(64, 512)], 32, 8) == 296 and A.shared_runs([], 32, 8) == 148
+    assert A.shared_runs([(64, 32)], 32, 8) == 128 and A.shared_runs([(2, 3)], 32, 8) == 6 and A.shared_runs([(64, 512)], 32, 8) == 296 and A.shared_runs([], 32, 8) == 148
 
 
 @pytest.mark.parametrize("groups, n", [([([0, 5], 2)], 5), ([([-1, 2], 2)], 5), ([([1, 1], 2)], 5), ([([0, 1], 2), ([1, 2], 2)], 5),
