@@ -1438,18 +1438,13 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, hi
     if out is None:
         out = logits
     here = torch._C._cuda_getDevice() if logits.is_cuda else -1
-
-    def need(t, dt, what):
-        if t.dtype is not dt or t.get_device() != here or not t.is_contiguous():
-            raise KernelError(f"shape_logits: {what} must be contiguous {dt} on the logits' device, got {t.dtype} on {t.device}")
-        return t.data_ptr()
-
-    (have, V), (ld, one) = logits.shape, logits.stride()
-    R = have if rows is None else index(rows)
-    ldo = out.stride(0)
-    if logits.dtype != torch.float32 or out.dtype != torch.float32 or one != 1 or out.stride(1) != 1:
+    (R, V), (ld, one), (out_rows, out_v), (ldo, out_one) = logits.shape, logits.stride(), out.shape, out.stride()
+    if logits.dtype is not torch.float32 or out.dtype is not torch.float32 or one != 1 or out_one != 1:
         raise KernelError("shape_logits: logits and out must be float32 rows")
-    if R < 0 or R > have or out.shape[0] < R or out.shape[1] != V or (R > 1 and (ld < V or ldo < V)):
+    have = R
+    if rows is not None:
+        R = index(rows)
+    if R < 0 or R > have or out_rows < R or out_v != V or (R > 1 and (ld < V or ldo < V)):
         raise KernelError(f"shape_logits: {R} rows of logits {tuple(logits.shape)} into {tuple(out.shape)}")
     if not (0 < repeat < math.inf and -math.inf < frequency < math.inf and -math.inf < presence < math.inf):
         raise KernelError("shape_logits: repeat must be positive, and it, frequency and presence finite")
@@ -1462,47 +1457,52 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, hi
     a, b = logits.data_ptr(), out.data_ptr()
     if (a != b or ld != ldo) and a < b + 4 * ((R - 1) * ldo + V) and b < a + 4 * ((R - 1) * ld + V):
         raise KernelError("shape_logits: out is neither the logits nor apart from them")
+    i32 = torch.int32
     p_ring = p_hist = p_len = p_start = p_ids = p_values = p_masks = p_mask_rows = 0
     last_n = n_biases = states = words = 0
-    requests = -1                                # the parts' number of requests
-
-    def agree(n, what):
-        if n != requests and requests >= 0 or (ring_rows is None and n < R):
-            raise KernelError(f"shape_logits: {what} is for {n} requests, other parts for {requests}, and there are {R} rows")
-        return n
-
+    parts, counts = (), ()                       # what must be contiguous on the device, and the parts' numbers of requests
     if ring_rows is not None:
-        p_ring = need(ring_rows, torch.int32, "ring_rows")
         if ring_rows.numel() < R:
             raise KernelError(f"shape_logits: {ring_rows.numel()} ring_rows for {R} rows")
+        parts, p_ring = ((ring_rows, i32),), ring_rows.data_ptr()
     if hist is not None:
-        p_hist, p_len = need(hist, torch.int32, "hist"), need(hist_len, torch.int32, "hist_len")
-        if hist.dim() != 2 or hist_len.numel() != hist.shape[0]:
+        if hist.dim() != 2:
             raise KernelError("shape_logits: hist and hist_len disagree")
-        requests, last_n = agree(hist.shape[0], "hist"), hist.shape[1]
-        if last_n == 0:
-            p_hist = p_len = 0
+        n, last_n = hist.shape
+        if hist_len.numel() != n:
+            raise KernelError("shape_logits: hist and hist_len disagree")
+        parts, counts = parts + ((hist, i32), (hist_len, i32)), (n,)
+        if last_n:
+            p_hist, p_len = hist.data_ptr(), hist_len.data_ptr()
     if bias is not None:
         start, ids, values = bias
-        p_start, p_ids, p_values = need(start, torch.int32, "bias start"), need(ids, torch.int32, "bias ids"), need(values, torch.float32,
-                                                                                                               "bias values")
-        n_biases = ids.numel()
-        if start.numel() < 2 or n_biases != values.numel():
+        n, n_biases = start.numel() - 1, ids.numel()
+        if n < 1 or n_biases != values.numel():
             raise KernelError("shape_logits: bias ids and values disagree")
-        requests = agree(start.numel() - 1, "bias")
-        if n_biases == 0:
-            p_start = p_ids = p_values = 0
+        parts, counts = parts + ((start, i32), (ids, i32), (values, torch.float32)), counts + (n,)
+        if n_biases:
+            p_start, p_ids, p_values = start.data_ptr(), ids.data_ptr(), values.data_ptr()
     if masks is not None:
-        p_masks, p_mask_rows = need(masks, torch.int32, "masks"), need(mask_rows, torch.int32, "mask_rows")
-        if masks.dim() != 2 or masks.shape[0] == 0 or masks.shape[1] * 32 < V:
+        if masks.dim() != 2:
             raise KernelError(f"shape_logits: masks {tuple(masks.shape)} do not cover {V} ids")
-        requests = agree(mask_rows.numel(), "mask_rows")
         states, words = masks.shape
+        if states == 0 or words * 32 < V:
+            raise KernelError(f"shape_logits: masks {tuple(masks.shape)} do not cover {V} ids")
+        parts, counts = parts + ((masks, i32), (mask_rows, i32)), counts + (mask_rows.numel(),)
+        p_masks, p_mask_rows = masks.data_ptr(), mask_rows.data_ptr()
+    requests = counts[0] if counts else R
+    for n in counts:
+        if n != requests or (ring_rows is None and n < R):
+            raise KernelError(f"shape_logits: the parts are for {counts} requests, and there are {R} rows")
+    for t, dt in parts:
+        if t.dtype is not dt or t.get_device() != here or not t.is_contiguous():
+            raise KernelError("shape_logits: ring_rows, hist, hist_len, the biases' start and ids, masks and mask_rows are int32, the biases' "
+                              f"values float32, all contiguous and on the logits' device: got {t.dtype} of {tuple(t.shape)} on {t.device}")
     if here < 0 or logits.get_device() != here or out.get_device() != here:
         raise KernelError("shape_logits: logits and out must be on the current CUDA device (there is no CPU path)")
     kernel("logit_shaping", "gg_shape_logits")(
-        a, ld, b, ldo, R, V, p_ring, requests if requests >= 0 else R, p_hist, p_len, last_n, float(repeat), float(frequency),
-        float(presence), p_start, p_ids, p_values, n_biases, p_masks, p_mask_rows, states, words, _stream())
+        a, ld, b, ldo, R, V, p_ring, requests, p_hist, p_len, last_n, float(repeat), float(frequency), float(presence), p_start, p_ids, p_values,
+        n_biases, p_masks, p_mask_rows, states, words, _stream())
     return out
 
 
