@@ -78,9 +78,10 @@ def shared_shares(n_tokens: int, nkv: int, own_pages: int) -> int:
 def prefix_pays(groups: Sequence[Tuple[int, int]], n_tokens: int, nkv: int) -> bool:
     """Is reading the prefixes of groups of (members, pages) once, in a step of n_tokens rows, quicker than every row for itself?  From
     12 pages of prefixes on that a CTA of the unshared kernel would read (measured, us, unshared / shared with two pages of a row's own,
-    32 heads of 128 on 8 kv heads: 2 rows, 8 pages a CTA 10 / 13, 16 15.4 / 15.4, 32 26 / 21; 8 rows, 8 10.6 / 12.1, 16 15.9 / 14.8;
-    32 rows, 16 16 / 19, 32 27 / 20; 64 rows, 14 21 / 22, 27 31 / 23; 16 heads of 64: 8 rows, 8 8.6 / 9.9, 16 14.1 / 11.4; 24 heads of
-    80 on 4 kv heads: 16 rows, 8 11.1 / 12.0, 16 16.2 / 13.3)."""
+    32 heads of 128 on 8 kv heads: 2 rows, 8 pages a CTA 10.0 / 13.0, 16 15.4 / 15.1, 32 26 / 20; 8 rows, 8 10.6 / 12.3, 16 16.0 / 14.9;
+    32 rows, 16 15.8 / 17.3, 32 26 / 19; 64 rows, 14 20.8 / 18.5, 27 31 / 19; 16 heads of 64 on 8: 8 rows, 8 8.7 / 10.3, 16 14.1 / 11.8; 64
+    rows, 14 13.7 / 15.0; 24 heads of 80 on 4: 16 rows, 8 11.1 / 12.9, 16 16.6 / 14.1; sixteen heads a kv head gain sooner, 32 of 128 on
+    2: 64 rows, 8 20.4 / 16.3)."""
     pairs, splits = n_tokens * nkv, 1
     while splits * 2 <= min(8, 296 // pairs):
         splits *= 2

@@ -1,4 +1,4 @@
-"""Kernel micro-benchmarks: python -m gogguf_b200.csrc.microbench [gemm|gemm_layer|attn|prefill_attn|sample|latent|retention|recurrence|dinuzen|kulesun|niresun|plain|shares|experts|f32_parts] [--m 1,8,64] [--ctx 2048,8192]
+"""Kernel micro-benchmarks: python -m gogguf_b200.csrc.microbench [gemm|gemm_layer|attn|prefill_attn|sample|latent|retention|recurrence|dinuzen|kulesun|niresun|plain|shares|experts|f32_parts|shared] [--m 1,8,64] [--ctx 2048,8192]
 
 Times single kernels the way a decode step runs them: forty launches captured in a CUDA graph and
 replayed, so that host launch cost is out of the picture and dependent launches overlap as they do
@@ -905,10 +905,49 @@ def experts() -> None:
         torch.cuda.empty_cache()
 
 
+def shared() -> None:
+    """Decode attention of rows that share leading pages, row by row (`attn_decode_tma`) and together (`attn_decode_shared`), with two
+    pages of a row's own; the pools' copies rotate over more than L2 holds.  Then the shaping of logits."""
+    from . import fast_attention as A
+    from . import kernels as K
+    dev, page, own = "cuda:0", 64, 2
+    for nq, nkv, d in ((32, 8, 128), (32, 2, 128), (24, 4, 80), (16, 8, 64)):
+        for T in (2, 4, 8, 16, 32, 64):
+            line = f"shared {nq:2d} heads on {nkv} of {d:3d}, {T:2d} rows, pages shared: row by row / together us"
+            for pre in (8, 16, 32, 64, 128, 256, 512):
+                if T * pre * nkv * d > 64 * 512 * 8 * 128:
+                    continue
+                lists = [list(range(pre)) + [pre + r * own + i for i in range(own)] for r in range(T)]
+                lens = [(pre + own) * page - 7 - r % 50 for r in range(T)]
+                pools = max(1, min(12, int(3e8 // ((pre + T * own) * nkv * page * d * 4)) + 1))
+                kv = [[torch.randn(pre + T * own, nkv, page, d, device=dev).to(torch.bfloat16) for _ in range(2)] for _ in range(pools)]
+                q = torch.randn(T, nq * d, device=dev).to(torch.bfloat16)
+                out = torch.empty_like(q)
+                pos, rows, table = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([n - 1 for n in lens], list(range(T)), lists))
+                plan = A.PrefixPlan.of_pages(lists, lens, page, dev)
+                scratch = torch.empty(A.shared_scratch(T, nq, nkv, d), device=dev)
+                us = [_time_graph(lambda i: A.attn_decode_shared(q, *kv[i % pools], out, pos, rows, table, page, plan, scratch, nq, nkv, d,
+                                                                 1 / math.sqrt(d), together=how)) for how in (False, True)]
+                line += f"  {pre}: {us[0]:.1f} / {us[1]:.1f}"
+                del kv
+            print(line, flush=True)
+    V = 151936
+    for R in (1, 8, 64, 256):
+        n = max(1, min(40, int(4e8 // (R * V * 8)) + 1))
+        xs = [torch.randn(R, V, device=dev) for _ in range(n)]
+        out = torch.empty_like(xs[0])
+        hist = torch.randint(0, V, (R, 64), dtype=torch.int32, device=dev)
+        length = torch.full((R,), 64, dtype=torch.int32, device=dev)
+        masks = torch.randint(-2 ** 31, 2 ** 31 - 1, (min(R, 100), V // 32), dtype=torch.int32, device=dev)
+        states = torch.arange(R, dtype=torch.int32, device=dev) % masks.shape[0]
+        us = _time_graph(lambda i: K.shape_logits(xs[i % n], out, hist=hist, hist_len=length, repeat=1.1, frequency=0.2, masks=masks, mask_rows=states))
+        print(f"shaping {R:3d} rows of {V}, 64 last ids, a grammar: {us:6.1f} us {R * V * 8 / us / 1e6:5.2f} TB/s", flush=True)
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("what", choices=["gemm", "gemm_layer", "attn", "prefill_attn", "sample", "latent", "retention", "recurrence", "dinuzen", "kulesun", "niresun",
-                                     "plain", "shares", "experts", "f32_parts"])
+                                     "plain", "shares", "experts", "f32_parts", "shared"])
     ap.add_argument("--m", default="1,8,64", help="token counts (gemm), batch sizes (attn) or prompt lengths (prefill_attn)")
     ap.add_argument("--ctx", default="2048", help="attn: cached positions per sequence (comma separated)")
     ap.add_argument("--scratch", action="store_true", help="attn: splits merged by a second kernel instead of inside clusters")
@@ -923,7 +962,7 @@ def main() -> None:
     if a.what == "recurrence":
         recurrence()
         return
-    alone = {"dinuzen": dinuzen, "kulesun": kulesun, "niresun": niresun, "plain": plain, "shares": shares, "experts": experts, "f32_parts": f32_parts}
+    alone = {"dinuzen": dinuzen, "kulesun": kulesun, "niresun": niresun, "plain": plain, "shares": shares, "experts": experts, "f32_parts": f32_parts, "shared": shared}
     if a.what in alone:
         alone[a.what]()
         return
