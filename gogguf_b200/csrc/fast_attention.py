@@ -107,7 +107,7 @@ def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[i
     in one group at most: where some rows of a group share more pages than all of it, the cut that saves more reads is taken."""
     table = np.asarray(table)
 
-    def best(rows: List[int], depth: int) -> Tuple[int, List[Tuple[List[int], int]]]:
+    def best(rows: List[int], depth: int, cuts: int = 0) -> Tuple[int, List[Tuple[List[int], int]]]:
         if len(rows) < 2:
             return 0, []
         most = min(limits[r] for r in rows)
@@ -116,12 +116,12 @@ def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[i
         common = depth + int(differs[0]) if differs.size else most
         whole = (len(rows) - 1) * common, ([(rows, common)] if common else [])
         below = {}
-        for r in rows:
+        for r in rows if cuts < 100 else ():            # (sequences that branch off one another a hundred times are read as one group)
             if limits[r] > common:
                 below.setdefault(int(table[r, common]), []).append(r)
         saved, groups = 0, []
         for members in below.values():
-            s, g = best(members, common + 1)
+            s, g = best(members, common + 1, cuts + 1)
             saved, groups = saved + s, groups + g
         return (saved, groups) if saved > whole[0] else whole
 

@@ -284,3 +284,14 @@ def test_refusals_on_the_device():
     s.q = s.q.float()
     with pytest.raises(KernelError, match="bfloat16"):
         s.run()
+
+
+def test_debug_build_checks_page_tables():
+    """GOGGUF_B200_DEBUG=1: pages beyond the pool are recorded and not read."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, os.path.join(root, "tests", "debug_shared_script.py"), root], env=dict(os.environ, GOGGUF_B200_DEBUG="1"),
+                       capture_output=True, text=True, timeout=600)
+    assert p.returncode == 0 and "debug shared ok" in p.stdout, p.stdout[-2000:] + p.stderr[-4000:]

@@ -67,6 +67,19 @@ def test_groups_of_random_trees_share_what_they_say(seed):
             assert pages[r][:n] == pages[rows[0]][:n] and n * 64 <= lengths[r] - 1
 
 
+def test_a_long_chain_of_forks():
+    """Row i shares i + 1 pages with the rows after it: a chain of two thousand forks is no deeper than Python goes."""
+    n = 2000
+    pages = np.full((n, n + 1), -1)
+    trunk = np.arange(n)
+    for r in range(n):
+        pages[r, :r + 1] = trunk[:r + 1]
+        pages[r, r + 1] = n + r
+    got = A.shared_groups(pages, [r + 1 for r in range(n)])
+    seen = [r for rows, _ in got for r in rows]
+    assert len(seen) == len(set(seen)) and all((pages[rows, :k] == pages[rows[0], :k]).all() and k >= 1 for rows, k in got)
+
+
 def test_plan_words():
     plan = A.PrefixPlan([([3, 0], 7), ([2], 1)], 5, "cpu")
     w = plan.words.tolist()
