@@ -145,6 +145,7 @@ class PrefixPlan:
         self.words = host.to(device)
         self.own_pages = None if own_pages is None else max(own_pages)
         self.groups: Optional[List[Tuple[int, int]]] = [(len(rows), int(pages)) for rows, pages in groups]
+        self.longest = max((pages for _, pages in self.groups), default=0)
 
     def pays(self, nkv: int) -> bool:
         """`prefix_pays` of this plan's groups (True where they are not known), worked out once."""
@@ -168,6 +169,7 @@ class PrefixPlan:
             raise KernelError(f"shared attention: a plan of {n_tokens} tokens has {cls.words_for(n_tokens)} int32 words")
         plan.n_tokens, plan.words, plan.own_pages, plan.groups = (
             n_tokens, words, own_pages, None if groups is None else list(groups))
+        plan.longest = max((pages for _, pages in plan.groups or ()), default=0)
         return plan
 
     @classmethod
@@ -236,20 +238,29 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
     T = plan.n_tokens
     if not takes(nq, nkv, d, dv):
         raise KernelError(f"shared attention: {nq} heads on {nkv} kv heads of {d} and {dv} are outside what the kernels take")
-    bf16, i32, words = torch.bfloat16, torch.int32, plan.words
+    bf16, i32, f32, words = torch.bfloat16, torch.int32, torch.float32, plan.words
     here = torch._C._cuda_getDevice() if q.is_cuda else -1
-    for t, dt in ((q, bf16), (k_pool, bf16), (v_pool, bf16), (out, bf16), (positions, i32), (seq_of_token, i32), (table, i32), (words, i32),
-                  (scratch, torch.float32)) + (() if sink is None else ((sink, torch.float32),)):
-        if t.dtype is not dt or t.get_device() != here or here < 0 or not t.is_contiguous():
-            raise KernelError("shared attention: q, the pools and out are bfloat16, positions, seq_of_token, the table and the plan int32, "
-                              "scratch and a sink float32, all contiguous and on the current CUDA device: got "
-                              f"{t.dtype} of {tuple(t.shape)} with strides {t.stride()} on {t.device}")
-    pools = k_pool.shape[0]
-    if plan.groups and max(pages for _, pages in plan.groups) > table.shape[-1]:
-        raise KernelError(f"shared attention: the plan's prefixes are longer than the table's {table.shape[-1]} pages")
-    if (q.numel() < T * nq * d or out.numel() < T * nq * dv or positions.numel() < T or seq_of_token.numel() < T or table.dim() != 2
-            or k_pool.shape != (pools, nkv, page_size, d) or v_pool.shape != (pools, nkv, page_size, dv)):
+    wrong = None if here >= 0 else q
+    for t in (q, k_pool, v_pool, out):
+        if t.dtype is not bf16 or t.get_device() != here or not t.is_contiguous():
+            wrong = t
+    for t in (positions, seq_of_token, table, words):
+        if t.dtype is not i32 or t.get_device() != here or not t.is_contiguous():
+            wrong = t
+    for t in (scratch,) if sink is None else (scratch, sink):
+        if t.dtype is not f32 or t.get_device() != here or not t.is_contiguous():
+            wrong = t
+    if wrong is not None:
+        raise KernelError("shared attention: q, the pools and out are bfloat16, positions, seq_of_token, the table and the plan int32, "
+                          "scratch and a sink float32, all contiguous and on the current CUDA device: got "
+                          f"{wrong.dtype} of {tuple(wrong.shape)} with strides {wrong.stride()} on {wrong.device}")
+    k_shape, t_shape = k_pool.shape, table.shape
+    pools, width = k_shape[0], t_shape[-1]
+    if (q.numel() < T * nq * d or out.numel() < T * nq * dv or positions.numel() < T or seq_of_token.numel() < T or len(t_shape) != 2
+            or k_shape != (pools, nkv, page_size, d) or v_pool.shape != (pools, nkv, page_size, dv)):
         raise KernelError("shared attention: shapes disagree")
+    if plan.longest > width:
+        raise KernelError(f"shared attention: the plan's prefixes are longer than the table's {width} pages")
     p_sink = p_gate = ldg = 0
     if sink is not None:
         if sink.numel() != nq:
@@ -265,14 +276,14 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
     if not together:
         if page_size != 64:
             raise KernelError(f"shared attention: pages of 64 positions, not {page_size}")
-        splits = decode_tma_splits(T, nkv, table.shape[1] * page_size, cluster=True)
+        splits = decode_tma_splits(T, nkv, width * page_size, True)
         if not (d == dv and d in (64, 128)):
             splits = min(splits, 8)
         attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page_size, T, nq, nkv, d, scale, 0, splits, cluster=True,
                         sink=sink, out_scale=out_scale, dv=dv, gate=gate)
         return
     if shares is None:
-        shares = shared_shares(T, nkv, table.shape[1] if plan.own_pages is None else plan.own_pages)
+        shares = shared_shares(T, nkv, width if plan.own_pages is None else plan.own_pages)
     elif not 1 <= shares <= SHARED_SHARES:
         raise KernelError(f"shared attention: 1 to {SHARED_SHARES} shares, not {shares}")
     room = shared_scratch(T, nq, nkv, dv, shares)
@@ -284,7 +295,7 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
         raise KernelError(f"shared attention: 1 to {SHARED_RUNS} runs, not {runs}")
     kernel("attention_shared", "gg_attn_decode_shared")(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), table.data_ptr(),
-        table.shape[1], page_size, pools, words.data_ptr(), T, nq, nkv, d, dv, float(scale), int(runs), int(shares), p_sink, float(out_scale),
+        width, page_size, pools, words.data_ptr(), T, nq, nkv, d, dv, float(scale), int(runs), int(shares), p_sink, float(out_scale),
         p_gate, ldg, scratch.data_ptr(), scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
 
 
