@@ -26,6 +26,9 @@
 // shared memory 40 and 62 (but 17 of 8 rows where this is 12), rows' own pages as rows of the product 74 and 168 or in the line of pages 44
 // and 73, own pages as CTAs of the prefix kernel 36 and 64 (24 and 30 of ragged prompts where this was 19 and 20), 128 keys a step 34
 // and 70, 256 rows a tile 44 and 73, eight warps for the softmax 37 and 69.
+#include <climits>
+#include <cstring>
+#include <initializer_list>
 #include <type_traits>
 
 #include "attention_common.cuh"
@@ -816,11 +819,40 @@ int launch_shared(const CUtensorMap& tk, const CUtensorMap& tv, int ntok, const 
 // Decode attention (see gg_attn_decode_tma) of a step with shared prefixes: plan as at SharedArgs; runs (1 to 296): CTAs over
 // the prefixes; shares (1 to 64): CTAs that share a row's own pages; part: scratch of (nq ntok (1 + shares) + 128 runs) (dv + 2) + 4 ntok nkv floats, on a 32-byte boundary.
 // status: codes 71-79 (prefixes), 11 and 12 (own pages) name the wait that ran out.
-GG_API gg_attn_decode_shared(const void* q, const void* k_pool, const void* v_pool, void* out, const int* positions,
-                             const int* seq_of_token, const int* page_table, int max_pages, int page_size, int n_pages, const int* plan,
-                             int ntok, int nq, int nkv, int d, int dv, float scale, int runs, int shares, const float* sink, float out_scale,
-                             const void* gate, long long ldg, float* part, long long part_floats, int* status, cudaStream_t stream) {
-    if (ntok <= 0) return 0;
+//
+// The arguments come packed, eight bytes each (see gg_shape_logits).
+struct SharedCall {
+    const void *q, *k_pool, *v_pool;
+    void* out;
+    const int *positions, *seq_of_token, *page_table;
+    long long max_pages, page_size, n_pages;
+    const int* plan;
+    long long ntok, nq, nkv, d, dv, runs, shares;
+    const float* sink;
+    const void* gate;
+    long long ldg;
+    float* part;
+    long long part_floats;
+    int* status;
+    double scale, out_scale;
+};
+static_assert(sizeof(SharedCall) == 26 * 8, "as the caller packs it");
+
+GG_API gg_attn_decode_shared(const void* call, cudaStream_t stream) {
+    SharedCall c;
+    memcpy(&c, call, sizeof(c));
+    if (c.ntok <= 0) return 0;
+    for (long long n : {c.max_pages, c.n_pages, c.ntok, c.nq, c.nkv, c.ntok * c.nq})
+        if (n <= 0 || n > INT_MAX) return GG_ERR_ARG;
+    const void *q = c.q, *k_pool = c.k_pool, *v_pool = c.v_pool, *gate = c.gate;
+    void* out = c.out;
+    const int *positions = c.positions, *seq_of_token = c.seq_of_token, *page_table = c.page_table, *plan = c.plan;
+    const int max_pages = (int)c.max_pages, page_size = (int)c.page_size, n_pages = (int)c.n_pages, ntok = (int)c.ntok, nq = (int)c.nq,
+              nkv = (int)c.nkv, d = (int)c.d, dv = (int)c.dv, runs = (int)c.runs, shares = (int)c.shares;
+    const float *sink = c.sink, scale = (float)c.scale, out_scale = (float)c.out_scale;
+    const long long ldg = c.ldg, part_floats = c.part_floats;
+    float* part = c.part;
+    int* status = c.status;
     if (page_size != PAGE || nq <= 0 || nkv <= 0 || nq % nkv || nq / nkv > 16 || !attn_shape_ok(d, dv, 0, gate, ldg) || shares < 1 || shares > 64 || runs < 1 || runs > MAX_RUNS ||
         n_pages <= 0 || max_pages <= 0 || status == nullptr || plan == nullptr)
         return GG_ERR_ARG;

@@ -3,6 +3,7 @@ decode kernel (every sequence brings one token) and the prefill kernel, scratch 
 from __future__ import annotations
 
 import functools
+import struct
 from typing import Callable, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -31,6 +32,10 @@ def attn_decode(q, k_pool, v_pool, out, positions, seq_of_token, table, page_siz
         status_word(q.device).data_ptr(), stream_ptr())
 
 
+# The launchers' arguments (csrc/attention_fast.cu: DecodeCall, csrc/attention_shared.cu: SharedCall).
+_DECODE_CALL, _SHARED_CALL = struct.Struct("=25q2d").pack, struct.Struct("=24q2d").pack
+
+
 @functools.lru_cache(maxsize=4096)
 def decode_tma_splits(n_tokens: int, nkv: int, max_ctx: int, cluster: bool = False) -> int:
     return int(module("attention_fast").lib.gg_attn_decode_tma_splits(int(n_tokens), int(nkv), int(max_ctx),
@@ -45,13 +50,13 @@ def attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page
     sink: float32 per query head, joins the softmax's denominator; out_scale: a factor on the result (neither is
     taken by the form that merges its splits with a second kernel).  dv: the values' head size (default d); chunk: a
     position sees its own chunk of that many positions only; gate (rows of nq * dv logits): multiplied in by its sigmoid."""
-    kernel("attention_fast", "gg_attn_decode_tma")(
+    kernel("attention_fast", "gg_attn_decode_tma_packed")(_DECODE_CALL(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(),
         part_o.data_ptr() if part_o is not None else 0, part_ml.data_ptr() if part_ml is not None else 0,
         positions.data_ptr(), seq_of_token.data_ptr(), table.data_ptr(), table.shape[-1], page_size,
-        k_pool.shape[0], n_tokens, nq, nkv, d, d if dv is None else int(dv), float(scale), int(window), int(chunk), int(splits),
-        int(bool(cluster)), sink.data_ptr() if sink is not None else 0, float(out_scale), *_gate(gate),
-        status_word(q.device).data_ptr(), stream_ptr())
+        k_pool.shape[0], n_tokens, nq, nkv, d, d if dv is None else int(dv), int(window), int(chunk), int(splits),
+        int(bool(cluster)), sink.data_ptr() if sink is not None else 0, *_gate(gate),
+        status_word(q.device).data_ptr(), scale, out_scale), stream_ptr())
 
 
 # The most runs over the prefixes, rows of a tile, and the most CTAs that may share a row's own pages (csrc/attention_shared.cu).
@@ -293,10 +298,10 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
         runs = shared_runs(plan.groups or (), nq, nkv)
     elif not 1 <= runs <= SHARED_RUNS:
         raise KernelError(f"shared attention: 1 to {SHARED_RUNS} runs, not {runs}")
-    kernel("attention_shared", "gg_attn_decode_shared")(
+    kernel("attention_shared", "gg_attn_decode_shared")(_SHARED_CALL(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), table.data_ptr(),
-        width, page_size, pools, words.data_ptr(), T, nq, nkv, d, dv, float(scale), int(runs), int(shares), p_sink, float(out_scale),
-        p_gate, ldg, scratch.data_ptr(), scratch.numel(), status_word(q.device).data_ptr(), stream_ptr())
+        width, page_size, pools, words.data_ptr(), T, nq, nkv, d, dv, runs, shares, p_sink, p_gate, ldg, scratch.data_ptr(), scratch.numel(),
+        status_word(q.device).data_ptr(), scale, out_scale), stream_ptr())
 
 
 def attn_prefill(q, k_pool, v_pool, out, cu_seqlens, ctx_lens, seq_of_token, table, page_size, n_seqs,

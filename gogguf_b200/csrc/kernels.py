@@ -1423,6 +1423,9 @@ def history_append(tokens: torch.Tensor, ring_rows: torch.Tensor, hist: torch.Te
                                              hist.shape[1], rows, _stream())
 
 
+_SHAPE_CALL = struct.Struct("=11q3d8q").pack            # csrc/logit_shaping.cu: ShapeCall
+
+
 def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, hist: Optional[torch.Tensor] = None,
                  hist_len: Optional[torch.Tensor] = None, ring_rows: Optional[torch.Tensor] = None, repeat: float = 1.0,
                  frequency: float = 0.0, presence: float = 0.0, bias=None, masks: Optional[torch.Tensor] = None,
@@ -1500,9 +1503,9 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, hi
                               f"values float32, all contiguous and on the logits' device: got {t.dtype} of {tuple(t.shape)} on {t.device}")
     if here < 0 or logits.get_device() != here or out.get_device() != here:
         raise KernelError("shape_logits: logits and out must be on the current CUDA device (there is no CPU path)")
-    kernel("logit_shaping", "gg_shape_logits")(
-        a, ld, b, ldo, R, V, p_ring, requests, p_hist, p_len, last_n, float(repeat), float(frequency), float(presence), p_start, p_ids, p_values,
-        n_biases, p_masks, p_mask_rows, states, words, _stream())
+    kernel("logit_shaping", "gg_shape_logits")(_SHAPE_CALL(
+        a, ld, b, ldo, R, V, p_ring, requests, p_hist, p_len, last_n, repeat, frequency, presence, p_start, p_ids, p_values,
+        n_biases, p_masks, p_mask_rows, states, words), _stream())
     return out
 
 

@@ -8,6 +8,9 @@
 // The rows are cut into slices, one block each: it counts those of the request's last ids that lie in its slice in shared
 // memory (whole numbers, so that the order of the additions does not matter), notes the biases that do, and passes once over
 // its logits.  Whatever the number of ids, no id is compared with another.
+#include <climits>
+#include <cstring>
+
 #include "common.cuh"
 
 namespace {
@@ -202,29 +205,52 @@ __global__ void shape_advance_kernel(int* tokens, const int* __restrict__ ring_r
 
 // out[r] = the shaped logits[r] for R rows of V; out == logits (and ldo == ld): in place, where only what changes is touched.
 // ring_rows (null: row r's request is r) names each row's request among `rings`.
-GG_API gg_shape_logits(const float* logits, long long ld, float* out, long long ldo, int R, int V, const int* ring_rows, int rings,
-                       const int* hist, const int* hist_len, int last_n, float repeat, float frequency, float presence,
-                       const int* bias_start, const int* bias_ids, const float* bias_values, int biases, const int* masks,
-                       const int* mask_rows, int states, int words, cudaStream_t stream) {
-    if (R <= 0) return 0;
-    if (V <= 0 || ld < V || ldo < V || R > 65535 || rings <= 0 || !(repeat > 0.f)) return GG_ERR_ARG;
-    if (hist != nullptr && (hist_len == nullptr || last_n <= 0)) return GG_ERR_ARG;
-    if (bias_start != nullptr && (bias_ids == nullptr || bias_values == nullptr || biases < 0)) return GG_ERR_ARG;
-    if (masks != nullptr && (mask_rows == nullptr || states <= 0 || words < (V + 31) / 32)) return GG_ERR_ARG;
-    const Shaping s = {hist, hist_len, last_n, repeat, frequency, presence, bias_start, bias_ids, bias_values, biases,
-                       masks, mask_rows, states, words};
+//
+// The arguments come packed, eight bytes each: of a call of 5 us on the device ctypes took 3.7 us of the host to convert 23 of them.
+struct ShapeCall {
+    const float* logits;
+    long long ld;
+    float* out;
+    long long ldo, R, V;
+    const int* ring_rows;
+    long long rings;
+    const int *hist, *hist_len;
+    long long last_n;
+    double repeat, frequency, presence;
+    const int *bias_start, *bias_ids;
+    const float* bias_values;
+    long long biases;
+    const int *masks, *mask_rows;
+    long long states, words;
+};
+static_assert(sizeof(ShapeCall) == 22 * 8, "as the caller packs it");
+
+GG_API gg_shape_logits(const void* call, cudaStream_t stream) {
+    ShapeCall c;
+    memcpy(&c, call, sizeof(c));
+    if (c.R <= 0) return 0;
+    if (c.V <= 0 || c.V > INT_MAX - SLICE || c.ld < c.V || c.ldo < c.V || c.R > 65535 || c.rings <= 0 || c.rings > INT_MAX || !(c.repeat > 0.)) return GG_ERR_ARG;
+    if (c.hist != nullptr && (c.hist_len == nullptr || c.last_n <= 0 || c.last_n > INT_MAX - 4 * THREADS)) return GG_ERR_ARG;
+    if (c.bias_start != nullptr && (c.bias_ids == nullptr || c.bias_values == nullptr || c.biases < 0 || c.biases > INT_MAX - THREADS)) return GG_ERR_ARG;
+    if (c.masks != nullptr && (c.mask_rows == nullptr || c.states <= 0 || c.states > INT_MAX || c.words < (c.V + 31) / 32 || c.words > INT_MAX)) return GG_ERR_ARG;
+    const Shaping s = {c.hist, c.hist_len, (int)c.last_n, (float)c.repeat, (float)c.frequency, (float)c.presence, c.bias_start, c.bias_ids,
+                       c.bias_values, (int)c.biases, c.masks, c.mask_rows, (int)c.states, (int)c.words};
+    const float* logits = c.logits;
+    float* out = c.out;
+    const long long ld = c.ld, ldo = c.ldo;
+    const int R = (int)c.R, V = (int)c.V;
     const dim3 grid((V + SLICE - 1) / SLICE, R);
     const bool vec = ((uintptr_t)logits & 15) == 0 && ((uintptr_t)out & 15) == 0 && (R == 1 || ((ld | ldo) & 3) == 0);
     const bool in_place = out == logits;
     if (in_place && R > 1 && ld != ldo) return GG_ERR_ARG;
-    if (in_place && hist == nullptr && bias_start == nullptr && masks == nullptr) return 0;
+    if (in_place && s.hist == nullptr && s.bias_start == nullptr && s.masks == nullptr) return 0;
     // (a request's own list is no longer than all of them)
-    const bool wide = (hist != nullptr && last_n > 65535) || biases > 65534;
+    const bool wide = (s.hist != nullptr && s.last_n > 65535) || s.biases > 65534;
 #define GG_SHAPE(WIDE_) (in_place ? (vec ? shape_logits_kernel<true, 4, WIDE_> : shape_logits_kernel<true, 1, WIDE_>) \
                                   : (vec ? shape_logits_kernel<false, 4, WIDE_> : shape_logits_kernel<false, 1, WIDE_>))
     auto kern = wide ? GG_SHAPE(true) : GG_SHAPE(false);
 #undef GG_SHAPE
-    return gg_launch(kern, grid, dim3(THREADS), 0, stream, 1, logits, ld, out, ldo, V, ring_rows, rings, s);
+    return gg_launch(kern, grid, dim3(THREADS), 0, stream, 1, logits, ld, out, ldo, V, c.ring_rows, (int)c.rings, s);
 }
 
 // R drawn ids (in place); the requests' last ids (hist null: none are kept) as gg_history_append appends to them; their grammar states
