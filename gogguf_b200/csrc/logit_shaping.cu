@@ -100,11 +100,13 @@ __global__ void __launch_bounds__(THREADS, 6) shape_logits_kernel(const float* l
         };
         count(first_id);
         int t = threadIdx.x + THREADS;
-        for (; t + 3 * THREADS < ids; t += 4 * THREADS) {
-            const int a = h[t], b = h[t + THREADS], c = h[t + 2 * THREADS], d = h[t + 3 * THREADS];
-            count(a); count(b); count(c); count(d);
+        for (; t < ids; t += 4 * THREADS) {
+            int some[4];                            // (asked for together)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) some[k] = t + k * THREADS < ids ? h[t + k * THREADS] : -1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) count(some[k]);
         }
-        for (; t < ids; t += THREADS) count(h[t]);
         for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
             const int id = e < b0 + THREADS ? first_bias : s.bias_ids[e];
             if (id < lo || id - lo >= n) continue;
