@@ -12,10 +12,11 @@
 // so that neither the number of readers nor that of kv heads leaves an SM without work, and the grid is the same for every plan:
 // a captured step replays with other groups.
 //
-// A row's own positions: a CTA a (token row, kv head, share), on mma.sync with the query heads as rows, as the decode kernel of a
-// step without prefixes does it (attention_fast.cu).  (As rows of the prefix's product, a page of a member's own took the tensor
-// core as long as one of the prefix: 64 rows with up to 500 positions of their own on 2,048 were 44 us.  As CTAs of the prefix's
-// kernel they ran one an SM: a CTA of a kernel that allocates tensor memory keeps others of it off its SM until it has done so.)
+// A row's own positions: a CTA a (token row, kv head, share), on mma.sync, with the query heads as columns where there are eight
+// at most, else as rows, as in the decode kernel of a step without prefixes (attention_fast.cu).  (As rows of the prefix's product, a
+// page of a member's own took the tensor core as long as one of the prefix: 64 rows with up to 500 positions of their own on 2,048 were
+// 44 us.  As CTAs of the prefix's kernel they ran one an SM: a CTA of a kernel that allocates tensor memory keeps others of it off its
+// SM until it has done so.)
 //
 // What bounds it.  64 rows of 32 heads (8 kv heads of 128) on 512 pages, with up to 200 positions of their own: 62 us (each row by
 // itself 700), of which the prefix kernel takes 45 (a page and tile 1.4 us of a CTA, two CTAs an SM, 268 MB through L2 at 6.7 TB/s, in which
@@ -25,7 +26,7 @@
 // Tried and slower (us, of 64 rows on 32 and 512 pages, when this was 33 and 67): runs in clusters of eight that add up their parts in
 // shared memory 40 and 62 (but 17 of 8 rows where this is 12), rows' own pages as rows of the product 74 and 168 or in the line of pages 44
 // and 73, own pages as CTAs of the prefix kernel 36 and 64 (24 and 30 of ragged prompts where this was 19 and 20), 128 keys a step 34
-// and 70, 256 rows a tile 44 and 73, eight warps for the softmax 37 and 69.
+// and 70, 256 rows a tile 44 and 73, eight warps for the softmax 37 and 69.  Now: K in three stages 28.7 and 63.4.
 #include <climits>
 #include <cstring>
 #include <initializer_list>
@@ -49,8 +50,8 @@ __host__ __device__ constexpr int own_stages(int stage_bytes, bool eight) {
 
 // The plan, integers of a step, with room for `cap` token rows: how many groups; from word 4 on, per group the place of its first
 // member in `rows` (and one place beyond the last group's), its pages and its first member; `rows`, the members' token rows group
-// by group; per token row the pages that are its prefix (0: none), its group (-1: none) and its place among the group's members; the token rows in
-// the order in which their own pages are read, most pages first.
+// by group; per token row the pages that are its prefix (0: none), its group (-1: none) and its place among the group's
+// members; the token rows in the order in which their own pages are read, most pages first.
 // A group's members are cut into tiles of equal size; the units of work are the pages of (group, tile, kv head) in that order, and
 // run c takes `per` of them from c per on.  The part that run c leaves of a (tile, kv head) begins at row row0 + 128 c, with row0
 // the rows of all (tile, kv head)s before: later parts are later in c or in row0, and 128 is the most a part has, so no two
@@ -817,7 +818,8 @@ int launch_shared(const CUtensorMap& tk, const CUtensorMap& tv, int ntok, const 
 }  // namespace
 
 // Decode attention (see gg_attn_decode_tma) of a step with shared prefixes: plan as at SharedArgs; runs (1 to 296): CTAs over
-// the prefixes; shares (1 to 64): CTAs that share a row's own pages; part: scratch of (nq ntok (1 + shares) + 128 runs) (dv + 2) + 4 ntok nkv floats, on a 32-byte boundary.
+// the prefixes; shares (1 to 64): CTAs that share a row's own pages; part: scratch of (nq ntok (1 + shares) + 128 runs) (dv + 2) + 4
+// ntok nkv floats, on a 32-byte boundary.
 // status: codes 71-79 (prefixes), 11 and 12 (own pages) name the wait that ran out.
 //
 // The arguments come packed, eight bytes each (see gg_shape_logits).
