@@ -86,6 +86,7 @@ def plan_shared_batches(prompt_lens: Sequence[int], sources: Sequence[int], max_
         raise ValueError("max_batch must be positive")
     batches: List[List[int]] = []
     cur: List[int] = []
+    held = set()                      # the sources of the requests in `cur`
     used = 0
     for i, n in enumerate(prompt_lens):
         if n <= 0:
@@ -96,11 +97,12 @@ def plan_shared_batches(prompt_lens: Sequence[int], sources: Sequence[int], max_
         alone = max(1, pages - min(prefix_tokens, n) // page_size)          # (a slot for itself is counted as a page, too)
         if alone * page_size > capacity_tokens:
             raise ValueError(f"request {i}: needs room for {alone * page_size} tokens but the cache holds {capacity_tokens}")
-        need = max(1, pages - n // page_size) if sources[i] in cur else alone
+        need = max(1, pages - n // page_size) if sources[i] in held else alone
         if cur and (len(cur) >= max_batch or (used + need) * page_size > capacity_tokens):
             batches.append(cur)
-            cur, used, need = [], 0, alone
+            cur, held, used, need = [], set(), 0, alone
         cur.append(i)
+        held.add(sources[i])
         used += need
     if cur:
         batches.append(cur)

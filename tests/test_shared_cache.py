@@ -298,3 +298,16 @@ def test_penalties_biases_and_a_grammar_in_the_loop():
         run(presence_penalty=float("inf"))
     with pytest.raises(ValueError):
         run(grammar=TokenGrammar.from_rows(V + 1, [{0: 0}]))
+
+
+def test_answers_beyond_one_batch_share_in_every_batch():
+    """A prompt counts once in every batch that holds answers to it, not only in the one with its first answer."""
+    plan = plan_shared_batches([2048] * 128, [0] * 128, 64, 64, 200 * 64, 64, 40960)
+    assert [len(b) for b in plan] == [64, 64]
+    # two prompts in turn: the second batch begins in the middle of one
+    plan = plan_shared_batches([640] * 8, [0] * 4 + [4] * 4, 10, 3, 64 * 25, 64, 1000)
+    assert plan == [[0, 1, 2], [3, 4, 5], [6, 7]]
+    st = ScriptedStepper(max_tokens=64 * 20, max_slots=8)
+    out = Generator(st, V, 1000, max_batch=4).generate([list(range(10)) * 64], GenerateParams(max_tokens=4, answers=12))
+    assert len(out) == 12 and all(r.tokens == [10, 11, 12, 13] for r in out)
+    assert [s for s in st.steps if s[0] == 640] == [[640]] * 3 and st.cache.live_slots == 0
