@@ -94,7 +94,9 @@ def plan_shared_batches(prompt_lens: Sequence[int], sources: Sequence[int], max_
         if n > context:
             raise ValueError(f"request {i}: prompt of {n} tokens exceeds the context of {context}")
         pages = -(-min(n + max(max_new, 0), context) // page_size)
-        alone = max(1, pages - min(prefix_tokens, n) // page_size)          # (a slot for itself is counted as a page, too)
+        # (a prompt that is the prefix itself gives its last token back, and the page it then writes to is its own; a slot for itself
+        # is counted as a page, too)
+        alone = max(1, pages - min(prefix_tokens, n - 1) // page_size)
         if alone * page_size > capacity_tokens:
             raise ValueError(f"request {i}: needs room for {alone * page_size} tokens but the cache holds {capacity_tokens}")
         need = max(1, pages - n // page_size) if sources[i] in held else alone

@@ -311,3 +311,20 @@ def test_answers_beyond_one_batch_share_in_every_batch():
     out = Generator(st, V, 1000, max_batch=4).generate([list(range(10)) * 64], GenerateParams(max_tokens=4, answers=12))
     assert len(out) == 12 and all(r.tokens == [10, 11, 12, 13] for r in out)
     assert [s for s in st.steps if s[0] == 640] == [[640]] * 3 and st.cache.live_slots == 0
+
+
+@pytest.mark.parametrize("answers", [1, 2])
+def test_prompts_that_are_a_prefix_of_whole_pages(answers):
+    """They give their last token back, and write it to a page of their own: it is counted."""
+    st = ScriptedStepper(max_tokens=64 * 6)
+    g = Generator(st, V, 1000)
+    from gogguf_b200.engine.step import StepEntry
+    slot = st.cache.open()
+    prefix = [k % V for k in range(128)]
+    st.step([StepEntry(slot, prefix)])
+    out = g.generate([list(prefix) for _ in range(4)], GenerateParams(max_tokens=10, answers=answers, stop_token_ids=[]), prefix=slot)
+    assert [r.tokens for r in out] == [[(prefix[-1] + 1 + k) % V for k in range(10)]] * (4 * answers)
+    assert st.cache.live_slots == 1 and st.cache.length(slot) == 128 and tuple(st.cache.groups[0].more_holders) == ()
+    # one of its own for the last token, one for what follows
+    assert plan_shared_batches([128] * 4, [0, 1, 2, 3], 10, 8, 64 * 4, 64, 1000, prefix_tokens=128) == [[0, 1], [2, 3]]
+    assert plan_shared_batches([129] * 4, [0, 1, 2, 3], 10, 8, 64 * 4, 64, 1000, prefix_tokens=128) == [[0, 1, 2, 3]]
