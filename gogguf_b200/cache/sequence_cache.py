@@ -585,19 +585,23 @@ class SequenceCache:
             raise CacheError(f"slot {slot} is not open")
         return self.lengths[slot]
 
+    def can_truncate(self, slot: int, length: int) -> bool:
+        """What `truncate` would return; changes nothing."""
+        cur = self.length(slot)
+        if length < 0 or length > cur:
+            raise CacheError(f"slot {slot} holds {cur} tokens, cannot be cut to {length}")
+        return length == cur or all(st.can_shorten(slot, length) for st in self.stores)
+
     def truncate(self, slot: int, length: int) -> bool:
         """Shorten an open sequence to its first `length` tokens (a conversation that is rolled back,
         a sequence that ran one step further than its result).  Returns False and changes nothing
         where that cannot be done: a windowed group has already given back a page that the shorter
         sequence's next token reads, or a layer keeps a fixed-size state, in which all tokens are
         folded together.  The caller then starts the sequence again."""
-        cur = self.length(slot)
-        if length < 0 or length > cur:
-            raise CacheError(f"slot {slot} holds {cur} tokens, cannot be cut to {length}")
-        if length == cur:
-            return True
-        if not all(st.can_shorten(slot, length) for st in self.stores):
+        if not self.can_truncate(slot, length):
             return False
+        if length == self.lengths[slot]:
+            return True
         for st in self.stores:
             st.shorten(slot, length)
         self.lengths[slot] = length

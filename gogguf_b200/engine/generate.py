@@ -79,9 +79,10 @@ def plan_batches(prompt_lens: Sequence[int], max_new: int, max_batch: int, capac
 
 
 def plan_shared_batches(prompt_lens: Sequence[int], sources: Sequence[int], max_new: int, max_batch: int, capacity_tokens: int,
-                        page_size: int, context: int, prefix_tokens: int = 0) -> List[List[int]]:
+                        page_size: int, context: int, prefix_tokens: int = 0, prefix_cut: bool = True) -> List[List[int]]:
     """`plan_batches` where request i has the prompt of request `sources[i]` (<= i) and all prompts begin with `prefix_tokens`
-    tokens that the cache holds already: the whole pages of a prompt are counted once in a batch, those of the prefix not at all."""
+    tokens that the cache holds already: the whole pages of a prompt are counted once in a batch, those of the prefix not at all.
+    `prefix_cut`: the prefix can give its last token back; where it cannot, a prompt that is no longer than it is run for itself."""
     if max_batch <= 0:
         raise ValueError("max_batch must be positive")
     batches: List[List[int]] = []
@@ -96,7 +97,8 @@ def plan_shared_batches(prompt_lens: Sequence[int], sources: Sequence[int], max_
         pages = -(-min(n + max(max_new, 0), context) // page_size)
         # (a prompt that is the prefix itself gives its last token back, and the page it then writes to is its own; a slot for itself
         # is counted as a page, too)
-        alone = max(1, pages - min(prefix_tokens, n - 1) // page_size)
+        shared = min(prefix_tokens, n - 1) if prefix_cut or n > prefix_tokens else 0
+        alone = max(1, pages - shared // page_size)
         if alone * page_size > capacity_tokens:
             raise ValueError(f"request {i}: needs room for {alone * page_size} tokens but the cache holds {capacity_tokens}")
         need = max(1, pages - n // page_size) if sources[i] in held else alone
@@ -195,8 +197,9 @@ class Generator:
         results: List[Optional[GenerationResult]] = [None] * len(prompts)
         lens = [len(p) for p in prompts]
         if (answers > 1 or prefix is not None) and self.cache.can_fork:
+            have = self.cache.length(prefix) if prefix is not None else 0
             batches = plan_shared_batches(lens, sources, max_new, self.max_batch, self._room(held), self.cache.page_size, self.context,
-                                          self.cache.length(prefix) if prefix is not None else 0)
+                                          have, have == 0 or self.cache.can_truncate(prefix, have - 1))
         else:
             batches = plan_batches(lens, max_new, self.max_batch, self._room(held), self.cache.page_size, self.context)
             sources = list(range(len(prompts)))

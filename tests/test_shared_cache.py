@@ -328,3 +328,23 @@ def test_prompts_that_are_a_prefix_of_whole_pages(answers):
     # one of its own for the last token, one for what follows
     assert plan_shared_batches([128] * 4, [0, 1, 2, 3], 10, 8, 64 * 4, 64, 1000, prefix_tokens=128) == [[0, 1], [2, 3]]
     assert plan_shared_batches([129] * 4, [0, 1, 2, 3], 10, 8, 64 * 4, 64, 1000, prefix_tokens=128) == [[0, 1, 2, 3]]
+
+
+def test_a_prefix_that_cannot_be_cut_back_is_run_again_by_prompts_that_are_it():
+    """A state in which all tokens are folded together cannot give the last one back: such a prompt shares nothing, and is planned so."""
+    st = ScriptedStepper(max_tokens=64 * 6, state=True)
+    g = Generator(st, V, 1000)
+    from gogguf_b200.engine.step import StepEntry
+    slot = st.cache.open()
+    prefix = [k % V for k in range(128)]
+    st.step([StepEntry(slot, prefix)])
+    run = dict(params=GenerateParams(max_tokens=10, stop_token_ids=[]), prefix=slot)
+    out = g.generate([list(prefix) for _ in range(3)], **run)
+    assert [r.tokens for r in out] == [[(prefix[-1] + 1 + k) % V for k in range(10)]] * 3
+    assert [s for s in st.steps if s[0] == 128] == [[128]] * 4
+    # prompts that go on from it do share it
+    out = g.generate([prefix + [k] for k in range(3)], **run)
+    assert [r.tokens[0] for r in out] == [1, 2, 3] and [1, 1, 1] in st.steps and st.cache.live_slots == 1
+    with pytest.raises(CacheError):
+        st.cache.can_truncate(slot, 129)
+    assert st.cache.can_truncate(slot, 128) and not st.cache.can_truncate(slot, 127) and st.cache.length(slot) == 128
