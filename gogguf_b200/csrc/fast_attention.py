@@ -153,12 +153,13 @@ class PrefixPlan:
         self.longest = max((pages for _, pages in self.groups), default=0)
 
     def pays(self, nkv: int) -> bool:
-        """`prefix_pays` of this plan's groups (True where they are not known), worked out once."""
-        if self._pays[0] != nkv:
+        """`prefix_pays` of this plan's groups (True where they are not known, or where the plan's maker has found so), worked out once."""
+        if not self.found and self._pays[0] != nkv:
             self._pays = (nkv, self.groups is None or prefix_pays(self.groups, self.n_tokens, nkv))
         return self._pays[1]
 
     _pays = (0, True)             # kv heads, and the answer for them
+    found = False                 # what shares was chosen because it pays
 
     @staticmethod
     def words_for(n_tokens: int) -> int:
@@ -166,14 +167,17 @@ class PrefixPlan:
 
     @classmethod
     def over(cls, words: torch.Tensor, n_tokens: int, own_pages: Optional[int] = None,
-             groups: Optional[Sequence[Tuple[int, int]]] = None) -> "PrefixPlan":
+             groups: Optional[Sequence[Tuple[int, int]]] = None, found: bool = False) -> "PrefixPlan":
         """A plan whose words are (or will be) on the device already, packed by `pack`; `groups`: (members, pages) of those it will
-        hold, and `own_pages`, the most that a row reads beside them, choose the launch (any others are right, too)."""
+        hold, and `own_pages`, the most that a row reads beside them, choose the launch (any others are right, too).  `found`: the
+        groups were chosen because reading them together pays, so that is not asked again (the rows that fill up a captured step
+        would be counted)."""
         plan = cls.__new__(cls)
         if words.dtype != torch.int32 or words.numel() != cls.words_for(n_tokens) or not words.is_contiguous():
             raise KernelError(f"shared attention: a plan of {n_tokens} tokens has {cls.words_for(n_tokens)} int32 words")
         plan.n_tokens, plan.words, plan.own_pages, plan.groups = (
             n_tokens, words, own_pages, None if groups is None else list(groups))
+        plan.found = bool(found)
         plan.longest = max((pages for _, pages in plan.groups or ()), default=0)
         return plan
 

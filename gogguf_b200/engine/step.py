@@ -219,7 +219,7 @@ class Stepper:
         if prefixes is None:
             return {}
         from ..csrc.fast_attention import PrefixPlan
-        return {g: PrefixPlan.over(lay.view(dev, f"prefix{g}"), lay.n_seqs, prefixes.own_pages, [(len(r), pages) for r, pages in gs])
+        return {g: PrefixPlan.over(lay.view(dev, f"prefix{g}"), lay.n_seqs, prefixes.own_pages, [(len(r), pages) for r, pages in gs], found=True)
                 for g, gs in prefixes.groups.items()}
 
     def build_context(self, entries: Sequence[StepEntry], host: Optional[torch.Tensor] = None,
