@@ -106,6 +106,14 @@ def shared_runs(groups: Sequence[Tuple[int, int]], nq: int, nkv: int) -> int:
     return min(SHARED_RUNS // 2, -(-units // 4)) or SHARED_RUNS // 2
 
 
+def step_launch(groups: Sequence[Tuple[int, int]], own_pages: int, n_tokens: int, nq: int, nkv: int) -> Tuple[int, int]:
+    """(runs, shares) of a model's step: `shared_runs` up to a power of two (or all SMs, or two a SM), and `shared_shares` of the own pages
+    down to one, so that a captured step is the same launch for prompts of about a length and while answers grow."""
+    runs, half = shared_runs(groups, nq, nkv), SHARED_RUNS // 2
+    runs = SHARED_RUNS if runs > half else min(half, 1 << (runs - 1).bit_length())
+    return runs, shared_shares(n_tokens, nkv, 1 << max(0, own_pages.bit_length() - 1))
+
+
 def shared_groups(table: np.ndarray, limits: Sequence[int]) -> List[Tuple[List[int], int]]:
     """The rows of a page table that read the same leading pages: [(rows, pages)], each with two rows and one page at least.
     `limits[r]`: how many leading pages of row r may be shared (those that lie wholly before its newest position).  A row is
@@ -158,8 +166,15 @@ class PrefixPlan:
             self._pays = (nkv, self.groups is None or prefix_pays(self.groups, self.n_tokens, nkv))
         return self._pays[1]
 
+    def launch(self, nq: int, nkv: int, width: int) -> Tuple[int, int]:
+        """(runs, shares) of a launch over a page table of `width` pages, where the caller does not choose them."""
+        if self.found:
+            return step_launch(self.groups or (), width if self.own_pages is None else self.own_pages, self.n_tokens, nq, nkv)
+        return (shared_runs(self.groups or (), nq, nkv),
+                shared_shares(self.n_tokens, nkv, width if self.own_pages is None else self.own_pages))
+
     _pays = (0, True)             # kv heads, and the answer for them
-    found = False                 # what shares was chosen because it pays
+    found = False                 # a model's step: what shares was chosen because it pays
 
     @staticmethod
     def words_for(n_tokens: int) -> int:
@@ -170,8 +185,8 @@ class PrefixPlan:
              groups: Optional[Sequence[Tuple[int, int]]] = None, found: bool = False) -> "PrefixPlan":
         """A plan whose words are (or will be) on the device already, packed by `pack`; `groups`: (members, pages) of those it will
         hold, and `own_pages`, the most that a row reads beside them, choose the launch (any others are right, too).  `found`: the
-        groups were chosen because reading them together pays, so that is not asked again (the rows that fill up a captured step
-        would be counted)."""
+        groups of a model's step, chosen because reading them together pays: that is not asked again (the rows that fill up a captured
+        step would be counted), and the launch is `step_launch`'s."""
         plan = cls.__new__(cls)
         if words.dtype != torch.int32 or words.numel() != cls.words_for(n_tokens) or not words.is_contiguous():
             raise KernelError(f"shared attention: a plan of {n_tokens} tokens has {cls.words_for(n_tokens)} int32 words")
@@ -242,7 +257,7 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
     that several rows share are read once for all of them, in three kernels, where that pays (`prefix_pays`; `together` True or
     False decides instead).  scratch: float32, `shared_scratch` of it; two launches that may run at the same time need scratch of
     their own.  runs: CTAs over the prefixes (default: `shared_runs`); shares: CTAs that share a row's own pages (default:
-    `shared_shares`)."""
+    `shared_shares`; `PrefixPlan.launch`)."""
     dv = d if dv is None else int(dv)
     T = plan.n_tokens
     if not takes(nq, nkv, d, dv):
@@ -291,17 +306,16 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
         attn_decode_tma(q, k_pool, v_pool, out, positions, seq_of_token, table, page_size, T, nq, nkv, d, scale, 0, splits, cluster=True,
                         sink=sink, out_scale=out_scale, dv=dv, gate=gate)
         return
-    if shares is None:
-        shares = shared_shares(T, nkv, width if plan.own_pages is None else plan.own_pages)
-    elif not 1 <= shares <= SHARED_SHARES:
+    if runs is None or shares is None:
+        launch = plan.launch(nq, nkv, width)
+        runs, shares = launch[0] if runs is None else runs, launch[1] if shares is None else shares
+    if not 1 <= runs <= SHARED_RUNS:
+        raise KernelError(f"shared attention: 1 to {SHARED_RUNS} runs, not {runs}")
+    if not 1 <= shares <= SHARED_SHARES:
         raise KernelError(f"shared attention: 1 to {SHARED_SHARES} shares, not {shares}")
     room = shared_scratch(T, nq, nkv, dv, shares)
     if scratch.numel() < room:
         raise KernelError(f"shared attention: scratch must have {room} elements")
-    if runs is None:
-        runs = shared_runs(plan.groups or (), nq, nkv)
-    elif not 1 <= runs <= SHARED_RUNS:
-        raise KernelError(f"shared attention: 1 to {SHARED_RUNS} runs, not {runs}")
     kernel("attention_shared", "gg_attn_decode_shared")(_SHARED_CALL(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), table.data_ptr(),
         width, page_size, pools, words.data_ptr(), T, nq, nkv, d, dv, runs, shares, p_sink, p_gate, ldg, scratch.data_ptr(), scratch.numel(),

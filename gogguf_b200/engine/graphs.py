@@ -20,7 +20,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from ..parts.base import Workspace
-from .step import StepEntry, StepLayout, Stepper
+from .step import SharedPrefixes, StepEntry, StepLayout, Stepper
 
 BATCH_BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)
 
@@ -50,15 +50,26 @@ class GraphStepper(Stepper):
     def __init__(self, model, cache, min_width: int = 16):
         super().__init__(model, cache)
         self.min_width = min_width
-        self._graphs: Dict[Tuple, _Captured] = {}       # by batch bucket, width bucket and what the sequences share
+        self._graphs: Dict[Tuple, _Captured] = {}       # by batch bucket, width bucket and the launches over shared pages
         self.replays = 0
         # a part that reads back to the host or allocates while it runs declares `capturable = False`;
         # such a model is stepped eagerly, and `decode_from_device` is not offered for it
         self.capturable = all(getattr(p, "capturable", True) for p in model.parts())
+        # (query heads, kv heads) of the layers whose attention may read shared pages together
+        self._heads = sorted({(p.nq, p.nkv) for p in model.parts() if getattr(p, "_fast", None) is not None and hasattr(p, "nkv")})
 
     def _width_bucket(self, slots: Sequence[int]) -> int:
         w = max(self.cache.table_width(slots), self.min_width)
         return 1 << (w - 1).bit_length()
+
+    def prefix_key(self, prefixes: SharedPrefixes, n_tokens: int) -> Tuple:
+        """What the launches of a captured step with these prefixes depend on, by KV group (its plans' words may say anything)."""
+        from ..csrc.fast_attention import step_launch
+        key = []
+        for g, gs in sorted(prefixes.groups.items()):
+            weights, nkv = [(len(rows), pages) for rows, pages in gs], self.cache.groups[g].request.num_kv_heads
+            key.append((g,) + tuple(step_launch(weights, prefixes.own_pages, n_tokens, nq, n) for nq, n in self._heads if n == nkv))
+        return tuple(key)
 
     def _capture(self, entries: Sequence[StepEntry], bucket: int, width: int, prefixes=None) -> _Captured:
         dev_t = self.model.rt.device
@@ -150,7 +161,7 @@ class GraphStepper(Stepper):
     def _replay(self, entries, slots, counts, bucket, sampled, rows):
         width = self._width_bucket(slots)
         prefixes = self.shared_prefixes(slots)
-        key = (bucket, width) if prefixes is None else (bucket, width, prefixes.key())
+        key = (bucket, width) if prefixes is None else (bucket, width, self.prefix_key(prefixes, bucket))
         cap = self._graphs.get(key)
         if cap is None:
             cap = self._graphs[key] = self._capture(entries, bucket, width, prefixes)

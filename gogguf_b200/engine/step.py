@@ -98,11 +98,6 @@ class SharedPrefixes:
     def own_pages(self) -> int:
         return max(max(have) for have in self.own.values())
 
-    def key(self) -> Tuple:
-        """What a captured step's launches depend on: the groups' weight and the own pages, each up to a power of two."""
-        return tuple((g, sum(len(rows) * pages for rows, pages in gs).bit_length()) for g, gs in sorted(self.groups.items())) + (
-            self.own_pages.bit_length(),)
-
 
 class StepLayout:
     """Packs the integer inputs of a step into one host buffer and one device buffer."""

@@ -1,4 +1,5 @@
-"""Steps of sequences that share pages: whether sharing pays is decided once (no GPU)."""
+"""Steps of sequences that share pages: whether sharing pays is decided once, and a captured step is found by what its launches
+depend on (no GPU)."""
 import types
 
 import pytest
@@ -71,3 +72,42 @@ def test_the_decision_is_made_once(rows, bucket):
     assert plan_of(st, prefixes, bucket).pays(NKV)
     c, slots = forks(rows, 64 * (pages - 1))
     assert Recorded(c).decode(slots) is None
+
+
+def test_captures_of_answers_that_grow():
+    """64 answers of 500 tokens to a prompt of 2,048: a graph for each width of the table."""
+    c, slots = forks(64, 2048)
+    st = Recorded(c)
+    widths = set()
+    for _ in range(500):
+        assert st.decode(slots) is not None
+        widths.add(st._width_bucket(slots))
+    assert len(st.captured) == len(widths) == 1, [(b, w, p.own_pages) for b, w, p in st.captured]
+
+
+def test_a_graph_serves_the_launch_it_was_captured_for():
+    """Steps that are answered by one graph have the same launches, and those are what their plans ask for."""
+    seen = {}
+    for rows, pages in ((5, 60), (5, 100), (7, 64), (8, 70), (6, 130), (8, 256)):
+        c, slots = forks(rows, 64 * pages)
+        st = Recorded(c)
+        for k in range(1200):
+            prefixes = st.decode(slots)
+            if prefixes is None or k % 37:
+                continue
+            plan = plan_of(st, prefixes, 8)
+            key, launch = st.prefix_key(prefixes, 8), plan.launch(NQ, NKV, 512)
+            assert (8, st._width_bucket(slots), key) in st._graphs and seen.setdefault(key, launch) == launch
+            assert 1 <= launch[0] <= A.SHARED_RUNS and 1 <= launch[1] <= A.SHARED_SHARES
+    assert len(set(seen.values())) == len(seen)
+
+
+def test_layers_with_other_numbers_of_heads():
+    """The key holds the launches of every number of query heads on a group's kv heads, and of no other."""
+    c, slots = forks(64, 64 * 12)
+    one, two, other = (Recorded(c, heads=h) for h in (((32, NKV),), ((32, NKV), (128, NKV)), ((32, NKV), (32, 4))))
+    prefixes = one.shared_prefixes(slots)
+    a, b, o = (st.prefix_key(prefixes, 64) for st in (one, two, other))
+    assert a == o and a != b
+    # 64 members are two tiles of 128 rows with four heads each, eight with sixteen: 192 and 768 pages of (tile, kv head), four a run
+    assert A.step_launch([(64, 12)], 1, 64, 32, NKV)[0] == 64 and A.step_launch([(64, 12)], 1, 64, 128, NKV)[0] == A.SHARED_RUNS // 2
