@@ -348,7 +348,9 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
                     tc5::ld32(S_t + lane_off + (uint32_t)(s * 64), sr);
                     tc5::ld32(S_t + lane_off + (uint32_t)(s * 64) + 32, sr + 32);
                     tc5::wait_ld();
-                    // P = 2^(score scale - maximum in use) as bfloat16 pairs; returns the sum of the page's P
+                    // P = 2^(score scale - maximum in use) as bfloat16 pairs; returns the sum of the page's P, as they are rounded: the
+                    // maximum in use is an old one, so a row's largest weight is not a power of two, and a row that looks at
+                    // one key gets that key's value only where both sums hold the same weight.
                     auto exponentials = [&]() -> float {
                         const float mu = m_used == -INFINITY ? 0.f : m_used;
                         const unsigned long long sc2 = pack2(scale_log2, scale_log2), nmu2 = pack2(-mu, -mu);
@@ -357,9 +359,8 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
                         for (int e = 0; e < 32; ++e) {
                             float x0, x1;
                             unpack2(fma2(pack2(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1])), sc2, nmu2), x0, x1);
-                            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-                            l4[e & 3] = add2(l4[e & 3], pack2(p0, p1));
-                            pk[e] = pack_bf16(p0, p1);
+                            pk[e] = pack_bf16(fast_exp2(x0), fast_exp2(x1));
+                            l4[e & 3] = add2(l4[e & 3], pack2(__uint_as_float(pk[e] << 16), __uint_as_float(pk[e] & 0xffff0000u)));
                         }
                         float la, lb;
                         unpack2(add2(add2(l4[0], l4[1]), add2(l4[2], l4[3])), la, lb);
