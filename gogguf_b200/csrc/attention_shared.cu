@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(256, 2) shared_prefix_kernel(const __grid_cons
     const uint32_t S_t = *tmem_slot, O_t = S_t + 128;
     // (a shared-memory base off the 1024-byte boundary would corrupt the swizzled tiles: refuse and say so)
     bool ok = (tma::smem_u32(smem) & 1023u) == 0;
-    if (!ok && threadIdx.x == 0) atomicCAS(status, 0, 29);
+    if (!ok && threadIdx.x == 0) atomicCAS(status, 0, 70);
 
     // The run is cut where the (tile, kv head) changes.  Every role walks the same cuts.
     struct Piece { int first, members, head, page0, pages, lead, all_first, all_members; size_t row0; };
@@ -821,7 +821,7 @@ int launch_shared(const CUtensorMap& tk, const CUtensorMap& tv, int ntok, const 
 // Decode attention (see gg_attn_decode_tma) of a step with shared prefixes: plan as at SharedArgs; runs (1 to 296): CTAs over
 // the prefixes; shares (1 to 64): CTAs that share a row's own pages; part: scratch of (nq ntok (1 + shares) + 128 runs) (dv + 2) + 4
 // ntok nkv floats, on a 32-byte boundary.
-// status: codes 71-79 (prefixes), 11 and 12 (own pages) name the wait that ran out.
+// status: codes 71-79 (prefixes), 11 and 12 (own pages) name the wait that ran out; 70: shared memory off its boundary.
 //
 // The arguments come packed, eight bytes each (see gg_shape_logits).
 struct SharedCall {
@@ -887,7 +887,7 @@ GG_API gg_attn_decode_shared(const void* call, cudaStream_t stream) {
 #undef GG_SHARED
     if (rc != 0) return rc;
     const AttnShape sh = {d, dv, 0, (const bf16*)gate, ldg};
-    // half warps a row: as many as fill the device once (a part read behind another takes 1 us longer), eight CTAs of 16 an SM
+    // half warps a row: as many as give each SM four CTAs of 16, at most (a part read behind another takes 1 us longer)
     int team = 1;
     while (team < JOIN_HALVES && (long long)ntok * nq * team * 2 <= 148 * 4 * JOIN_HALVES) team *= 2;
     const long long halves = (long long)ntok * nq * team;

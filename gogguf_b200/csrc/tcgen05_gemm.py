@@ -40,6 +40,10 @@ def check_status(device: torch.device) -> None:
                    54: "attn_decode_shared"}[v]
             raise KernelError(f"debug build: kernel {who} met a page-table index or page id out of range (code {v}); "
                               "it read page 0 (a reader) or wrote nothing (a writer), results of that step are invalid")
+        if v in (29, 69, 70):
+            who = {29: "attn_prefill_tc", 69: "mixed_head_attention", 70: "attn_decode_shared"}[v]
+            raise KernelError(f"{who} refused a shared memory that does not begin on a 1,024-byte boundary (code {v}); "
+                              "results of that step are invalid")
         raise KernelError(f"a bounded wait inside a kernel ran out (code {v}: 1 TMA producer, 2 MMA issuer, "
                           "3 epilogue of a product, 11-12 decode attention, 21-28 prefill attention, 61-68 prefill attention "
                           "with mixed heads, 71-79 a shared prefix); "
