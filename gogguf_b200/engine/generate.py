@@ -283,7 +283,7 @@ class Generator:
                      and getattr(logits, "is_cuda", False) and len(live) <= 256 and not params.keep_logits)
             kept = {i: [] for i in batch} if params.keep_logits else None
             if ahead:
-                sampler.begin(live, [prompts[i] for i in live], logits.device)     # rings for a repeat penalty
+                sampler.begin(live, [prompts[i] for i in live], logits.device, max_new)     # rings for penalties
             if ahead and sampler.device_only:
                 self._decode_one_ahead(live, logits, sampler, slots, generated, prompts, params, max_new, stop, results,
                                        held)

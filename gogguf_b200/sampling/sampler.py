@@ -197,17 +197,18 @@ class Sampler:
         """True when every row can be sampled by kernels alone (with a repeat penalty: after `begin`)."""
         return self.on_device and (not (self.penalised or self.shaped) or self._rings is not None)
 
-    def begin(self, streams: Sequence[int], prompts: Sequence[Sequence[int]], device) -> None:
+    def begin(self, streams: Sequence[int], prompts: Sequence[Sequence[int]], device, most: Optional[int] = None) -> None:
         """Put the last `repeat_last_n` ids of each request's prompt on the device, one ring per request, so
         that the penalty can be applied, and every sampled id appended, without the host.  Only needed (and
-        only done) with a repeat penalty and a configuration whose sampling runs on the device."""
+        only done) with a repeat penalty and a configuration whose sampling runs on the device.  `most`: ids that
+        a request may make at most, where that is known (a ring need not be longer than what can come)."""
         if not ((self.penalised or self.shaped) and self.on_device):
             return
         n, rows = self.repeat_last_n, len(streams)
         if self.shaped:
             if not ShapingState.advances(self.shaping):
                 return
-            self._state = ShapingState(self.shaping, prompts, [()] * rows, device)
+            self._state = ShapingState(self.shaping, prompts, [()] * rows, device, most)
             self._rings = ()
             self._ring_rows = self._ring_pairs(rows, device)
             self._ring_of = {int(s): r for r, s in enumerate(streams)}
@@ -383,7 +384,7 @@ class FunctionSampler:
     def shaped(self) -> bool:
         return self.shaping is not None
 
-    def begin(self, streams, prompts, device) -> None:
+    def begin(self, streams, prompts, device, most=None) -> None:
         pass
 
     def sample(self, logits: torch.Tensor, streams: Sequence[int], steps: Sequence[int],

@@ -90,10 +90,15 @@ class ShapingState:
         """Can a state follow the drawn ids on the device?  Not where the window has no end."""
         return shaping.last_n > 0 or not shaping.counts
 
-    def __init__(self, shaping: LogitShaping, histories: Sequence[Sequence[int]], generated: Sequence[Sequence[int]], device):
+    def __init__(self, shaping: LogitShaping, histories: Sequence[Sequence[int]], generated: Sequence[Sequence[int]], device,
+                 most: Optional[int] = 0):
+        """`most`: ids that may still join a request's history by `advance` (0: the state is made for a step; None: any number)."""
         self.shaping = shaping
-        # (a window below one is the whole history: as it is now, for states that are made for a step)
-        rows, n = len(histories), shaping.last_n if shaping.last_n > 0 else max([1] + [len(h) for h in histories])
+        # (a window is no longer than what it can hold, and one below one is the whole history)
+        rows, n = len(histories), shaping.last_n
+        if n < 1 or most is not None:
+            held = max([1] + [len(h) + (most or 0) for h in histories])
+            n = held if n < 1 else min(n, held)
         self.hist = self.hist_len = self.hist_pos = None
         if shaping.counts:
             hist = np.full((rows, n), -1, dtype=np.int32)
