@@ -26,7 +26,7 @@ from typing import List, Optional, Sequence
 import numpy as np
 import torch
 
-from .shaping import LogitShaping, ShapingState, shape_host
+from .shaping import GrammarWalks, LogitShaping, ShapingState, shape_host
 
 _M64 = (1 << 64) - 1
 
@@ -175,6 +175,9 @@ class Sampler:
         self.cfg = cfg
         self.shaping = shaping    # penalties, biases and a grammar; the repeat penalty is then part of it
         self._state = None        # what of it is on the device (`begin`)
+        self._walks = GrammarWalks(shaping.grammar if shaping is not None else None)
+        self._biases = {}         # (rows, device) of the last step that was waited for -> its biases there
+        self._plain = {}          # (vocabulary, device) -> what draws from rows that are shaped already
         # The chain with a top-k has a kernel as long as the slices' candidates fit its shared memory (top-k
         # 1,024 up to a vocabulary of 163,840); beyond that the host chain takes the rows, as it does for
         # every configuration without a kernel.
@@ -347,19 +350,19 @@ class Sampler:
         if not rows:
             return []
         made = [list(h)[len(h) - k:] for h, k in zip(histories, steps)]
+        states = self._walks.states(streams, made)
         if logits.is_cuda:
-            state = ShapingState(self.shaping, histories[:rows], made, logits.device)
+            state = ShapingState(self.shaping, histories[:rows], made, logits.device, states=states, bias=self._biases.get((rows, logits.device)))
+            self._biases = {(rows, logits.device): state.bias}
             x = state.apply(logits, None, rows, out=torch.empty((rows, logits.shape[1]), dtype=torch.float32, device=logits.device))
         else:
             x = logits[:rows].detach().to(torch.float32).clone()
             for r in range(rows):
-                shape_host(x[r].numpy(), self.shaping, histories[r], made[r])
-        plain = Sampler(self.cfg, vocab_size=logits.shape[1])
-        got = plain.sample(x, streams, steps)
-        if self.shaping.grammar is not None:
-            g = self.shaping.grammar
-            got = [t if g.step(g.walk(m), int(t)) >= 0 else -1 for t, m in zip(got, made)]
-        return got
+                shape_host(x[r].numpy(), self.shaping, histories[r], made[r], states[r])
+        kind = (logits.shape[1], logits.device)
+        if kind not in self._plain:
+            self._plain[kind] = Sampler(self.cfg, vocab_size=logits.shape[1])
+        return self._walks.keep(states, self._plain[kind].sample(x, streams, steps))
 
 
 class FunctionSampler:
@@ -373,6 +376,7 @@ class FunctionSampler:
     def __init__(self, fn, repeat_penalty: float = 1.0, repeat_last_n: int = 64, shaping: Optional[LogitShaping] = None):
         self.fn = fn
         self.shaping = shaping
+        self._walks = GrammarWalks(shaping.grammar if shaping is not None else None)
         self.repeat_penalty = float(repeat_penalty)
         self.repeat_last_n = int(repeat_last_n) if repeat_last_n else 64
 
@@ -391,22 +395,20 @@ class FunctionSampler:
                histories: Optional[Sequence[Sequence[int]]] = None) -> List[int]:
         rows = len(streams)
         host = logits[:rows].detach().to("cpu", torch.float32).numpy()
-        res = []
+        res, made, states = [], [], []
+        if self.shaped:
+            if histories is None:
+                raise ValueError("penalties, biases and grammars need the rows' histories")
+            made = [list(h)[len(h) - k:] for h, k in zip(histories, steps)]
+            states = self._walks.states(streams, made)
         for r in range(rows):
             row = host[r].copy()
             if self.penalised and histories is not None:
                 apply_repeat_penalty(row, histories[r], self.repeat_penalty, self.repeat_last_n)
-            made = ()
             if self.shaped:
-                if histories is None:
-                    raise ValueError("penalties, biases and grammars need the rows' histories")
-                made = list(histories[r])[len(histories[r]) - steps[r]:]
-                shape_host(row, self.shaping, histories[r], made)
-            t = int(self.fn(row))
-            if self.shaped and self.shaping.grammar is not None and self.shaping.grammar.walk(made + [t]) < 0:
-                t = -1
-            res.append(t)
-        return res
+                shape_host(row, self.shaping, histories[r], made[r], states[r])
+            res.append(int(self.fn(row)))
+        return self._walks.keep(states, res) if self.shaped else res
 
 
 def make_sampler(sampler, repeat_penalty: float = 1.0, repeat_last_n: int = 64, vocab_size: Optional[int] = None,

@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -66,8 +66,38 @@ class LogitShaping:
         return self.grammar.walk(generated) if self.grammar is not None else -1
 
 
-def shape_host(row: np.ndarray, shaping: LogitShaping, history: Sequence[int], generated: Sequence[int]) -> None:
-    """One row of float32 logits, in place; `history` is prompt and generated ids."""
+class GrammarWalks:
+    """The states of a sampler's rows, from one step to the next: where a stream's ids begin with those of its last step, only what
+    came after them is walked."""
+
+    def __init__(self, grammar: Optional[TokenGrammar]):
+        self.grammar = grammar
+        self._at: Dict[int, Tuple[List[int], int]] = {}          # stream -> (the ids walked, the state behind them)
+
+    def states(self, streams: Sequence[int], made: Sequence[List[int]]) -> List[int]:
+        """A state per row (-1 without a grammar, or where the row has left it)."""
+        if self.grammar is None:
+            return [-1] * len(made)
+        was, self._at, out = self._at, {}, []
+        for stream, ids in zip(streams, made):
+            known, state = was.get(stream, ([], self.grammar.start))
+            if ids[:len(known)] != known:
+                known, state = [], self.grammar.start
+            state = self.grammar.walk(ids[len(known):], state)
+            self._at[stream] = (ids, state)
+            out.append(state)
+        return out
+
+    def keep(self, states: Sequence[int], tokens: Sequence[int]) -> List[int]:
+        """`tokens` drawn in `states`, -1 in the place of one that is not allowed."""
+        if self.grammar is None:
+            return list(tokens)
+        return [t if self.grammar.step(s, int(t)) >= 0 else -1 for s, t in zip(states, tokens)]
+
+
+def shape_host(row: np.ndarray, shaping: LogitShaping, history: Sequence[int], generated: Sequence[int], state: Optional[int] = None) -> None:
+    """One row of float32 logits, in place; `history` is prompt and generated ids; `state`: the grammar's behind `generated`, where it is
+    known."""
     if shaping.counts:
         ids, times = np.unique(np.asarray(list(shaping.window(history)), dtype=np.int64), return_counts=True)
         inside = (ids >= 0) & (ids < row.size)
@@ -79,7 +109,7 @@ def shape_host(row: np.ndarray, shaping: LogitShaping, history: Sequence[int], g
     for t, b in shaping.bias:
         row[t] += np.float32(b)
     if shaping.grammar is not None:
-        row[~shaping.grammar.allowed(shaping.state_of(generated))] = -np.inf
+        row[~shaping.grammar.allowed(shaping.state_of(generated) if state is None else state)] = -np.inf
 
 
 class ShapingState:
@@ -91,8 +121,9 @@ class ShapingState:
         return shaping.last_n > 0 or not shaping.counts
 
     def __init__(self, shaping: LogitShaping, histories: Sequence[Sequence[int]], generated: Sequence[Sequence[int]], device,
-                 most: Optional[int] = 0):
-        """`most`: ids that may still join a request's history by `advance` (0: the state is made for a step; None: any number)."""
+                 most: Optional[int] = 0, states: Optional[Sequence[int]] = None, bias=None):
+        """`most`: ids that may still join a request's history by `advance` (0: the state is made for a step; None: any number);
+        `states`: the grammar's behind `generated`, where they are known; `bias`: that of a state for as many requests."""
         self.shaping = shaping
         # (a window is no longer than what it can hold, and one below one is the whole history)
         rows, n = len(histories), shaping.last_n
@@ -108,8 +139,8 @@ class ShapingState:
                 hist[r, :len(tail)] = tail
                 lens[r] = len(tail)
             self.hist, self.hist_len, self.hist_pos = (torch.from_numpy(a).to(device) for a in (hist, lens, lens % n))
-        self.bias = None
-        if shaping.bias:
+        self.bias = bias
+        if shaping.bias and bias is None:
             nb = len(shaping.bias)
             ids, values = zip(*shaping.bias)
             self.bias = (torch.arange(rows + 1, dtype=torch.int32, device=device) * nb,
@@ -119,7 +150,7 @@ class ShapingState:
         if shaping.grammar is not None:
             self.masks, self.classes, self.next = shaping.grammar.on(device)
             # (a sequence that has left the grammar is where nothing is allowed: beyond the table)
-            at = [shaping.state_of(g) for g in generated]
+            at = [shaping.state_of(g) for g in generated] if states is None else states
             self.states = torch.tensor([s if s >= 0 else shaping.grammar.states for s in at], dtype=torch.int32, device=device)
 
     def apply(self, logits: torch.Tensor, ring_rows: Optional[torch.Tensor], rows: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
