@@ -1,8 +1,9 @@
 """Which ids a sequence may go on with: a deterministic automaton over token ids.
 
 The ids are sorted into classes, and a table says which state follows a state and a class (-1: such an id is not allowed
-there), so that an automaton over a large vocabulary stays small: the vocabulary is kept once, not once per state.  The masks of
-allowed ids that the logits take (`csrc.kernels.shape_logits`) are made from it, one row of bits per state.  What builds an
+there), so that the automaton itself stays small: the vocabulary is kept once, not once per state.  The masks of
+allowed ids that the logits take (`csrc.kernels.shape_logits`) are made from it, one row of bits per state: on a device a grammar
+keeps a bit for every id and state while it lives (10,000 states of 151,936 ids: 190 MB).  What builds an
 automaton from a schema or a context-free grammar is outside this library; `from_rows` and `choices` build small ones."""
 from __future__ import annotations
 
@@ -99,14 +100,16 @@ class TokenGrammar:
     def masks(self) -> np.ndarray:
         """[states, words] int32: bit v % 32 of word v / 32 is set where id v is allowed."""
         words = -(-self.classes.size // 32)
-        bits = np.zeros((self.states, words * 32), dtype=np.uint8)
+        packed = np.zeros((self.states, words * 4), dtype=np.uint8)
         for s in range(self.states):
-            bits[s, :self.classes.size] = self.allowed(s)
-        return np.packbits(bits, axis=1, bitorder="little").view(np.int32).reshape(self.states, words)
+            row = np.packbits(self.allowed(s), bitorder="little")
+            packed[s, :row.size] = row
+        return packed.view(np.int32)
 
     def on(self, device) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """(masks, classes, next) on a device, made at the first call."""
         device = torch.device(device)
         if device not in self._on:
-            self._on[device] = tuple(torch.from_numpy(np.array(a)).to(device) for a in (self.masks(), self.classes, self.next))
+            self._on[device] = tuple(torch.from_numpy(a if a.flags.writeable else np.array(a)).to(device)
+                                     for a in (self.masks(), self.classes, self.next))
         return self._on[device]
