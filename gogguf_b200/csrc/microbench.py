@@ -938,10 +938,20 @@ def shared() -> None:
         out = torch.empty_like(xs[0])
         hist = torch.randint(0, V, (R, 64), dtype=torch.int32, device=dev)
         length = torch.full((R,), 64, dtype=torch.int32, device=dev)
-        masks = torch.randint(-2 ** 31, 2 ** 31 - 1, (min(R, 100), V // 32), dtype=torch.int32, device=dev)
-        states = torch.arange(R, dtype=torch.int32, device=dev) % masks.shape[0]
-        us = _time_graph(lambda i: K.shape_logits(xs[i % n], out, hist=hist, hist_len=length, repeat=1.1, frequency=0.2, masks=masks, mask_rows=states))
-        print(f"shaping {R:3d} rows of {V}, 64 last ids, a grammar: {us:6.1f} us {R * V * 8 / us / 1e6:5.2f} TB/s", flush=True)
+        # states that allow nearly all, about half and nearly none of the ids
+        bits = torch.randint(-2 ** 31, 2 ** 31, (3, min(R, 100), V // 32), dtype=torch.int64, device=dev).to(torch.int32)
+        states = torch.arange(R, dtype=torch.int32, device=dev) % bits.shape[1]
+        line = f"shaping {R:3d} rows of {V}, 64 last ids, a grammar that allows 7/8, 1/2, 1/8 of them: beside the logits / in place us"
+        for masks in (bits[0] | bits[1] | bits[2], bits[0], bits[0] & bits[1] & bits[2]):
+            us = [_time_graph(lambda i: K.shape_logits(xs[i % n], where, hist=hist, hist_len=length, repeat=1.1, frequency=0.2, masks=masks, mask_rows=states))
+                  for where in (out, None)]
+            line += f"  {us[0]:.1f} / {us[1]:.1f}"
+        print(line, flush=True)
+        tokens = torch.randint(0, V, (R,), dtype=torch.int32, device=dev)
+        classes, after = torch.zeros(V, dtype=torch.int32, device=dev), torch.zeros(bits.shape[1], 1, dtype=torch.int32, device=dev)
+        pos = torch.zeros(R, dtype=torch.int32, device=dev)
+        us = _time_graph(lambda i: K.shape_advance(tokens, None, R, hist, length, pos, states, classes, after))
+        print(f"what {R:3d} drawn ids change: {us:.1f} us", flush=True)
 
 
 def main() -> None:
