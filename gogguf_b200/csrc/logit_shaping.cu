@@ -80,7 +80,8 @@ __global__ void __launch_bounds__(THREADS, 6) shape_logits_kernel(const float* l
     const bool known = ring >= 0 && ring < rings;
     const int ids = known && s.hist != nullptr ? min(s.hist_len[ring], s.last_n) : 0;
     const int state = known && s.masks != nullptr ? s.mask_rows[ring] : -1;
-    const int b0 = known && s.bias_start != nullptr ? max(s.bias_start[ring], 0) : 0;
+    // (a start beyond the list is a list that is over: what is added to it below stays within 32 bits)
+    const int b0 = known && s.bias_start != nullptr ? min(max(s.bias_start[ring], 0), s.biases) : 0;
     const int b1 = known && s.bias_start != nullptr ? min(s.bias_start[ring + 1], s.biases) : 0;
     const int* h = s.hist + (size_t)ring * s.last_n;
     int first_id = -1, first_bias = -1;
