@@ -7,7 +7,6 @@ tensor that is not on a CUDA device, or a missing compiler, raises.
 from __future__ import annotations
 
 import ctypes
-import math
 import struct
 from operator import index
 from typing import List, Optional, Sequence, Tuple
@@ -1424,6 +1423,7 @@ def history_append(tokens: torch.Tensor, ring_rows: torch.Tensor, hist: torch.Te
 
 
 _SHAPE_CALL = struct.Struct("=11q3d8q").pack            # csrc/logit_shaping.cu: ShapeCall
+_F32_LEAST, _F32_MOST = 2.0 ** -149, (2.0 - 2.0 ** -23) * 2.0 ** 127
 
 
 def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, hist: Optional[torch.Tensor] = None,
@@ -1449,8 +1449,8 @@ def shape_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, hi
         R = index(rows)
     if R < 0 or R > have or out_rows < R or out_v != V or (R > 1 and (ld < V or ldo < V)):
         raise KernelError(f"shape_logits: {R} rows of logits {tuple(logits.shape)} into {tuple(out.shape)}")
-    if not (0 < repeat < math.inf and -math.inf < frequency < math.inf and -math.inf < presence < math.inf):
-        raise KernelError("shape_logits: repeat must be positive, and it, frequency and presence finite")
+    if not (_F32_LEAST <= repeat <= _F32_MOST and -_F32_MOST <= frequency <= _F32_MOST and -_F32_MOST <= presence <= _F32_MOST):
+        raise KernelError("shape_logits: repeat must be positive, and it, frequency and presence finite, as float32 numbers")
     if (hist is None) != (hist_len is None) or (masks is None) != (mask_rows is None):
         raise KernelError("shape_logits: hist goes with hist_len, masks with mask_rows")
     if R == 0 or V == 0:

@@ -19,6 +19,11 @@ import torch
 from .grammar import TokenGrammar
 
 
+def _finite(x: float) -> bool:
+    """Is x a finite number, and does it stay one in 32 bits?"""
+    return abs(x) <= float(np.finfo(np.float32).max)
+
+
 @dataclass(frozen=True)
 class LogitShaping:
     repeat: float
@@ -32,14 +37,14 @@ class LogitShaping:
     def of(cls, params, vocab_size: int) -> Optional["LogitShaping"]:
         """What a request's parameters ask for beyond the repeat penalty alone, or None."""
         frequency, presence = float(params.frequency_penalty), float(params.presence_penalty)
-        if not (math.isfinite(frequency) and math.isfinite(presence)):
-            raise ValueError("frequency_penalty and presence_penalty must be finite")
+        if not (_finite(frequency) and _finite(presence)):
+            raise ValueError("frequency_penalty and presence_penalty must be finite (as float32 numbers)")
         bias = []
         for t, b in (params.logit_bias or {}).items():
             b = float(b)
             if not 0 <= int(t) < vocab_size or int(t) != t:
                 raise ValueError(f"logit_bias: id {t} is outside the vocabulary (0..{vocab_size - 1})")
-            if math.isnan(b) or b == math.inf:
+            if math.isnan(b) or b == math.inf or not (b == -math.inf or _finite(b)):
                 raise ValueError(f"logit_bias: {b} for id {t} is not a number that a logit takes")
             if b != 0:
                 bias.append((int(t), b))
@@ -49,8 +54,8 @@ class LogitShaping:
         if frequency == 0 and presence == 0 and not bias and grammar is None:
             return None
         repeat = float(params.repeat_penalty)
-        if repeat == math.inf:
-            raise ValueError("repeat_penalty must be finite")
+        if repeat > 0 and not (_finite(repeat) and np.float32(repeat) > 0):
+            raise ValueError("repeat_penalty must be finite and no less than 2^-149 (as a float32 number)")
         return cls(repeat if repeat > 0 else 1.0, int(params.repeat_last_n) if params.repeat_last_n else 64, frequency, presence,
                    tuple(sorted(bias)), grammar)
 
