@@ -18,9 +18,18 @@
 // 44 us.  As CTAs of the prefix's kernel they ran one an SM: a CTA of a kernel that allocates tensor memory keeps others of it off its
 // SM until it has done so.)
 //
+// Rounding.  P is bfloat16 in front of V, below a maximum that may be an old one, and is summed as it is rounded.  Relative error of
+// the output against 64 bits, together / by the kernel for rows alone / of the output's own rounding (10^-3; 64 rows of 32 heads of 128 on 32
+// pages, scores of standard deviation 0.5, 1.5, 3, 6): 2.34 2.19 1.91 1.76 / 2.33 1.97 1.70 1.67 / 1.66 all; 16 rows on 512 pages 2.32 2.31 2.11
+// 1.82 / 2.30 2.09 1.71 1.66.  The kernel for rows alone has a weight of exactly 1 at the maximum so far, this one does not: summed
+// before rounding, that alone was up to 2.4 in steep rows (in a model of both in 64 bits; summed so, 1.8 to 1.9).  The sums as rounded cost nothing
+// (64 rows on 512 pages 62.1 us, now 61.7).
+//
 // What bounds it.  64 rows of 32 heads (8 kv heads of 128) on 512 pages, with up to 200 positions of their own: 62 us (each row by
-// itself 700), of which the prefix kernel takes 45 (a page and tile 1.4 us of a CTA, two CTAs an SM, 268 MB through L2 at 6.7 TB/s, in which
-// its products alone would take half), the rows' own pages behind it 6 more, the parts 5.  On 32 pages, with up to 500 positions of their
+// itself 700), of which the prefix kernel takes 45 (a page and tile 1.4 us of a CTA, two CTAs an SM; its products alone would take half), the
+// rows' own pages behind it 6 more, the parts 5.  Its two tiles ask for 268 MB of pages, of which 134 MB are different: 228 MB come from DRAM,
+// 467 MB are read in L2 (ncu, which counts what crosses from one half of L2 to the other twice), so neither is at its rate, and tiles
+// side by side, which brought DRAM to 136 MB, took as long.  On 32 pages, with up to 500 positions of their
 // own, 28 us (61): the own pages' 74 MB in 17 us (a CTA's beginning and end are worth three of its pages, of which it has one to eight),
 // the prefix kernel beside them for the first 10, the parts 3.
 // Tried and slower (us, of 64 rows on 32 and 512 pages, when this was 33 and 67): runs in clusters of eight that add up their parts in

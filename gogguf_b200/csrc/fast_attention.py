@@ -83,10 +83,14 @@ def shared_shares(n_tokens: int, nkv: int, own_pages: int) -> int:
 def prefix_pays(groups: Sequence[Tuple[int, int]], n_tokens: int, nkv: int) -> bool:
     """Is reading the prefixes of groups of (members, pages) once, in a step of n_tokens rows, quicker than every row for itself?  From
     12 pages of prefixes on that a CTA of the unshared kernel would read (measured, us, unshared / shared with two pages of a row's own,
-    32 heads of 128 on 8 kv heads: 2 rows, 8 pages a CTA 10.0 / 13.0, 16 15.4 / 15.1, 32 26 / 20; 8 rows, 8 10.6 / 12.3, 16 16.0 / 14.9;
-    32 rows, 16 15.8 / 17.3, 32 26 / 19; 64 rows, 14 20.8 / 18.5, 27 31 / 19; 16 heads of 64 on 8: 8 rows, 8 8.7 / 10.3, 16 14.1 / 11.8; 64
-    rows, 14 13.7 / 15.0; 24 heads of 80 on 4: 16 rows, 8 11.1 / 12.9, 16 16.6 / 14.1; sixteen heads a kv head gain sooner, 32 of 128 on
-    2: 64 rows, 8 20.4 / 16.3)."""
+    32 heads of 128 on 8 kv heads: 2 rows, 8 pages a CTA 10.0 / 12.7, 16 15.3 / 14.8, 32 26 / 20; 8 rows, 8 10.6 / 12.1, 16 16.0 / 14.7;
+    32 rows, 32 26 / 19; 64 rows, 14 20.9 / 18.1, 27 31 / 19; 16 heads of 64 on 8: 8 rows, 8 8.7 / 10.2, 16 14.1 / 11.5; 24 heads of 80 on
+    4: 16 rows, 8 11.2 / 12.7, 16 16.7 / 13.9).
+
+    It counts pages, neither head sizes nor the query heads of a kv head.  Of 168 measured calls it takes the slower form, by more
+    than 5 %, in six: with sixteen query heads a kv head sharing gains sooner (32 heads of 128 on 2, read apart: 64 rows, 16 pages shared
+    20.4 / 16.0, 8 17.4 / 15.4; 32 rows, 32 17.2 / 15.7); and around the bound (read together: 32 heads on 8, 32 rows, 16 pages 15.9 / 17.1;
+    16 heads of 64 on 8, 64 rows, 8 13.8 / 14.9; 2 rows, 128 11.6 / 12.3)."""
     pairs, splits = n_tokens * nkv, 1
     while splits * 2 <= min(8, 296 // pairs):
         splits *= 2
@@ -255,7 +259,10 @@ def attn_decode_shared(q, k_pool, v_pool, out, positions, seq_of_token, table, p
                        shares: Optional[int] = None) -> None:
     """Decode attention (`attn_decode_tma`, without windows and chunks) of the plan's token rows: the keys and values of a prefix
     that several rows share are read once for all of them, in three kernels, where that pays (`prefix_pays`; `together` True or
-    False decides instead).  scratch: float32, `shared_scratch` of it; two launches that may run at the same time need scratch of
+    False decides instead).  What is shared, the plan and the table are read before the kernel that was launched before this call has
+    ended (what other kernels and PyTorch wrote before that is there), so that one must not write to them; only a row's own positions
+    may be the kernel before's.  The pages hold finite numbers behind a row's newest position, too (a cache begins as zeros): their
+    weight is 0.  scratch: float32, `shared_scratch` of it; two launches that may run at the same time need scratch of
     their own.  runs: CTAs over the prefixes (default: `shared_runs`); shares: CTAs that share a row's own pages (default:
     `shared_shares`; `PrefixPlan.launch`)."""
     dv = d if dv is None else int(dv)
