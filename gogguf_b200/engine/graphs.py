@@ -46,6 +46,15 @@ class _Captured:
     turn: int = 0
 
 
+def _heads(parts):
+    for p in parts:
+        if getattr(p, "_fast", None) is not None and hasattr(p, "nkv"):
+            yield p.nq, p.nkv
+        members = getattr(p, "members", None)                              # (mixers side by side in one part)
+        if isinstance(members, list):
+            yield from _heads(m[0] for m in members if isinstance(m, tuple))
+
+
 class GraphStepper(Stepper):
     def __init__(self, model, cache, min_width: int = 16):
         super().__init__(model, cache)
@@ -56,7 +65,7 @@ class GraphStepper(Stepper):
         # such a model is stepped eagerly, and `decode_from_device` is not offered for it
         self.capturable = all(getattr(p, "capturable", True) for p in model.parts())
         # (query heads, kv heads) of the layers whose attention may read shared pages together
-        self._heads = sorted({(p.nq, p.nkv) for p in model.parts() if getattr(p, "_fast", None) is not None and hasattr(p, "nkv")})
+        self._heads = sorted(set(_heads(model.parts())))
 
     def _width_bucket(self, slots: Sequence[int]) -> int:
         w = max(self.cache.table_width(slots), self.min_width)
@@ -68,7 +77,9 @@ class GraphStepper(Stepper):
         key = []
         for g, gs in sorted(prefixes.groups.items()):
             weights, nkv = [(len(rows), pages) for rows, pages in gs], self.cache.groups[g].request.num_kv_heads
-            key.append((g,) + tuple(step_launch(weights, prefixes.own_pages, n_tokens, nq, n) for nq, n in self._heads if n == nkv))
+            launches = tuple(step_launch(weights, prefixes.own_pages, n_tokens, nq, n) for nq, n in self._heads if n == nkv)
+            # (of a part that does not say its heads, what its launches may depend on)
+            key.append((g,) + (launches or (sum(rows * pages for rows, pages in weights).bit_length(), prefixes.own_pages.bit_length())))
         return tuple(key)
 
     def _capture(self, entries: Sequence[StepEntry], bucket: int, width: int, prefixes=None) -> _Captured:

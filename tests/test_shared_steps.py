@@ -111,3 +111,21 @@ def test_layers_with_other_numbers_of_heads():
     assert a == o and a != b
     # 64 members are two tiles of 128 rows with four heads each, eight with sixteen: 192 and 768 pages of (tile, kv head), four a run
     assert A.step_launch([(64, 12)], 1, 64, 32, NKV)[0] == 64 and A.step_launch([(64, 12)], 1, 64, 128, NKV)[0] == A.SHARED_RUNS // 2
+
+
+def test_heads_inside_a_mixer_of_mixers_and_heads_that_are_not_known():
+    """Attention that stands beside other mixers in one part counts as any other; where no part says its heads, steps are told apart by
+    the weight of their groups and their own pages."""
+    c, slots = forks(64, 64 * 12)
+    flat = Recorded(c)
+    inner = types.SimpleNamespace(nq=NQ, nkv=NKV, _fast=object())
+    other = types.SimpleNamespace(_fast=object())
+    nested = Recorded(c)
+    nested.model.parts = lambda: iter([types.SimpleNamespace(members=[(other, 1.0, True), (inner, 0.5, None)]), other])
+    GraphStepper.__init__(nested, nested.model, c)
+    prefixes = flat.shared_prefixes(slots)
+    assert nested._heads == flat._heads == [(NQ, NKV)] and nested.prefix_key(prefixes, 64) == flat.prefix_key(prefixes, 64)
+    unknown = Recorded(c, heads=())
+    c2, slots2 = forks(64, 64 * 48)
+    few, many = unknown.prefix_key(prefixes, 64), Recorded(c2, heads=()).prefix_key(Recorded(c2).shared_prefixes(slots2), 64)
+    assert few != many
